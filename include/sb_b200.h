@@ -51,7 +51,14 @@ enum SbDeviceStatus {
                                 call then computes anything, and every row of the call's outputs
                                 is filled with NaN (where the reference raises on the host,
                                 sb_varlen/__init__.py:72-74)                                   */
-  SB_DEV_WAIT_TIMEOUT = 2    /* a bounded on-chip wait gave up; status[1] = which barrier      */
+  SB_DEV_WAIT_TIMEOUT = 2,   /* a bounded on-chip wait gave up; status[1] = which barrier      */
+  SB_DEV_BAD_PAGE = 3,       /* a page table names a page that the pool does not have, for a token that its
+                                sequence holds; status[1] = sequence.  The page is not touched        */
+  SB_DEV_BAD_SEQ_LEN = 4,    /* a sequence's length, or the length it would grow to, is negative or beyond its row of
+                                the page table; status[1] = sequence                                  */
+  SB_DEV_OUT_OF_PAGES = 5,   /* fewer free pages than the call needs; status[1] = how many it needs.  Nothing was changed */
+  SB_DEV_BAD_SEQUENCE = 6    /* an index of sb_kv_fork or sb_kv_free is no sequence, or one that the call cannot take;
+                                status[1] = the index.  Nothing was changed                           */
 };
 
 enum SbKernelPath {
@@ -220,10 +227,128 @@ SB_EXPORT int sb_fwd_static_scratch(const SbParams *p, void *stream);
  * counterpart: its backward keeps nothing but lock arrays (sb_varlen_bwd.py:568-573). */
 SB_EXPORT size_t sb_set_backward_scratch_budget(size_t bytes);
 
+/* ---- serving: a paged key-value cache, and attention of new tokens over it --------------------------------------
+ *
+ * The cache.  Keys and values live in pools of pages; a page holds `page_size` consecutive tokens of one sequence, for all
+ * key heads: (layers, pages, kv_heads, page_size, head_dim) with a unit stride on head_dim and any positive strides on the
+ * other axes (so (pages, page_size, kv_heads, head_dim) is a matter of strides).  `page_table` row b lists the pages of
+ * sequence b in the order of its tokens, `seq_lens[b]` is its length.  Entries behind the last page in use are not read.
+ * Lengths and tables stay on the device; no call looks at them on the host.  The reference has no cache: its operators
+ * attend over whole sequences (sb_varlen/__init__.py:24-82).                                                           */
+typedef struct SbCache {
+  void *ptr;            /* element (0, 0, 0, 0, 0)                           */
+  int64_t stride_layer; /* element strides; sb_attn_decode and sb_kv_append take one layer and do not use the first */
+  int64_t stride_page;
+  int64_t stride_h;
+  int64_t stride_t;
+} SbCache;
+
+/* Stick-breaking attention of the newest `new_tokens` tokens of every sequence over its cache, which already holds them:
+ * query t of sequence b has position seq_lens[b] - new_tokens + t and attends to the keys before it (attend_current: up to
+ * it).  A query whose position is negative, or that has no key, gets o = 0, rem = 1 (a padded batch).  Query head h reads key
+ * head h / (heads / kv_heads).  A sequence whose length is refused gets NaN (SB_DEV_BAD_SEQ_LEN); so does what a refused
+ * page would have gone into (SB_DEV_BAD_PAGE).  Keys behind the point where the stick of all query rows that are computed together is
+ * used up (weights exactly 0 in fp32) are not visited, unless flags has SB_FLAG_DENSE_ROW_PASS; a value that is not finite
+ * is only seen by rows that visit it.  Same call, same bits: the order of every sum depends on the shapes and lengths alone. */
+typedef struct SbDecodeParams {
+  int32_t struct_bytes;   /* = sizeof(SbDecodeParams)                                        */
+  int32_t dtype;          /* SbDtype of q, o, rem and the cache                              */
+  int32_t batch;          /* sequences                                                       */
+  int32_t heads;          /* query heads, a multiple of kv_heads                             */
+  int32_t kv_heads;
+  int32_t new_tokens;     /* queries per sequence, 1..1024                                   */
+  int32_t head_dim;       /* 1..256                                                          */
+  int32_t page_size;
+  int32_t num_pages;
+  int32_t max_pages;      /* entries of a row of page_table                                  */
+  int32_t attend_current;
+  float logit_scale;
+  int32_t flags;          /* SB_FLAG_FORCE_SIMT, SB_FLAG_DENSE_ROW_PASS                      */
+  int32_t reserved;       /* must be 0                                                       */
+  SbTensor q, o;          /* (batch, heads, new_tokens, head_dim)                            */
+  void *rem;              /* out: (batch, heads, new_tokens) contiguous                      */
+  SbCache k, v;           /* one layer                                                       */
+  const int32_t *page_table;
+  int64_t page_table_stride;
+  const int32_t *seq_lens;
+  void *workspace;        /* sb_attn_decode_workspace_bytes() bytes, 256-byte aligned; nothing is kept in it */
+  size_t workspace_bytes;
+  int32_t *status;        /* as in SbParams                                                  */
+} SbDecodeParams;
+
+/* Scratch of sb_attn_decode for these shapes, on the current device; (size_t)-1 for invalid parameters. */
+SB_EXPORT size_t sb_attn_decode_workspace_bytes(const SbDecodeParams *p);
+SB_EXPORT int sb_attn_decode(const SbDecodeParams *p, void *stream);
+/* An SbKernelPath: SB_PATH_TCGEN05 stands for the tensor-core kernel here too (mma.sync); -1 if invalid. */
+SB_EXPORT int sb_attn_decode_path(const SbDecodeParams *p);
+
+/* Writes new keys and values (batch, kv_heads, tokens, head_dim) into the pages of one layer: token t of sequence b, of n, to
+ * position seq_lens[b] - n + t.  With cu_seqlens the tokens are packed (batch 1), n differs by sequence, and tokens behind the
+ * last end belong to none; without it n = tokens for every sequence.  Tokens whose position is negative are left out (a
+ * padded batch).  A refused cu_seqlens (SB_DEV_BAD_CU_SEQLENS): nothing is written.  No two sequences may hold the page that a
+ * token goes to. */
+typedef struct SbAppendParams {
+  int32_t struct_bytes;   /* = sizeof(SbAppendParams)                                        */
+  int32_t dtype;
+  int32_t num_seq;        /* rows of page_table, entries of seq_lens and of cu_seqlens       */
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t num_pages;
+  int32_t max_pages;
+  int32_t cu_seqlens_int64;
+  int32_t flags;          /* SB_FLAG_CHECK_LEADING_ZERO                                      */
+  int64_t tokens;         /* of every sequence; packed: of all                               */
+  const void *cu_seqlens; /* num_seq END offsets, or NULL                                    */
+  SbTensor k, v;          /* in                                                              */
+  SbCache k_cache, v_cache;
+  const int32_t *page_table;
+  int64_t page_table_stride;
+  const int32_t *seq_lens;
+  int32_t *status;
+} SbAppendParams;
+SB_EXPORT int sb_kv_append(const SbAppendParams *p, void *stream);
+
+/* The keeping of the pages.  `page_refs[page]` is the number of sequences that hold a page, 0 for a free one; page tables and
+ * lengths as above, an empty sequence having length 0.  Pages are given out lowest first, in the order of sequences (or listed
+ * pairs) and positions.  A call that cannot do all it is asked to changes nothing and sets the status word.  Only the last
+ * page of a sequence can be partly filled, and no two sequences share one that is. */
+typedef struct SbPagesParams {
+  int32_t struct_bytes;   /* = sizeof(SbPagesParams)                                         */
+  int32_t max_seqs;       /* rows of page_table, entries of seq_lens                         */
+  int32_t max_pages;
+  int32_t num_pages;      /* up to 1 << 20                                                   */
+  int32_t page_size;
+  int32_t n;              /* entries of `first` (and `second`)                               */
+  int32_t count;          /* sb_kv_extend without `first`: new tokens of every sequence that is not empty */
+  int32_t dtype, layers, kv_heads, head_dim; /* sb_kv_fork, sb_kv_compact                    */
+  int32_t reserved;       /* must be 0                                                       */
+  int32_t *page_table;
+  int64_t page_table_stride;
+  int32_t *seq_lens, *page_refs;
+  const int32_t *first;   /* extend: new tokens per sequence (max_seqs of them) or NULL; fork: sources; free: sequences */
+  const int32_t *second;  /* fork: destinations                                              */
+  SbCache k_cache, v_cache; /* sb_kv_fork, sb_kv_compact: all layers                         */
+  void *workspace;        /* sb_kv_pages_workspace_bytes() bytes, 256-byte aligned; nothing is kept in it */
+  size_t workspace_bytes;
+  int32_t *status;
+} SbPagesParams;
+SB_EXPORT size_t sb_kv_pages_workspace_bytes(const SbPagesParams *p);
+/* Room for new tokens: lengths grow by `first` (or `count`), and rows get the pages they lack. */
+SB_EXPORT int sb_kv_extend(const SbPagesParams *p, void *stream);
+/* second[i], an empty sequence, becomes a copy of first[i]: full pages are shared, the tokens of a last page that is not full
+ * are copied to a page of its own, all layers.  A sequence may be forked several times in a call but not be a fork in it. */
+SB_EXPORT int sb_kv_fork(const SbPagesParams *p, void *stream);
+/* The listed sequences give their pages back and are empty; one that is empty, or listed twice, is no error. */
+SB_EXPORT int sb_kv_free(const SbPagesParams *p, void *stream);
+/* Moves the pages in use to the front of the pool: with N of them, the r-th one at or behind N goes to the r-th free one before
+ * N, all layers, and the tables follow.  Pages that have become free keep what they held. */
+SB_EXPORT int sb_kv_compact(const SbPagesParams *p, void *stream);
+
 /* Which kernels sb_fwd / sb_bwd run for these parameters (an SbKernelPath), or -1 if invalid. */
 SB_EXPORT int sb_kernel_path(const SbParams *p);
 
-/* Number of kernel launches the last sb_fwd / sb_bwd call of this thread enqueued. */
+/* Number of kernel launches the last enqueuing call of this thread (sb_fwd, sb_bwd, sb_attn_decode, sb_kv_*) made. */
 SB_EXPORT int sb_last_launch_count(void);
 
 /* Text of the last error returned to this thread ("" if none). */

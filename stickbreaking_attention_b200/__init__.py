@@ -17,10 +17,12 @@ from .ops import (check_status, dense_row_pass, force_simt, kernel_launches, ker
                   small_backward_workspace)
 from .sb_attn import sb_attn, sb_attn_fused  # noqa: E402
 from .sb_varlen import sb_attn_varlen, sb_attn_varlen_fused  # noqa: E402
+from .sb_decode import sb_attn_decode  # noqa: E402
+from .kv_cache import PagedKVCache, kv_append, kv_compact, kv_extend, kv_fork, kv_free  # noqa: E402
 
 __all__ = ["sb_attn", "sb_attn_varlen", "sb_attn_fused", "sb_attn_varlen_fused", "check_status", "force_simt",
            "small_backward_workspace", "dense_row_pass", "set_backward_scratch_budget", "kernel_launches", "kernel_path", "install_as_dropin",
-           "ops"]
+           "ops", "sb_attn_decode", "PagedKVCache", "kv_append", "kv_extend", "kv_fork", "kv_free", "kv_compact"]
 
 
 def install_as_dropin(name: str = "stickbreaking_attention") -> None:

@@ -24,9 +24,15 @@ SB_DEV_MESSAGES = {
     1: "cu_seqlens is invalid (not non-decreasing, beyond the token count, longer than max_seqlens, "
        "or without its leading zero); offending sequence index: {0}",
     2: "a bounded on-chip wait timed out in barrier {0}",
+    3: "a page table names a page that the cache does not have; sequence: {0}",
+    4: "a sequence's length, or the length it would grow to, is negative or beyond its row of the page table; sequence: {0}",
+    5: "the cache has too few free pages: {0} needed; nothing was changed",
+    6: "listed sequence {0} is none, or one that the call cannot take; nothing was changed",
 }
 EXPORTS = ("sb_workspace_bytes", "sb_fwd", "sb_bwd", "sb_fwd_static_scratch", "sb_set_backward_scratch_budget",
-           "sb_kernel_path", "sb_last_launch_count", "sb_last_error", "sb_abi_version")
+           "sb_kernel_path", "sb_last_launch_count", "sb_last_error", "sb_abi_version", "sb_attn_decode_workspace_bytes",
+           "sb_attn_decode", "sb_attn_decode_path", "sb_kv_append", "sb_kv_pages_workspace_bytes", "sb_kv_extend", "sb_kv_fork",
+           "sb_kv_free", "sb_kv_compact")
 ABI_VERSION = 2
 
 
@@ -49,6 +55,39 @@ class SbParams(ctypes.Structure):
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("status", ctypes.c_void_p),
         ("attn_weights", ctypes.c_void_p), ("attn_cols", ctypes.c_int64),
         ("tile_start", ctypes.c_void_p), ("tile_start_stride", ctypes.c_int64),
+    ]
+
+
+class SbCache(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("stride_layer", ctypes.c_int64), ("stride_page", ctypes.c_int64),
+                ("stride_h", ctypes.c_int64), ("stride_t", ctypes.c_int64)]
+
+
+class SbDecodeParams(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("struct_bytes", "dtype", "batch", "heads", "kv_heads", "new_tokens", "head_dim",
+                                                    "page_size", "num_pages", "max_pages", "attend_current")] + [
+        ("logit_scale", ctypes.c_float), ("flags", ctypes.c_int32), ("reserved", ctypes.c_int32), ("q", SbTensor), ("o", SbTensor),
+        ("rem", ctypes.c_void_p), ("k", SbCache), ("v", SbCache), ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64), ("seq_lens", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t), ("status", ctypes.c_void_p),
+    ]
+
+
+class SbAppendParams(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("struct_bytes", "dtype", "num_seq", "kv_heads", "head_dim", "page_size",
+                                                    "num_pages", "max_pages", "cu_seqlens_int64", "flags")] + [
+        ("tokens", ctypes.c_int64), ("cu_seqlens", ctypes.c_void_p), ("k", SbTensor), ("v", SbTensor), ("k_cache", SbCache),
+        ("v_cache", SbCache), ("page_table", ctypes.c_void_p), ("page_table_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p), ("status", ctypes.c_void_p),
+    ]
+
+
+class SbPagesParams(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("struct_bytes", "max_seqs", "max_pages", "num_pages", "page_size", "n", "count",
+                                                    "dtype", "layers", "kv_heads", "head_dim", "reserved")] + [
+        ("page_table", ctypes.c_void_p), ("page_table_stride", ctypes.c_int64), ("seq_lens", ctypes.c_void_p),
+        ("page_refs", ctypes.c_void_p), ("first", ctypes.c_void_p), ("second", ctypes.c_void_p), ("k_cache", SbCache),
+        ("v_cache", SbCache), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("status", ctypes.c_void_p),
     ]
 
 
@@ -81,6 +120,15 @@ def load(path: str | None = None) -> ctypes.CDLL:
     lib.sb_last_error.restype = ctypes.c_char_p
     lib.sb_set_backward_scratch_budget.restype = ctypes.c_size_t
     lib.sb_set_backward_scratch_budget.argtypes = [ctypes.c_size_t]
+    lib.sb_attn_decode_workspace_bytes.restype = lib.sb_kv_pages_workspace_bytes.restype = ctypes.c_size_t
+    lib.sb_attn_decode_workspace_bytes.argtypes = [ctypes.POINTER(SbDecodeParams)]
+    lib.sb_attn_decode_path.argtypes = [ctypes.POINTER(SbDecodeParams)]
+    lib.sb_kv_pages_workspace_bytes.argtypes = [ctypes.POINTER(SbPagesParams)]
+    for name, params in (("sb_attn_decode", SbDecodeParams), ("sb_kv_append", SbAppendParams), ("sb_kv_extend", SbPagesParams),
+                         ("sb_kv_fork", SbPagesParams), ("sb_kv_free", SbPagesParams), ("sb_kv_compact", SbPagesParams)):
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(params), ctypes.c_void_p]
     lib.sb_abi_version.restype = ctypes.c_int
     if lib.sb_abi_version() != ABI_VERSION:
         raise SbError(f"{path}: ABI version {lib.sb_abi_version()} but this binding speaks {ABI_VERSION}; "

@@ -13,7 +13,13 @@ namespace sb {
 static thread_local char g_err[512] = "";
 static thread_local int g_launches = 0;
 
-static int fail(int code, const char *fmt, ...) {
+int *begin_call() {
+  g_err[0] = 0;
+  g_launches = 0;
+  return &g_launches;
+}
+
+int fail(int code, const char *fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -153,7 +159,7 @@ static TensorRef ref_of(const SbTensor &t) {
   return TensorRef{reinterpret_cast<char *>(t.ptr), (long long)t.stride_b, (long long)t.stride_h, (long long)t.stride_t};
 }
 
-static int device_ok() {
+int device_ok() {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return fail(SB_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));

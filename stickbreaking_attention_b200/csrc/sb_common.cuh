@@ -359,6 +359,12 @@ inline cudaError_t launch_kernel(void (*kernel)(Params...), dim3 grid, int threa
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Of every C entry point: the thread's error text and launch count start over (the count's address); an error's code and text;
+// whether the current device can run the kernels.
+int *begin_call();
+int fail(int code, const char *fmt, ...);
+int device_ok();
+
 // Host-side launch helpers implemented in the .cu files; all return cudaError_t of the launch.
 cudaError_t launch_fused_drem(const KParams &p, int dtype, cudaStream_t s);   // fills d_rem_fused (all heads)
 cudaError_t launch_fused_dv(const KParams &p, int dtype, cudaStream_t s);     // dv += rem * d_out (all heads)

@@ -1,0 +1,526 @@
+// The pages of a key-value cache: new keys and values written into them, and their keeping (room for new tokens, forks, freed
+// sequences, compaction) with the tables on the device, so that a serving step needs no host synchronisation and can be captured.
+//
+// Which page a sequence gets is a rule, not a race: the lowest free pages (count 0), in the order of sequences and positions.
+// An operator that cannot do all it is asked to (too few pages, an index that is none) changes nothing and says so in the
+// status word.
+#include "sb_pages.cuh"
+
+#include <algorithm>
+#include <initializer_list>
+
+namespace sb {
+
+namespace {
+
+// ---- append -------------------------------------------------------------------------------------------------------------
+// Memory-bound: every new row read and written once.  A block looks up where its tokens go (sequence, page, slot), then its
+// threads copy 16 bytes at a time, all heads of a token, keys and values, kDeep of them in flight per thread.
+constexpr int kAppendThreads = 256, kMaxTokens = 64;
+
+__device__ __forceinline__ long long append_end(const AppendParams &p, int i) {
+  return p.cu64 ? reinterpret_cast<const long long *>(p.cu)[i] : (long long)reinterpret_cast<const int *>(p.cu)[i];
+}
+__device__ __forceinline__ void report(int *status, int code, int which) {
+  if (status != nullptr) {
+    status[0] = code;
+    status[1] = which;
+  }
+}
+
+template <typename V>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
+  __shared__ long long src[kMaxTokens], dst[kMaxTokens];   // elements; of the keys' tensors, and of the values' in the loop
+  __shared__ long long vsrc[kMaxTokens], vdst[kMaxTokens];
+  enter_kernel<true>();
+  if (p.cu != nullptr) {
+    bool bad = false;
+    for (int i = threadIdx.x; i < p.num_seq; i += kAppendThreads) {
+      const long long start = i == 0 ? 0 : append_end(p, i - 1), end = append_end(p, i);
+      if (start < 0 || end < start || end > p.tokens) {
+        bad = true;
+        if (blockIdx.x == 0) report(p.status, SB_DEV_BAD_CU_SEQLENS, i);
+      }
+    }
+    if (p.check_leading_zero && threadIdx.x == 0 && append_end(p, -1) != 0) {
+      bad = true;
+      if (blockIdx.x == 0) report(p.status, SB_DEV_BAD_CU_SEQLENS, -1);
+    }
+    if (__syncthreads_or(bad)) return;
+  }
+  const long long all = p.cu != nullptr ? p.tokens : p.tokens * p.num_seq;
+  const long long t0 = (long long)blockIdx.x * p.per_block;
+  const int count = (int)min((long long)p.per_block, all - t0);
+  if ((int)threadIdx.x < count) {
+    const long long token = t0 + threadIdx.x;
+    long long seq, back, from = token;        // back: how many tokens of the sequence follow, with this one
+    if (p.cu != nullptr) {
+      int lo = 0, hi = p.num_seq;             // the first sequence that ends behind the token
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (append_end(p, mid) > token) hi = mid;
+        else lo = mid + 1;
+      }
+      seq = lo;
+      back = lo < p.num_seq ? append_end(p, lo) - token : 0;
+    } else {
+      seq = token / p.tokens;
+      from = token - seq * p.tokens;
+      back = p.tokens - from;
+    }
+    long long to = -1;
+    if (back > 0) {
+      const int len = p.seq_lens[seq];
+      const long long pos = len - back;
+      if (len < 0 || len > (long long)p.max_pages * p.page_size) report(p.status, SB_DEV_BAD_SEQ_LEN, (int)seq);
+      else if (pos >= 0) {
+        const int index = (int)(pos / p.page_size), page = p.page_table[seq * p.table_stride + index];
+        if ((unsigned)page >= (unsigned)p.num_pages) report(p.status, SB_DEV_BAD_PAGE, (int)seq);
+        else {
+          const int slot = (int)(pos - (long long)index * p.page_size);
+          to = page * p.kc.sp + slot * p.kc.st;
+          vdst[threadIdx.x] = page * p.vc.sp + slot * p.vc.st;
+        }
+      }
+    }
+    const long long b = p.cu != nullptr ? 0 : seq;
+    src[threadIdx.x] = b * p.k.sb + from * p.k.st;
+    vsrc[threadIdx.x] = b * p.v.sb + from * p.v.st;
+    dst[threadIdx.x] = to;
+  }
+  __syncthreads();
+  const int per_row = p.head_dim * p.esize / (int)sizeof(V);
+  const int per_token = 2 * p.kv_heads * per_row, work = count * per_token;
+  constexpr int kDeep = 4;
+  for (int e0 = threadIdx.x; e0 < work; e0 += kDeep * kAppendThreads) {
+    V x[kDeep];
+    V *to[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int e = e0 + i * kAppendThreads;
+      to[i] = nullptr;
+      if (e < work) {
+        const int t = e / per_token, in = e - t * per_token, row = in / per_row, c = in - row * per_row;
+        const bool val = row >= p.kv_heads;
+        const int h = val ? row - p.kv_heads : row;
+        if (dst[t] >= 0) {
+          const TensorRef &s = val ? p.v : p.k;
+          const CacheRef &d = val ? p.vc : p.kc;
+          x[i] = reinterpret_cast<const V *>(s.ptr + ((val ? vsrc[t] : src[t]) + h * s.sh) * p.esize)[c];
+          to[i] = reinterpret_cast<V *>(d.ptr + ((val ? vdst[t] : dst[t]) + h * d.sh) * p.esize) + c;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+      if (to[i] != nullptr) *to[i] = x[i];
+  }
+}
+
+// ---- the keeping of the pages ----------------------------------------------------------------------------------------------
+// One block decides what happens (which pages go where), many carry it out.  The deciding block reads the counts of all pages,
+// 16 per thread at a time.
+constexpr int kBookThreads = 1024, kPer = 16;
+
+// Exclusive prefix sum over the block's threads; total in `all`.  shared: 33 ints.  Contains barriers.
+__device__ __forceinline__ int block_scan(int x, int *shared, int &all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int sum = x;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += other;
+  }
+  __syncthreads();
+  if (lane == 31) shared[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    const int own = shared[lane];
+    int s = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += other;
+    }
+    shared[lane] = s - own;
+    if (lane == 31) shared[32] = s;
+  }
+  __syncthreads();
+  all = shared[32];
+  return shared[warp] + sum - x;
+}
+
+// The counts of the pages [first, first + kPer); -1 behind the last page.
+__device__ __forceinline__ void read_refs(const PagesParams &p, int first, int (&x)[kPer]) {
+  if (first + kPer <= p.num_pages && reinterpret_cast<uintptr_t>(p.refs) % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4) {
+      const int4 v = *reinterpret_cast<const int4 *>(p.refs + first + i);
+      x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] = first + i < p.num_pages ? p.refs[first + i] : -1;
+  }
+}
+
+// The `want` lowest free pages, into list; false if there are fewer.
+__device__ __forceinline__ bool list_free(const PagesParams &p, int want, int *list, int *shared) {
+  int found = 0;
+  for (int base = 0; base < p.num_pages && found < want; base += kBookThreads * kPer) {
+    const int first = base + threadIdx.x * kPer;
+    int x[kPer], mine = 0, all;
+    read_refs(p, first, x);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) mine += x[i] == 0;
+    int rank = found + block_scan(mine, shared, all);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (x[i] == 0) {
+        if (rank < want) list[rank] = first + i;
+        ++rank;
+      }
+    found += all;
+  }
+  __syncthreads();
+  return found >= want;
+}
+
+__device__ __forceinline__ bool length_ok(const PagesParams &p, long long len) {
+  return len >= 0 && len <= (long long)p.max_pages * p.page_size;
+}
+__device__ __forceinline__ int pages_for(const PagesParams &p, int len) { return (int)(((long long)len + p.page_size - 1) / p.page_size); }
+
+// New tokens of sequence b.
+__device__ __forceinline__ int extra(const PagesParams &p, int b, int len) { return p.a != nullptr ? p.a[b] : len > 0 ? p.count : 0; }
+
+__global__ void __launch_bounds__(kBookThreads) extend_kernel(const __grid_constant__ PagesParams p) {
+  __shared__ int shared[33];
+  enter_kernel<true>();
+  int *list = p.work + kPagesHeader, *prefix = list + p.num_pages;
+  int want = 0;
+  bool bad = false;
+  for (int base = 0; base < p.max_seqs; base += kBookThreads) {
+    const int b = base + threadIdx.x;
+    int need = 0;
+    if (b < p.max_seqs) {
+      const int len = p.seq_lens[b], more = extra(p, b, len);
+      if (more < 0 || !length_ok(p, len) || !length_ok(p, (long long)len + more)) {
+        bad = true;
+        report(p.status, SB_DEV_BAD_SEQ_LEN, b);
+      } else {
+        need = min(pages_for(p, len + more) - pages_for(p, len), p.num_pages + 1);
+      }
+    }
+    int all;
+    const int before = block_scan(need, shared, all);
+    // (a sum beyond the pool is refused below; kept from wrapping here)
+    if (b < p.max_seqs) prefix[b] = want + before;
+    want = min(want + all, p.num_pages + 1);
+  }
+  if (__syncthreads_or(bad)) return;
+  if (want > 0 && !list_free(p, want, list, shared)) {
+    if (threadIdx.x == 0) report(p.status, SB_DEV_OUT_OF_PAGES, want);
+    return;
+  }
+  for (int r = threadIdx.x; r < want; r += kBookThreads) {
+    int lo = 0, hi = p.max_seqs;              // the last sequence whose pages begin at or before r
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (prefix[mid] <= r) lo = mid;
+      else hi = mid;
+    }
+    const int page = list[r];
+    p.page_table[lo * p.table_stride + pages_for(p, p.seq_lens[lo]) + r - prefix[lo]] = page;
+    p.refs[page] = 1;
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < p.max_seqs; b += kBookThreads) {
+    const int len = p.seq_lens[b], more = extra(p, b, len);
+    if (more > 0) p.seq_lens[b] = len + more;
+  }
+}
+
+// A block per entry.  An entry that is listed twice is freed once: whoever takes a page out of the table counts it down.
+constexpr int kFreeThreads = 128;
+__global__ void __launch_bounds__(kFreeThreads) free_kernel(const __grid_constant__ PagesParams p) {
+  enter_kernel<true>();
+  bool bad = false;
+  for (int i = threadIdx.x; i < p.n; i += kFreeThreads)
+    if ((unsigned)p.a[i] >= (unsigned)p.max_seqs) {
+      bad = true;
+      if (blockIdx.x == 0) report(p.status, SB_DEV_BAD_SEQUENCE, p.a[i]);
+    }
+  if (__syncthreads_or(bad)) return;
+  const int b = p.a[blockIdx.x], len = *reinterpret_cast<volatile int *>(p.seq_lens + b);
+  const int pages = length_ok(p, len) ? pages_for(p, len) : 0;
+  for (int i = threadIdx.x; i < pages; i += kFreeThreads) {
+    const int page = atomicExch(p.page_table + b * p.table_stride + i, -1);
+    if ((unsigned)page < (unsigned)p.num_pages) atomicSub(p.refs + page, 1);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) p.seq_lens[b] = 0;
+}
+
+// Copies `bytes` from one place to another, a block's share of it.
+template <typename V> __device__ __forceinline__ void copy_share(char *to, const char *from, long long count, long long start, long long step) {
+  constexpr int kDeep = 4;
+  const V *s = reinterpret_cast<const V *>(from);
+  V *d = reinterpret_cast<V *>(to);
+  for (long long e0 = start; e0 < count; e0 += kDeep * step) {
+    V x[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+      if (e0 + i * step < count) x[i] = s[e0 + i * step];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+      if (e0 + i * step < count) d[e0 + i * step] = x[i];
+  }
+}
+
+// The first `rows` slots of page `from` to page `to`: all heads of one layer's keys or values, by the block.
+template <typename V>
+__device__ __forceinline__ void copy_page(const PagesParams &p, const CacheRef &c, int layer, int from, int to, int rows) {
+  const char *src = c.ptr + layer * c.sl + from * c.sp;
+  char *dst = c.ptr + layer * c.sl + to * c.sp;
+  const int per_row = p.row_bytes / (int)sizeof(V);
+  const bool dense = c.st == p.row_bytes;
+  if (dense && rows == p.page_size && c.sh == (long long)p.row_bytes * p.page_size) {
+    copy_share<V>(dst, src, (long long)p.heads * rows * per_row, threadIdx.x, blockDim.x);
+    return;
+  }
+  constexpr int kDeep = 4;
+  const int per_head = rows * per_row, work = p.heads * per_head;
+  for (int e0 = threadIdx.x; e0 < work; e0 += kDeep * (int)blockDim.x) {
+    V x[kDeep];
+    long long at[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int e = e0 + i * (int)blockDim.x;
+      at[i] = -1;
+      if (e < work) {
+        const int h = e / per_head, in = e - h * per_head, r = in / per_row, col = in - r * per_row;
+        at[i] = h * c.sh + r * c.st + col * (int)sizeof(V);
+        x[i] = *reinterpret_cast<const V *>(src + at[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+      if (at[i] >= 0) *reinterpret_cast<V *>(dst + at[i]) = x[i];
+  }
+}
+
+// header of `work`: [0] whether there is something to carry out, [1] pages to move, [2] live pages
+// fork: behind the lists, for each pair the source's length and the page that its copied rows get (or -1)
+__device__ __forceinline__ int *fork_plan(const PagesParams &p) { return p.work + kPagesHeader + 2 * p.num_pages + p.max_seqs; }
+
+__global__ void __launch_bounds__(kBookThreads) fork_plan_kernel(const __grid_constant__ PagesParams p) {
+  __shared__ int shared[33];
+  enter_kernel<true>();
+  int *list = p.work + kPagesHeader, *mark = list + 2 * p.num_pages, *plan = fork_plan(p);
+  if (threadIdx.x == 0) p.work[0] = 0;
+  for (int i = threadIdx.x; i < p.max_seqs; i += kBookThreads) mark[i] = 0;
+  __syncthreads();
+  bool bad = false;
+  for (int i = threadIdx.x; i < p.n; i += kBookThreads) {
+    const int s = p.a[i], d = p.b[i];
+    int wrong = -1;
+    if ((unsigned)s >= (unsigned)p.max_seqs) wrong = s;
+    else if ((unsigned)d >= (unsigned)p.max_seqs || p.seq_lens[d] != 0 || atomicExch(mark + d, 1) != 0) wrong = d;
+    else if (!length_ok(p, p.seq_lens[s])) wrong = s;
+    else continue;
+    bad = true;
+    report(p.status, SB_DEV_BAD_SEQUENCE, wrong);
+  }
+  if (__syncthreads_or(bad)) return;
+  for (int i = threadIdx.x; i < p.n; i += kBookThreads)
+    if (mark[p.a[i]] != 0) {                  // a sequence cannot be forked and be a fork in one call
+      bad = true;
+      report(p.status, SB_DEV_BAD_SEQUENCE, p.a[i]);
+    }
+  if (__syncthreads_or(bad)) return;
+  int want = 0;
+  for (int base = 0; base < p.n; base += kBookThreads) {
+    const int i = base + threadIdx.x;
+    int len = 0;
+    if (i < p.n) len = p.seq_lens[p.a[i]];
+    const int need = len % p.page_size != 0;
+    int all;
+    const int rank = want + block_scan(need, shared, all);
+    if (i < p.n) {
+      plan[2 * i] = len;
+      plan[2 * i + 1] = need ? rank : -1;
+    }
+    want += all;
+  }
+  if (want > p.num_pages || !list_free(p, want, list, shared)) {
+    if (threadIdx.x == 0) report(p.status, SB_DEV_OUT_OF_PAGES, want);
+    return;
+  }
+  for (int i = threadIdx.x; i < p.n; i += kBookThreads) {
+    const int rank = plan[2 * i + 1];
+    if (rank >= 0) {
+      plan[2 * i + 1] = list[rank];
+      p.refs[list[rank]] = 1;
+    }
+    p.seq_lens[p.b[i]] = plan[2 * i];
+  }
+  if (threadIdx.x == 0) p.work[0] = 1;
+}
+
+// Blocks (pair, part): the parts of a pair are its layers' keys and values, and first its row of the table.
+constexpr int kCopyThreads = 256;
+template <typename V>
+__global__ void __launch_bounds__(kCopyThreads) fork_kernel(const __grid_constant__ PagesParams p) {
+  enter_kernel<true>();
+  if (p.work[0] == 0) return;
+  const int pair = blockIdx.y, part = blockIdx.x;
+  const int *plan = fork_plan(p);
+  const int len = plan[2 * pair], fresh = plan[2 * pair + 1], full = len / p.page_size, rest = len - full * p.page_size;
+  const int *from = p.page_table + p.a[pair] * p.table_stride;
+  int *to = p.page_table + p.b[pair] * p.table_stride;
+  if (part == 0) {
+    for (int i = threadIdx.x; i < full; i += kCopyThreads) {
+      const int page = from[i];
+      if ((unsigned)page < (unsigned)p.num_pages) atomicAdd(p.refs + page, 1);
+      else report(p.status, SB_DEV_BAD_PAGE, p.a[pair]);
+      to[i] = page;
+    }
+    if (threadIdx.x == 0 && rest > 0) to[full] = fresh;
+    return;
+  }
+  if (rest == 0) return;
+  const int old = from[full];
+  if ((unsigned)old >= (unsigned)p.num_pages) {
+    report(p.status, SB_DEV_BAD_PAGE, p.a[pair]);
+    return;
+  }
+  const int layer = (part - 1) >> 1;
+  copy_page<V>(p, (part - 1) & 1 ? p.v : p.k, layer, old, fresh, rest);
+}
+
+__global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid_constant__ PagesParams p) {
+  __shared__ int shared[33];
+  enter_kernel<true>();
+  int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;    // (hole, page) pairs, no more than half the pages; new place of each
+  int live = 0, mine = 0;
+  for (int base = 0; base < p.num_pages; base += kBookThreads * kPer) {
+    int x[kPer];
+    read_refs(p, base + threadIdx.x * kPer, x);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) mine += x[i] > 0;
+  }
+  block_scan(mine, shared, live);
+  int holes = 0, moved = 0;
+  for (int base = 0; base < p.num_pages; base += kBookThreads * kPer) {
+    const int first = base + threadIdx.x * kPer;
+    int x[kPer], h = 0, m = 0, all_h, all_m;
+    read_refs(p, first, x);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      h += first + i < live && x[i] == 0;
+      m += first + i >= live && x[i] > 0;
+    }
+    int rank_h = holes + block_scan(h, shared, all_h), rank_m = moved + block_scan(m, shared, all_m);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (first + i < live && x[i] == 0) pairs[2 * rank_h++] = first + i;
+      if (first + i >= live && x[i] > 0) pairs[2 * rank_m++ + 1] = first + i;
+    }
+    holes += all_h;
+    moved += all_m;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < moved; r += kBookThreads) {
+    const int to = pairs[2 * r], from = pairs[2 * r + 1];
+    place[from] = to;
+    p.refs[to] = p.refs[from];
+    p.refs[from] = 0;
+  }
+  if (threadIdx.x == 0) {
+    p.work[1] = moved;
+    p.work[2] = live;
+  }
+}
+
+// Blocks below copy_blocks copy the moved pages, a (page, layer, keys or values) at a time; the others rewrite the tables.
+template <typename V>
+__global__ void __launch_bounds__(kCopyThreads) compact_kernel(const __grid_constant__ PagesParams p, int copy_blocks) {
+  enter_kernel<true>();
+  const int moved = p.work[1], live = p.work[2];
+  const int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;
+  if ((int)blockIdx.x < copy_blocks) {
+    const long long jobs = (long long)moved * p.layers * 2;
+    for (long long j = blockIdx.x; j < jobs; j += copy_blocks) {
+      const int r = (int)(j / (2 * p.layers)), part = (int)(j - (long long)r * 2 * p.layers);
+      copy_page<V>(p, part & 1 ? p.v : p.k, part >> 1, pairs[2 * r + 1], pairs[2 * r], p.page_size);
+    }
+    return;
+  }
+  if (moved == 0) return;
+  for (int b = blockIdx.x - copy_blocks; b < p.max_seqs; b += gridDim.x - copy_blocks) {
+    const int len = p.seq_lens[b], pages = length_ok(p, len) ? pages_for(p, len) : 0;
+    int *row = p.page_table + b * p.table_stride;
+    for (int i = threadIdx.x; i < pages; i += kCopyThreads) {
+      const int page = row[i];
+      if ((unsigned)page >= (unsigned)p.num_pages) report(p.status, SB_DEV_BAD_PAGE, b);
+      else if (page >= live) row[i] = place[page];
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_append(const AppendParams &p, cudaStream_t s) {
+  const long long all = p.cu != nullptr ? p.tokens : p.tokens * p.num_seq;
+  AppendParams q = p;
+  int sms = 0;
+  const cudaError_t e = sm_count(&sms);
+  if (e != cudaSuccess) return e;
+  q.per_block = (int)std::min<long long>(kMaxTokens, std::max<long long>(1, all / (8 * sms)));
+  const dim3 grid((unsigned)((all + q.per_block - 1) / q.per_block));
+  auto aligned = [&](const char *ptr, std::initializer_list<long long> strides) {
+    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0) return false;
+    for (long long x : strides)
+      if (x * p.esize % 16 != 0) return false;
+    return true;
+  };
+  if (p.head_dim * p.esize % 16 == 0 && aligned(p.k.ptr, {p.k.sb, p.k.sh, p.k.st}) && aligned(p.v.ptr, {p.v.sb, p.v.sh, p.v.st}) &&
+      aligned(p.kc.ptr, {p.kc.sp, p.kc.sh, p.kc.st}) && aligned(p.vc.ptr, {p.vc.sp, p.vc.sh, p.vc.st}))
+    return launch_kernel(append_kernel<uint4>, grid, kAppendThreads, 0, s, q);
+  if (p.esize == 4) return launch_kernel(append_kernel<uint32_t>, grid, kAppendThreads, 0, s, q);
+  return launch_kernel(append_kernel<unsigned short>, grid, kAppendThreads, 0, s, q);
+}
+
+cudaError_t launch_extend(const PagesParams &p, cudaStream_t s) { return launch_kernel(extend_kernel, dim3(1), kBookThreads, 0, s, p); }
+
+cudaError_t launch_free(const PagesParams &p, cudaStream_t s) { return launch_kernel(free_kernel, dim3(p.n), kFreeThreads, 0, s, p); }
+
+cudaError_t launch_fork(const PagesParams &p, cudaStream_t s, int *launches) {
+  cudaError_t e = launch_kernel(fork_plan_kernel, dim3(1), kBookThreads, 0, s, p);
+  if (e != cudaSuccess) return e;
+  *launches += 2;
+  const dim3 grid(1 + 2 * p.layers, p.n);
+  switch (p.vec) {
+    case 16: return launch_kernel(fork_kernel<uint4>, grid, kCopyThreads, 0, s, p);
+    case 4: return launch_kernel(fork_kernel<uint32_t>, grid, kCopyThreads, 0, s, p);
+    default: return launch_kernel(fork_kernel<unsigned short>, grid, kCopyThreads, 0, s, p);
+  }
+}
+
+cudaError_t launch_compact(const PagesParams &p, cudaStream_t s, int *launches) {
+  int sms = 0;
+  cudaError_t e = sm_count(&sms);
+  if (e != cudaSuccess) return e;
+  if ((e = launch_kernel(compact_plan_kernel, dim3(1), kBookThreads, 0, s, p)) != cudaSuccess) return e;
+  *launches += 2;
+  const int copy_blocks = 8 * sms, table_blocks = std::min(p.max_seqs, sms);
+  const dim3 grid(copy_blocks + table_blocks);
+  switch (p.vec) {
+    case 16: return launch_kernel(compact_kernel<uint4>, grid, kCopyThreads, 0, s, p, copy_blocks);
+    case 4: return launch_kernel(compact_kernel<uint32_t>, grid, kCopyThreads, 0, s, p, copy_blocks);
+    default: return launch_kernel(compact_kernel<unsigned short>, grid, kCopyThreads, 0, s, p, copy_blocks);
+  }
+}
+
+}  // namespace sb

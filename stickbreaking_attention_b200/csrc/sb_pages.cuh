@@ -1,0 +1,54 @@
+// Keys and values in the pages of a cache, and the keeping of the pages: what the kernels and their host side share.
+#pragma once
+
+#include "sb_common.cuh"
+
+namespace sb {
+
+// Keys or values of a cache: (layers, pages, heads, slots, head_dim), in units of `vec` bytes (16, or one element).
+struct CacheRef {
+  char *ptr;
+  long long sl, sp, sh, st;
+};
+
+struct AppendParams {
+  TensorRef k, v;                  // (batch, heads, tokens, head_dim); packed: batch 1
+  CacheRef kc, vc;                 // strides in elements
+  const int *page_table;
+  long long table_stride;
+  const int *seq_lens;
+  const void *cu;                  // packed: num_seq sequence ends; null: every sequence has `tokens` new tokens
+  int cu64, check_leading_zero;
+  int num_seq, kv_heads, head_dim, page_size, num_pages, max_pages, esize;
+  long long tokens;                // of a sequence; packed: of all
+  int per_block;                   // tokens of a block
+  int *status;
+};
+
+// The tables of a pool: which pages a sequence has, how long it is, how many sequences have a page.
+struct PagesParams {
+  int *page_table;
+  long long table_stride;
+  int *seq_lens, *refs;
+  int max_seqs, max_pages, num_pages, page_size;
+  const int *a, *b;                // extend: counts (or null); fork: sources, destinations; free: sequences
+  int n, count;                    // entries of a and b; extend without counts: new tokens of every sequence that has some
+  CacheRef k, v;                   // fork, compact: strides in bytes
+  int layers, heads, row_bytes, vec;
+  int *work;                       // see work_ints
+  int *status;
+};
+
+// Scratch of the keeping operators, in ints: header, then one entry per page twice, one per sequence and pair each.
+constexpr int kPagesHeader = 16;
+inline long long pages_work_ints(long long num_pages, long long max_seqs, long long n) {
+  return kPagesHeader + 2 * num_pages + max_seqs + 2 * n + 64;
+}
+
+cudaError_t launch_append(const AppendParams &p, cudaStream_t s);
+cudaError_t launch_extend(const PagesParams &p, cudaStream_t s);
+cudaError_t launch_fork(const PagesParams &p, cudaStream_t s, int *launches);
+cudaError_t launch_free(const PagesParams &p, cudaStream_t s);
+cudaError_t launch_compact(const PagesParams &p, cudaStream_t s, int *launches);
+
+}  // namespace sb

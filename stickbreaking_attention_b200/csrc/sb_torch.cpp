@@ -353,6 +353,242 @@ std::tuple<Tensor, Tensor, Tensor> backward(const Tensor &dout, const std::optio
   return {g[0], g[1], g[2]};
 }
 
+// ---- serving: a paged key-value cache and attention over it ------------------------------------------------------------
+
+void refuse_grad(const char *what, std::initializer_list<const Tensor *> ts) {
+  for (const Tensor *t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t->requires_grad()) && !t->_fw_grad(0).defined(), what,
+                                " has no derivative: call it under torch.no_grad(), or detach its inputs");
+}
+// What the call wrote to: a backward that saved it earlier has to notice.
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void check_int32(const Tensor &t, int64_t dim, const char *name, const Tensor &like) {
+  TORCH_CHECK_VALUE(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == dim, name,
+                    " must be a ", dim == 1 ? "1-D" : "2-D", " int32 tensor on the device of the cache");
+  TORCH_CHECK_VALUE(t.size(dim - 1) <= 1 || t.stride(dim - 1) == 1, name, " must be contiguous in its last axis");
+}
+void check_table(const Tensor &table, const Tensor &lens, const Tensor &like) {
+  check_int32(table, 2, "page_table", like);
+  check_int32(lens, 1, "seq_lens", like);
+  TORCH_CHECK_VALUE(table.size(0) == lens.size(0), "page_table must have a row for each entry of seq_lens");
+}
+// Pools of keys and values: (pages, kv_heads, page_size, head_dim), with the layers before that where `layers`.
+void check_pools(const Tensor &k, const Tensor &v, bool layers) {
+  TORCH_CHECK_VALUE(k.is_cuda(), "the cache must be on a CUDA device (no CPU path)");
+  dtype_code(k.scalar_type());
+  TORCH_CHECK_VALUE(k.scalar_type() == v.scalar_type() && k.device() == v.device() && k.sizes() == v.sizes(),
+                    "the caches of keys and values must share dtype, device and shape");
+  TORCH_CHECK_VALUE(k.dim() == 4 || (layers && k.dim() == 5), "expected a cache of shape (", layers ? "[layers,] " : "",
+                    "pages, kv_heads, page_size, head_dim)");
+  TORCH_CHECK_VALUE(k.size(-1) <= 1 || (k.stride(-1) == 1 && v.stride(-1) == 1), "the cache must be contiguous in head_dim");
+}
+int64_t stride_of(const Tensor &t, int64_t axis) { return t.size(axis) == 1 ? 0 : t.stride(axis); }
+SbCache cache_arg(const Tensor &t) {
+  const int64_t a = t.dim() - 4;
+  return SbCache{t.data_ptr(), a ? stride_of(t, 0) : 0, stride_of(t, a), stride_of(t, a + 1), stride_of(t, a + 2)};
+}
+SbTensor rows_arg(const Tensor &t) {   // (batch, heads, tokens, d), or packed (heads, tokens, d)
+  const int64_t a = t.dim() - 3;
+  return SbTensor{t.data_ptr(), a ? stride_of(t, 0) : 0, stride_of(t, a), stride_of(t, a + 1)};
+}
+int32_t to_int32(int64_t x, const char *name) {
+  TORCH_CHECK_VALUE(x >= 0 && x <= 0x7fffffff, name, " ", std::to_string(x), " is out of range");
+  return (int32_t)x;
+}
+void count_launches(const char *what, int rc) {
+  if (rc != SB_OK) raise_library_error(what, rc);
+  g_launches.fetch_add(sb_last_launch_count(), std::memory_order_relaxed);
+}
+void *stream_of(const Tensor &t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+std::tuple<Tensor, Tensor> decode(const Tensor &q_in, const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &lens,
+                                  double scale, bool attend_current, int64_t flags) {
+  refuse_grad("sb_attn_decode", {&q_in, &k, &v});
+  at::AutoDispatchBelowADInplaceOrView below;
+  check_pools(k, v, false);
+  TORCH_CHECK_VALUE(q_in.device() == k.device() && q_in.scalar_type() == k.scalar_type(), "q must share the cache's device and dtype");
+  TORCH_CHECK_VALUE(q_in.dim() == 4, "expected q of shape (batch, heads, new_tokens, head_dim)");
+  TORCH_CHECK_VALUE(q_in.size(3) == k.size(3), "q and the cache must share head_dim");
+  check_table(table, lens, k);
+  TORCH_CHECK_VALUE(lens.size(0) == q_in.size(0), "seq_lens must have an entry for each sequence of q");
+  c10::cuda::CUDAGuard guard(k.device());
+  const Tensor q = q_in.size(3) <= 1 || q_in.stride(3) == 1 ? q_in : q_in.contiguous();
+  const Tensor o = empty_as(q), rem = empty_cuda(q.sizes().slice(0, 3), q.scalar_type(), q);
+  SbDecodeParams p;
+  memset(&p, 0, sizeof(p));
+  p.struct_bytes = (int32_t)sizeof(p);
+  p.dtype = dtype_code(q.scalar_type());
+  p.batch = to_int32(q.size(0), "batch");
+  p.heads = to_int32(q.size(1), "heads");
+  p.new_tokens = to_int32(q.size(2), "new_tokens");
+  p.head_dim = to_int32(q.size(3), "head_dim");
+  p.num_pages = to_int32(k.size(0), "pages");
+  p.kv_heads = to_int32(k.size(1), "kv_heads");
+  p.page_size = to_int32(k.size(2), "page_size");
+  p.max_pages = to_int32(table.size(1), "pages per sequence");
+  p.attend_current = attend_current;
+  p.logit_scale = (float)scale;
+  p.flags = (int32_t)(flags & (SB_FLAG_FORCE_SIMT | SB_FLAG_DENSE_ROW_PASS));
+  p.q = rows_arg(q);
+  p.o = rows_arg(o);
+  p.rem = rem.data_ptr();
+  p.k = cache_arg(k);
+  p.v = cache_arg(v);
+  p.page_table = static_cast<const int32_t *>(table.data_ptr());
+  p.page_table_stride = table.stride(0);
+  p.seq_lens = static_cast<const int32_t *>(lens.data_ptr());
+  p.status = status_ptr(k.get_device());
+  const size_t need = sb_attn_decode_workspace_bytes(&p);
+  if (need == (size_t)-1) raise_library_error("sb_attn_decode", -1);
+  const Tensor scratch = empty_cuda({(int64_t)need}, at::kByte, k);
+  p.workspace = scratch.data_ptr();
+  p.workspace_bytes = need;
+  count_launches("sb_attn_decode", sb_attn_decode(&p, stream_of(k)));
+  return {o, rem};
+}
+
+void append(const Tensor &k_in, const Tensor &v_in, const Tensor &k_pages, const Tensor &v_pages, const Tensor &table,
+            const Tensor &lens, const std::optional<Tensor> &cu, bool leading_zero) {
+  refuse_grad("kv_append", {&k_in, &v_in, &k_pages, &v_pages});
+  at::AutoDispatchBelowADInplaceOrView below;
+  check_pools(k_pages, v_pages, false);
+  TORCH_CHECK_VALUE(k_in.scalar_type() == k_pages.scalar_type() && v_in.scalar_type() == k_pages.scalar_type() &&
+                        k_in.device() == k_pages.device() && v_in.device() == k_pages.device(),
+                    "k and v must share the cache's dtype and device");
+  TORCH_CHECK_VALUE(k_in.sizes() == v_in.sizes() && k_in.dim() == (cu.has_value() ? 3 : 4),
+                    "expected k and v of shape (batch, kv_heads, tokens, head_dim), or (kv_heads, tokens, head_dim) with cu_seqlens");
+  TORCH_CHECK_VALUE(k_in.size(-1) == k_pages.size(3) && k_in.size(-3) == k_pages.size(1), "k, v and the cache must share kv_heads and head_dim");
+  check_table(table, lens, k_pages);
+  c10::cuda::CUDAGuard guard(k_pages.device());
+  const bool unit = k_in.size(-1) <= 1;
+  const Tensor k = unit || k_in.stride(-1) == 1 ? k_in : k_in.contiguous(), v = unit || v_in.stride(-1) == 1 ? v_in : v_in.contiguous();
+  SbAppendParams p;
+  memset(&p, 0, sizeof(p));
+  p.struct_bytes = (int32_t)sizeof(p);
+  p.dtype = dtype_code(k.scalar_type());
+  p.num_seq = to_int32(lens.size(0), "sequences");
+  p.tokens = k.size(-2);
+  if (cu.has_value()) {
+    TORCH_CHECK_VALUE(cu->is_cuda() && cu->dim() == 1 && cu->device() == k.device() &&
+                          (cu->scalar_type() == at::kInt || cu->scalar_type() == at::kLong) && (cu->numel() <= 1 || cu->stride(0) == 1),
+                      "cu_seqlens must be a contiguous 1-D int32 or int64 tensor on the device of the cache");
+    TORCH_CHECK_VALUE(cu->numel() == lens.size(0) + leading_zero, "cu_seqlens must have an end for each entry of seq_lens",
+                      leading_zero ? " behind its leading zero" : "");
+    p.cu_seqlens = static_cast<const char *>(cu->data_ptr()) + (leading_zero ? cu->element_size() : 0);
+    p.cu_seqlens_int64 = cu->scalar_type() == at::kLong;
+    p.flags = leading_zero ? SB_FLAG_CHECK_LEADING_ZERO : 0;
+  } else {
+    TORCH_CHECK_VALUE(k.size(0) == lens.size(0), "seq_lens must have an entry for each sequence of k and v");
+  }
+  p.num_pages = to_int32(k_pages.size(0), "pages");
+  p.kv_heads = to_int32(k_pages.size(1), "kv_heads");
+  p.page_size = to_int32(k_pages.size(2), "page_size");
+  p.head_dim = to_int32(k_pages.size(3), "head_dim");
+  p.max_pages = to_int32(table.size(1), "pages per sequence");
+  p.k = rows_arg(k);
+  p.v = rows_arg(v);
+  p.k_cache = cache_arg(k_pages);
+  p.v_cache = cache_arg(v_pages);
+  p.page_table = static_cast<const int32_t *>(table.data_ptr());
+  p.page_table_stride = table.stride(0);
+  p.seq_lens = static_cast<const int32_t *>(lens.data_ptr());
+  p.status = status_ptr(k_pages.get_device());
+  count_launches("sb_kv_append", sb_kv_append(&p, stream_of(k_pages)));
+  written(k_pages);
+  written(v_pages);
+}
+
+SbPagesParams pages_params(const Tensor &table, const Tensor &lens, const Tensor &refs, int64_t page_size) {
+  TORCH_CHECK_VALUE(table.is_cuda(), "the page tables must be on a CUDA device (no CPU path)");
+  check_table(table, lens, table);
+  check_int32(refs, 1, "page_refs", table);
+  SbPagesParams p;
+  memset(&p, 0, sizeof(p));
+  p.struct_bytes = (int32_t)sizeof(p);
+  p.max_seqs = to_int32(table.size(0), "sequences");
+  p.max_pages = to_int32(table.size(1), "pages per sequence");
+  p.num_pages = to_int32(refs.size(0), "pages");
+  p.page_size = to_int32(page_size, "page_size");
+  p.page_table = static_cast<int32_t *>(table.data_ptr());
+  p.page_table_stride = table.stride(0);
+  p.seq_lens = static_cast<int32_t *>(lens.data_ptr());
+  p.page_refs = static_cast<int32_t *>(refs.data_ptr());
+  p.status = status_ptr(table.get_device());
+  return p;
+}
+void set_pools(SbPagesParams &p, const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &refs) {
+  refuse_grad("the keeping of a cache's pages", {&k, &v});
+  check_pools(k, v, true);
+  TORCH_CHECK_VALUE(k.device() == table.device(), "page_table must be on the device of the cache");
+  TORCH_CHECK_VALUE(k.size(-4) == refs.size(0), "page_refs must have an entry for each page of the cache");
+  p.dtype = dtype_code(k.scalar_type());
+  p.layers = k.dim() == 5 ? to_int32(k.size(0), "layers") : 1;
+  p.kv_heads = to_int32(k.size(-3), "kv_heads");
+  p.head_dim = to_int32(k.size(-1), "head_dim");
+  p.k_cache = cache_arg(k);
+  p.v_cache = cache_arg(v);
+}
+void listed(const Tensor &t, const char *name, const Tensor &table) {
+  check_int32(t, 1, name, table);
+}
+void run_pages(SbPagesParams &p, int (*call)(const SbPagesParams *, void *), const char *what, const Tensor &table, bool scratch_needed) {
+  c10::cuda::CUDAGuard guard(table.device());
+  Tensor scratch;
+  if (scratch_needed) {
+    const size_t need = sb_kv_pages_workspace_bytes(&p);
+    if (need == (size_t)-1) raise_library_error(what, -1);
+    scratch = empty_cuda({(int64_t)need}, at::kByte, table);
+    p.workspace = scratch.data_ptr();
+    p.workspace_bytes = need;
+  }
+  count_launches(what, call(&p, stream_of(table)));
+}
+
+void kv_extend(const Tensor &table, const Tensor &lens, const Tensor &refs, const std::optional<Tensor> &counts, int64_t count,
+               int64_t page_size) {
+  SbPagesParams p = pages_params(table, lens, refs, page_size);
+  if (counts.has_value()) {
+    listed(*counts, "counts", table);
+    TORCH_CHECK_VALUE(counts->size(0) == lens.size(0), "counts must have an entry for each entry of seq_lens");
+    p.first = static_cast<const int32_t *>(counts->data_ptr());
+  } else {
+    p.count = to_int32(count, "counts");
+  }
+  run_pages(p, sb_kv_extend, "sb_kv_extend", table, true);
+  for (const Tensor *t : {&table, &lens, &refs}) written(*t);
+}
+void kv_fork(const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &lens, const Tensor &refs, const Tensor &src,
+             const Tensor &dst) {
+  check_pools(k, v, true);
+  SbPagesParams p = pages_params(table, lens, refs, k.size(-2));
+  set_pools(p, k, v, table, refs);
+  listed(src, "src", table);
+  listed(dst, "dst", table);
+  TORCH_CHECK_VALUE(src.size(0) == dst.size(0), "src and dst must have the same number of entries");
+  p.n = to_int32(src.size(0), "listed sequences");
+  p.first = static_cast<const int32_t *>(src.data_ptr());
+  p.second = static_cast<const int32_t *>(dst.data_ptr());
+  run_pages(p, sb_kv_fork, "sb_kv_fork", table, true);
+  for (const Tensor *t : {&k, &v, &table, &lens, &refs}) written(*t);
+}
+void kv_free(const Tensor &table, const Tensor &lens, const Tensor &refs, const Tensor &seqs, int64_t page_size) {
+  SbPagesParams p = pages_params(table, lens, refs, page_size);
+  listed(seqs, "seqs", table);
+  p.n = to_int32(seqs.size(0), "listed sequences");
+  p.first = static_cast<const int32_t *>(seqs.data_ptr());
+  run_pages(p, sb_kv_free, "sb_kv_free", table, false);
+  for (const Tensor *t : {&table, &lens, &refs}) written(*t);
+}
+void kv_compact(const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &lens, const Tensor &refs) {
+  check_pools(k, v, true);
+  SbPagesParams p = pages_params(table, lens, refs, k.size(-2));
+  set_pools(p, k, v, table, refs);
+  run_pages(p, sb_kv_compact, "sb_kv_compact", table, true);
+  for (const Tensor *t : {&k, &v, &table, &lens, &refs}) written(*t);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_sb_torch, m) {
@@ -366,6 +602,12 @@ PYBIND11_MODULE(_sb_torch, m) {
   m.def("attention", &attention, py::call_guard<py::gil_scoped_release>());
   m.def("forward", &forward, py::call_guard<py::gil_scoped_release>());
   m.def("backward", &backward, py::call_guard<py::gil_scoped_release>());
+  m.def("decode", &decode, py::call_guard<py::gil_scoped_release>());
+  m.def("append", &append, py::call_guard<py::gil_scoped_release>());
+  m.def("kv_extend", &kv_extend, py::call_guard<py::gil_scoped_release>());
+  m.def("kv_fork", &kv_fork, py::call_guard<py::gil_scoped_release>());
+  m.def("kv_free", &kv_free, py::call_guard<py::gil_scoped_release>());
+  m.def("kv_compact", &kv_compact, py::call_guard<py::gil_scoped_release>());
   m.def("tma_ready", &tma_ready);
   m.def("status_word", &status_word, py::call_guard<py::gil_scoped_release>());
   m.def("launches", [] { return g_launches.load(); });

@@ -458,3 +458,22 @@ def kernel_path(q, fixed: bool = False) -> int:
     _fill(prm, fixed=fixed, q=q, k=q, v=q, cu_seqlens=dummy_cu, max_seqlens=None, logit_scale=1.0,
           attend_current=False, leading_zero=False)
     return _cabi.load().sb_kernel_path(prm)
+
+
+# ---- serving operators, as torch.compile sees them -------------------------------------------------
+
+@torch.library.custom_op(f"{NAMESPACE}::decode", mutates_args=(), device_types="cuda")
+def decode_op(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+              logit_scale: float, attend_current: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return _sb_torch.decode(q, k_pages, v_pages, page_table, seq_lens, logit_scale, attend_current, switch_flags())
+
+
+@decode_op.register_fake
+def _(q, k_pages, v_pages, page_table, seq_lens, logit_scale, attend_current):
+    return torch.empty_like(q), q.new_empty(q.shape[:3])
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv_append", mutates_args={"k_pages", "v_pages"}, device_types="cuda")
+def append_op(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+              seq_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor], zero_start: bool) -> None:
+    _sb_torch.append(k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, zero_start and cu_seqlens is not None)
