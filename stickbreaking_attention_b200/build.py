@@ -23,7 +23,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libsb_b200.so")
 EXT_PATH = os.path.join(PKG_DIR, "_sb_torch.so")
 EXT_SOURCE = "sb_torch.cpp"
 SOURCES = ("sb_api.cu", "sb_simt.cu", "sb_tc.cu", "sb_tc_fwd256.cu", "sb_tc_fwd128.cu", "sb_tc_bwd.cu",
-           "sb_serve.cu", "sb_decode.cu", "sb_pages.cu")
+           "sb_serve.cu", "sb_decode.cu", "sb_decode_tc.cu", "sb_pages.cu")
 HEADERS = ("sb_common.cuh", "sb_ptx.cuh", "sb_tc_common.cuh", "sb_tc_fwd_rows.cuh", "sb_decode.cuh", "sb_pages.cuh", "../../include/sb_b200.h")
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

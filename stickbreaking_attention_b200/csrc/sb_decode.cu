@@ -9,12 +9,6 @@ namespace {
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool take) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool take) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int n> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
-
 constexpr int kTileKeys = 16, kStages = 3;
 
 // kCols: columns a lane holds (32 kCols >= head_dim); kRows: query rows (1, 2, 4, 8).
@@ -94,7 +88,7 @@ template <typename T, int kCols, int kRows> struct SimtWarp {
   double left[kPairs];
   int limit[kPairs];
 
-  __device__ __forceinline__ void tile(const DecodeParams &p, const float *stage, int key0) {
+  __device__ __forceinline__ void tile(const DecodeParams &p, const Piece &w, const float *stage, int key0) {
     using S = SimtShape<kCols>;
     const int lane = threadIdx.x & 31;
     const float *ks = stage + (kCols == 2 ? 2 : 4) * lane, *vs = ks + kTileKeys * S::kWidth;
@@ -145,15 +139,18 @@ template <typename T, int kCols, int kRows> struct SimtWarp {
       a[pr] = in ? expf((fminf(x, 0.0f) - l1) + ((float)left[pr] + later)) : 0.0f;
       left[pr] += (double)__shfl_sync(0xffffffffu, sum, lane & 1);
     }
+    // a value that a row does not attend to is left out, not multiplied by 0: it may be no number
+    const bool edge = key0 + kTileKeys > w.edge;
 #pragma unroll
     for (int j = 0; j < kTileKeys; ++j) {
       float v[kCols];
       load_cols<kCols>(vs + j * S::kWidth, v);
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        const float w = __shfl_sync(0xffffffffu, a[r / 2], 2 * j + (r & 1));
+        const float weight = __shfl_sync(0xffffffffu, a[r / 2], 2 * j + (r & 1));
+        if (edge && key0 + j >= __shfl_sync(0xffffffffu, limit[r / 2], r & 1)) continue;
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) acc[r][i] = fmaf(w, v[i], acc[r][i]);
+        for (int i = 0; i < kCols; ++i) acc[r][i] = fmaf(weight, v[i], acc[r][i]);
       }
     }
   }
@@ -215,7 +212,7 @@ __global__ void __launch_bounds__(SimtShape<kCols>::kWarps * 32, 1) decode_simt_
       const int ahead = t - (kStages - 1), into = at_stage == 0 ? kStages - 1 : at_stage - 1;
       if (ahead >= t0) bad |= load_stage<T, kCols>(p, w, w.k0 + ahead * kTileKeys, w.k1, stages + into * S::kStage, vec);
       cp_async_commit();
-      sum.tile(p, stages + at_stage * S::kStage, w.k0 + t * kTileKeys);
+      sum.tile(p, w, stages + at_stage * S::kStage, w.k0 + t * kTileKeys);
       at_stage = at_stage == kStages - 1 ? 0 : at_stage + 1;
       if (!p.dense) {
         bool gone = true;
@@ -225,10 +222,6 @@ __global__ void __launch_bounds__(SimtShape<kCols>::kWarps * 32, 1) decode_simt_
       }
     }
     cp_async_wait<0>();
-    if (w.bad && threadIdx.x == 0 && p.status != nullptr) {
-      p.status[0] = SB_DEV_BAD_SEQ_LEN;
-      p.status[1] = w.seq;
-    }
     __syncthreads();
     // the warps' sums: each into its own stages' memory, [rows][width], then joined
     if (bad || w.bad) {
@@ -246,28 +239,7 @@ __global__ void __launch_bounds__(SimtShape<kCols>::kWarps * 32, 1) decode_simt_
       if (lane < 2 && 2 * pr + lane < kRows)
         left_of[warp][2 * pr + lane] = bad || w.bad ? __int_as_float(0x7fffffff) : (float)(sum.left[pr] * kLog2eD);
     __syncthreads();
-    for (int e = threadIdx.x; e < w.rows * p.head_dim; e += kThreads) {
-      const int r = e / p.head_dim, c = e - r * p.head_dim;
-      float o = 0.0f, left = 0.0f;
-      for (int n = 0; n < S::kWarps; ++n) {
-        const float stick = exp2f(left);
-        if (stick == 0.0f) break;
-        o += stick * ring[n * kStages * S::kStage + r * S::kWidth + c];
-        left += left_of[n][r];
-      }
-      if (w.slot < 0)
-        reinterpret_cast<T *>(p.o.ptr)[row_offset(p, p.o, w, r) + c] = from_f32<T>(o);
-      else
-        p.part_o[((long long)w.slot * p.rows_per_block + r) * p.head_dim + c] = o;
-    }
-    if (threadIdx.x < w.rows) {
-      float left = 0.0f;
-      for (int n = 0; n < S::kWarps; ++n) left += left_of[n][threadIdx.x];
-      if (w.slot < 0)
-        reinterpret_cast<T *>(p.rem)[rem_index(p, w, threadIdx.x)] = from_f32<T>(exp2f(left));
-      else
-        p.part_l[(long long)w.slot * p.rows_per_block + threadIdx.x] = left;
-    }
+    finish_piece<T, kThreads, S::kWarps, kRows>(p, w, ring, kStages * S::kStage, S::kWidth, 1.0f, left_of);
     __syncthreads();
   }
 }

@@ -102,6 +102,7 @@ __device__ __forceinline__ Place find_place(const DecodeParams &p, int chunk_ind
 // One block's part of one item: keys [k0, k1) for the query rows [row0, row0 + rows) of key head `head`.
 struct Piece {
   int seq, head, row0, rows, keys, k0, k1;
+  int edge;               // some row does not attend to the keys from here on (k1 and more if there is no such row)
   int slot;               // where it is left for the join kernel, -1: it is the whole item
   bool bad;               // the sequence's length was refused
 };
@@ -119,8 +120,12 @@ __device__ __forceinline__ int next_piece(const DecodeParams &p, const Place &at
   w.head = item / p.row_blocks;
   w.row0 = (item - w.head * p.row_blocks) * p.rows_per_block;
   w.rows = min(p.rows - w.row0, p.rows_per_block);
+  // the first and the last token among the rows: what none of them attends to is not read, what some do not is looked at per row
+  const int tok = w.row0 % p.new_tokens, last = tok + w.rows - 1;
+  const int high = min(last, p.new_tokens - 1), low = last >= p.new_tokens ? 0 : tok;
   w.k0 = u0 * kUnit;
-  w.k1 = min((u0 + count) * kUnit, w.keys);
+  w.k1 = max(min((u0 + count) * kUnit, w.keys - (p.new_tokens - 1 - high)), w.k0);
+  w.edge = w.keys - (p.new_tokens - 1 - low);
   const bool whole = u0 == 0 && count == n;
   w.slot = whole ? -1 : 2 * chunk_index + (u0 > 0 && unit == begin ? 0 : 1);
   return count;
@@ -146,8 +151,50 @@ __device__ __forceinline__ int page_of(const DecodeParams &p, int seq, int index
   return -1;
 }
 
+// The epilogue of a piece, by all threads of the block behind a barrier: joins the warps' sums (warp 0 has the newest keys),
+// warp n's at sums + n * warp_stride as [rows][width] times `unscale`, and writes the result or leaves it for the join kernel.
+template <typename T, int kThreads, int kWarps, int kRows>
+__device__ __forceinline__ void finish_piece(const DecodeParams &p, const Piece &w, const float *sums, int warp_stride, int width,
+                                             float unscale, const float (&left_of)[kWarps][kRows]) {
+  for (int e = threadIdx.x; e < w.rows * p.head_dim; e += kThreads) {
+    const int r = e / p.head_dim, c = e - r * p.head_dim;
+    float o = 0.0f, left = 0.0f;
+    for (int n = 0; n < kWarps; ++n) {
+      const float stick = exp2f(left);
+      if (stick == 0.0f) break;
+      o += stick * sums[n * warp_stride + r * width + c];
+      left += left_of[n][r];
+    }
+    o *= unscale;
+    if (w.slot < 0)
+      reinterpret_cast<T *>(p.o.ptr)[row_offset(p, p.o, w, r) + c] = from_f32<T>(o);
+    else
+      p.part_o[((long long)w.slot * p.rows_per_block + r) * p.head_dim + c] = o;
+  }
+  for (int r = threadIdx.x; r < w.rows; r += kThreads) {
+    float left = 0.0f;
+    for (int n = 0; n < kWarps; ++n) left += left_of[n][r];
+    if (w.slot < 0)
+      reinterpret_cast<T *>(p.rem)[rem_index(p, w, r)] = from_f32<T>(exp2f(left));
+    else
+      p.part_l[(long long)w.slot * p.rows_per_block + r] = left;
+  }
+  if (w.bad && threadIdx.x == 0 && p.status != nullptr) {
+    p.status[0] = SB_DEV_BAD_SEQ_LEN;
+    p.status[1] = w.seq;
+  }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int n> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
+
 cudaError_t launch_decode_simt(const DecodeParams &p, int dtype, cudaStream_t s);
 cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s);
+cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s);
+int decode_tc_rows(int rows, int head_dim);
 int decode_simt_rows(int rows, int head_dim);   // query rows per item
 
 }  // namespace sb

@@ -1,0 +1,387 @@
+// Attention of new tokens over a paged key-value cache, tensor-core kernel: bf16 and fp16, rows of whole 16-byte chunks.
+//
+// What bounds it: every key and value is read once from HBM and takes part in 4 * rows operations per element, `rows` (query
+// heads per key head times new tokens) being 1 to 16 here: 1 to 16 operations per byte, where the GPU's ratio is 250.  So the
+// kernel is built around the copies: each warp has a ring of 16-key stages of its own, filled with cp.async, and no barrier
+// with other warps inside a piece; 192 KiB of stages per SM keep more bytes in flight than the latency of HBM needs (some 50 KiB).
+//
+// The products are mma.sync ones with the keys as the rows of the tile: S^T = K Q^T, O^T = V^T P^T, 16 keys by 8 queries.  A
+// tcgen05 tile takes 64 or 128 rows of one operand from shared memory that whole warps have to hand over; with 8 queries it
+// would be no less empty, and the products are not what takes the time.
+//
+// Row m of the score tile is key 2 m for m < 8, key 2 (m - 8) + 1 otherwise: a thread then holds two neighbouring keys of
+// two queries, and the sums over later keys take four shuffles per query.  Base 2 throughout:
+//   x = s log2(e) <q, k>,  u = 2^-|x|,  l = log2(1 + u);  log2 beta = min(x, 0) - l,  log2(1 - beta) = -max(x, 0) - l.
+// l comes from the series 2 atanh(u / (2 + u)) = 2 (w + w^3 / 3 + w^5 / 5 + ...), to 2^-22 of itself also where u is small: what
+// thousands of keys break off adds up.
+//
+// P enters the second product as the sum of two 16-bit numbers (16 or 22 bits): rounded once it would double the error that the
+// output's own rounding makes, and the second product of the pair is free.  In fp16 it is scaled by 2^15, since a weight of 1e-5
+// has few bits left there.  Scores, sums and the output's accumulators are 32-bit, the stick between tiles 64-bit.
+#include "sb_decode.cuh"
+#include "sb_ptx.cuh"
+
+namespace sb {
+
+namespace {
+
+using ptx::ex2;
+using ptx::rcp;
+using ptx::smem_u32;
+
+constexpr int kTileKeys = 16;
+
+template <int kD> struct TcShape {                                  // kD: head_dim rounded up to 64, 128, 256
+  static constexpr int kChunks = kD / 8;                            // 16-byte chunks of a row
+  static constexpr int kHalf = kTileKeys * kD * 2;                  // bytes of a stage's keys (or values)
+  static constexpr int kStage = 2 * kHalf;
+  static constexpr int kWarps = kD <= 128 ? 8 : 4;
+  static constexpr int kStages = kD <= 64 ? 6 : 3;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kBytes = kWarps * kStages * kStage;          // 192 KiB
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+template <typename T> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <typename T> __device__ __forceinline__ float2 unpack(uint32_t x);
+template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t x) {
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
+template <typename T> constexpr float kScaleP = 1.0f;
+template <> constexpr float kScaleP<__half> = 32768.0f;
+
+// (ptx::ex2 gives 0 for what is below 2^-126; weights go down to 2^-149, where the stick counts as used up)
+__device__ __forceinline__ float weight(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// log2(1 + u), 0 <= u <= 1; NaN for NaN.
+__device__ __forceinline__ float log2_1p(float u) {
+  const float w = u * rcp(2.0f + u), t = w * w;
+  float s = fmaf(t, 1.0f / 11, 1.0f / 9);
+  s = fmaf(t, s, 1.0f / 7);
+  s = fmaf(t, s, 1.0f / 5);
+  s = fmaf(t, s, 1.0f / 3);
+  s = fmaf(t, s, 1.0f);
+  return 2.0f * kLog2e * w * s;
+}
+
+// Where chunk c of row r of a stage's keys or values lies: the eight even (or odd) rows that one ldmatrix reads are in eight
+// different places of the 128 bytes that the banks span.
+template <int kD> __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return (uint32_t)(r * kD * 2 + ((c ^ ((r >> 1) & 7)) << 4));
+}
+
+// The copies of one warp.  `page_at` is the table's entry for the next tile, read a tile ahead.
+template <int kD> struct Loader {
+  using S = TcShape<kD>;
+  const DecodeParams &p;
+  const Piece &w;
+  const char *k, *v;      // the key head's first row of page 0
+  int page = -1;          // of the next tile's key that this lane looks up
+  bool bad = false;
+
+  __device__ __forceinline__ Loader(const DecodeParams &p_, const Piece &w_)
+      : p(p_), w(w_), k(p_.k.ptr + w_.head * p_.k.sh * 2), v(p_.v.ptr + w_.head * p_.v.sh * 2) {}
+  // lane l & 15 looks up key l & 15 of the tile
+  __device__ __forceinline__ void look_up(int key0) {
+    const int key = key0 + (threadIdx.x & 15);
+    page = -1;
+    if (key < w.k1) page = page_of(p, w.seq, key / p.page_size);
+  }
+  __device__ __forceinline__ void copy(int key0, uint32_t stage) {
+    const int lane = threadIdx.x & 31, key = key0 + (lane & 15);
+    bad = bad || (key < w.k1 && page < 0);
+    const long long slot = key - key / p.page_size * p.page_size;
+    const bool value = lane >= 16;               // lanes 16..31 hold the values' offsets
+    long long at = page < 0 ? -1 : (page * (value ? p.v.sp : p.k.sp) + slot * (value ? p.v.st : p.k.st)) * 2;
+    constexpr int kAtOnce = 32 / S::kChunks > 0 ? 32 / S::kChunks : 1;      // rows of one instruction
+    constexpr int kSplit = S::kChunks > 32 ? S::kChunks / 32 : 1;
+    static_assert(kSplit == 1, "a row is at most 32 chunks");
+    const int c = lane % S::kChunks, r0 = lane / S::kChunks;
+    const bool col = c * 8 < p.head_dim;
+#pragma unroll
+    for (int i = 0; i < kTileKeys / kAtOnce; ++i) {
+      const int r = i * kAtOnce + r0;
+      const long long ak = __shfl_sync(0xffffffffu, at, r), av = __shfl_sync(0xffffffffu, at, r + 16);
+      const uint32_t to = stage + chunk_at<kD>(r, c);
+      const bool take = ak >= 0 && col;
+      cp_async16(to, take ? k + ak + c * 16 : k, take);
+      cp_async16(to + S::kHalf, take ? v + av + c * 16 : v, take);
+    }
+  }
+};
+
+// A warp's keys, newest first.  kN: blocks of 8 query rows.
+template <typename T, int kD, int kN> struct TcWarp {
+  using S = TcShape<kD>;
+  uint32_t q[kN][kD / 16][2];
+  float acc[kD / 16][kN][4];
+  double left[kN][2];
+  int limit[kN][2];
+  bool real[kN][2];
+
+  __device__ __forceinline__ void start(const DecodeParams &p, const Piece &w) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const int r = n * 8 + g;
+      const unsigned short *row = reinterpret_cast<const unsigned short *>(p.q.ptr) + row_offset(p, p.q, w, min(r, w.rows - 1));
+#pragma unroll
+      for (int i = 0; i < kD / 16; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int c = i * 16 + half * 8 + t * 2;
+          q[n][i][half] = r < w.rows && c < p.head_dim ? row[c] | (uint32_t)row[c + 1] << 16 : 0;
+        }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int query = n * 8 + t * 2 + j;
+        left[n][j] = 0.0;
+        real[n][j] = query < w.rows;
+        limit[n][j] = row_limit(p, w.keys, w.row0 + min(query, w.rows - 1));
+      }
+#pragma unroll
+      for (int i = 0; i < kD / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
+    }
+  }
+
+  // O^T += V^T P^T, P as two 16-bit numbers; `b`: [row block][keys 2 m, 2 m + 1][high, low]
+  __device__ __forceinline__ void add_values(uint32_t values, const uint32_t (&b)[kN][2][2]) {
+    const int lane = threadIdx.x & 31;
+    const int r = 2 * (lane & 7) + (lane >> 4), c = (lane >> 3) & 1;
+#pragma unroll
+    for (int i = 0; i < kD / 16; ++i) {
+      uint32_t a[4];
+      ldsm4_t(values + chunk_at<kD>(r, 2 * i + c), a);
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        mma<T>(acc[i][n], a, b[n][0][0], b[n][1][0]);
+        mma<T>(acc[i][n], a, b[n][0][1], b[n][1][1]);
+      }
+    }
+  }
+  // The two 16-bit parts of the weights, moved from (key, query) to (query, key); only queries with limits in [low, high).
+  __device__ __forceinline__ void split(const float (&a)[kN][4], uint32_t (&b)[kN][2][2], int low, int high) {
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const bool x = limit[n][0] >= low && limit[n][0] < high, y = limit[n][1] >= low && limit[n][1] < high;
+#pragma unroll
+      for (int key = 0; key < 2; ++key) {
+        const float a0 = x ? a[n][2 * key] : 0.0f, a1 = y ? a[n][2 * key + 1] : 0.0f;
+        const uint32_t hi = pack<T>(a0, a1);
+        const float2 back = unpack<T>(hi);
+        b[n][key][0] = transpose8x8(hi);
+        b[n][key][1] = transpose8x8(pack<T>(a0 - back.x, a1 - back.y));
+      }
+    }
+  }
+
+  __device__ __forceinline__ void tile(const DecodeParams &p, const Piece &w, uint32_t stage, int key0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    float s[kN][4];
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
+    {
+      const int r = 2 * (lane & 7) + ((lane >> 3) & 1), c = lane >> 4;
+#pragma unroll
+      for (int i = 0; i < kD / 16; ++i) {
+        uint32_t a[4];
+        ldsm4(stage + chunk_at<kD>(r, 2 * i + c), a);
+#pragma unroll
+        for (int n = 0; n < kN; ++n) mma<T>(s[n], a, q[n][i][0], q[n][i][1]);
+      }
+    }
+    const float scale = p.scale * kLog2e;
+    float a[kN][4];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {                  // queries 2 t + j; keys 2 g (s[n][j]) and 2 g + 1 (s[n][2 + j])
+        float beta[2], broken[2];
+#pragma unroll
+        for (int key = 0; key < 2; ++key) {
+          const float x = s[n][2 * key + j] * scale, l = log2_1p(ex2(-fabsf(x)));
+          const bool in = key0 + 2 * g + key < limit[n][j];
+          beta[key] = in ? fminf(x, 0.0f) - l : -INFINITY;
+          broken[key] = in ? -(fmaxf(x, 0.0f) + l) : 0.0f;
+          if (in && x != x) beta[key] = broken[key] = x;      // (fminf and fmaxf drop a NaN)
+        }
+        const float both = broken[0] + broken[1];
+        float later = __shfl_down_sync(0xffffffffu, both, 4);
+        if (g == 7) later = 0.0f;
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          const float other = __shfl_down_sync(0xffffffffu, later, d);
+          if (lane + d < 32) later += other;
+        }
+        const float base = (float)left[n][j] + later;
+        a[n][2 + j] = weight(beta[1] + base) * kScaleP<T>;
+        a[n][j] = weight(beta[0] + (base + broken[1])) * kScaleP<T>;
+        left[n][j] += (double)__shfl_sync(0xffffffffu, later + both, lane & 3);
+      }
+    }
+    const uint32_t values = stage + S::kHalf;
+    uint32_t b[kN][2][2];
+    if (key0 + kTileKeys <= w.edge) {
+      split(a, b, 0, 0x7fffffff);
+      add_values(values, b);
+      return;
+    }
+    // Some rows do not attend to some keys of the tile.  Those keys' values are taken out, not multiplied by 0 (they may be no
+    // numbers): the rows take their turns from the longest reach down, and the values that are out of reach become zeros.
+    split(a, b, key0 + kTileKeys, 0x7fffffff);
+    add_values(values, b);
+    for (int reach = min(w.k1, key0 + kTileKeys - 1); reach >= max(w.edge, key0 + 1); --reach) {
+      __syncwarp();
+      if (lane < S::kChunks)
+        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(values + chunk_at<kD>(reach - key0, lane)), "r"(0) : "memory");
+      __syncwarp();
+      split(a, b, reach, reach + 1);
+      add_values(values, b);
+    }
+  }
+};
+
+template <typename T, int kD, int kN>
+__global__ void __launch_bounds__(TcShape<kD>::kThreads, 1) decode_tc_kernel(const __grid_constant__ DecodeParams p) {
+  using S = TcShape<kD>;
+  extern __shared__ __align__(128) char ring[];
+  __shared__ long long place[40];
+  __shared__ float left_of[S::kWarps][kN * 8];
+  enter_kernel<true>();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Place at = find_place<S::kThreads>(p, blockIdx.x, 0, place);
+  const long long begin = blockIdx.x * at.chunk, end = min(begin + at.chunk, at.units);
+  const uint32_t stages = smem_u32(ring) + warp * S::kStages * S::kStage;
+  float *sums = reinterpret_cast<float *>(ring + warp * S::kStages * S::kStage);
+  for (long long unit = begin; unit < end;) {
+    const int keys = seq_keys(p, at.seq);
+    const long long seq_units = (long long)p.kv_heads * p.row_blocks * units_of(keys);
+    if (unit >= at.first + seq_units) {
+      at.first += seq_units;
+      ++at.seq;
+      continue;
+    }
+    Piece w;
+    unit += next_piece(p, at, blockIdx.x, unit, begin, end, keys, w);
+
+    // the warps' ranges, warp 0 the newest
+    const int tiles = (w.k1 - w.k0 + kTileKeys - 1) / kTileKeys, share = (tiles + S::kWarps - 1) / S::kWarps;
+    const int t1 = max(tiles - warp * share, 0), t0 = max(t1 - share, 0);
+    Loader<kD> load(p, w);
+    if (t1 > t0) load.look_up(w.k0 + (t1 - 1) * kTileKeys);
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) {
+      const int t = t1 - 1 - i;
+      if (t >= t0) load.copy(w.k0 + t * kTileKeys, stages + i * S::kStage);
+      if (t > t0) load.look_up(w.k0 + (t - 1) * kTileKeys);
+      cp_async_commit();
+    }
+    TcWarp<T, kD, kN> sum;
+    sum.start(p, w);
+    int at_stage = 0;
+    for (int t = t1 - 1; t >= t0; --t) {
+      cp_async_wait<S::kStages - 2>();
+      __syncwarp();
+      const int ahead = t - (S::kStages - 1), into = at_stage == 0 ? S::kStages - 1 : at_stage - 1;
+      if (ahead >= t0) load.copy(w.k0 + ahead * kTileKeys, stages + into * S::kStage);
+      if (ahead > t0) load.look_up(w.k0 + (ahead - 1) * kTileKeys);
+      cp_async_commit();
+      sum.tile(p, w, stages + at_stage * S::kStage, w.k0 + t * kTileKeys);
+      at_stage = at_stage == S::kStages - 1 ? 0 : at_stage + 1;
+      if (!p.dense) {
+        bool gone = true;
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) gone = gone && (!sum.real[n][j] || sum.left[n][j] < (double)kStickGone);
+        if (__all_sync(0xffffffffu, gone)) break;
+      }
+    }
+    cp_async_wait<0>();
+    const bool bad = __any_sync(0xffffffffu, load.bad) || w.bad;
+    __syncwarp();
+    // the warp's sums into its own stages: [row][kD]
+    const int g = lane >> 2, tt = lane & 3;
+    const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+      for (int i = 0; i < kD / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sums[(n * 8 + tt * 2 + (j & 1)) * kD + i * 16 + g + (j >> 1) * 8] = bad ? nan : sum.acc[i][n][j];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (g == 0) left_of[warp][n * 8 + tt * 2 + j] = bad ? nan : (float)sum.left[n][j];
+    }
+    __syncthreads();
+    finish_piece<T, S::kThreads, S::kWarps, kN * 8>(p, w, reinterpret_cast<const float *>(ring), S::kStages * S::kStage / 4, kD,
+                                                    1.0f / kScaleP<T>, left_of);
+    __syncthreads();
+  }
+}
+
+template <typename T, int kD, int kN> cudaError_t launch_one(const DecodeParams &p, cudaStream_t s) {
+  using S = TcShape<kD>;
+  static_assert(kN * 8 * kD * 4 <= S::kStages * S::kStage, "a warp's sums fit into its stages");
+  const auto kernel = decode_tc_kernel<T, kD, kN>;
+  const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kBytes);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kernel, dim3(p.chunks), S::kThreads, S::kBytes, s, p);
+}
+template <typename T> cudaError_t launch_shape(const DecodeParams &p, cudaStream_t s) {
+  const int n = p.rows_per_block / 8;
+  if (p.head_dim <= 64) return n == 1 ? launch_one<T, 64, 1>(p, s) : n == 2 ? launch_one<T, 64, 2>(p, s) : launch_one<T, 64, 4>(p, s);
+  if (p.head_dim <= 128) return n == 1 ? launch_one<T, 128, 1>(p, s) : launch_one<T, 128, 2>(p, s);
+  return launch_one<T, 256, 1>(p, s);
+}
+
+}  // namespace
+
+// Query rows per item, as many as a thread's 64 accumulators hold; the keys are read once for them.
+int decode_tc_rows(int rows, int head_dim) {
+  const int most = head_dim <= 64 ? 32 : head_dim <= 128 ? 16 : 8;
+  return rows <= 8 || most == 8 ? 8 : rows <= 16 || most == 16 ? 16 : 32;
+}
+
+cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s) {
+  return dtype == SB_DTYPE_BF16 ? launch_shape<__nv_bfloat16>(p, s) : launch_shape<__half>(p, s);
+}
+
+}  // namespace sb

@@ -54,9 +54,14 @@ int check_decode(const SbDecodeParams *p) {
 }
 
 int plan_decode(const SbDecodeParams *p, DecodePlan &pl) {
-  pl.path = SB_PATH_SIMT;
+  // whole 16-byte chunks in every row of the cache
+  auto chunks = [](const SbCache &c) {
+    return reinterpret_cast<uintptr_t>(c.ptr) % 16 == 0 && c.stride_page % 8 == 0 && c.stride_h % 8 == 0 && c.stride_t % 8 == 0;
+  };
+  const bool tc = p->dtype != SB_DTYPE_F32 && !(p->flags & SB_FLAG_FORCE_SIMT) && p->head_dim % 8 == 0 && chunks(p->k) && chunks(p->v);
+  pl.path = tc ? SB_PATH_TCGEN05 : SB_PATH_SIMT;
   pl.rows = p->heads / p->kv_heads * p->new_tokens;
-  pl.rows_per_block = decode_simt_rows(pl.rows, p->head_dim);
+  pl.rows_per_block = tc ? decode_tc_rows(pl.rows, p->head_dim) : decode_simt_rows(pl.rows, p->head_dim);
   pl.row_blocks = (pl.rows + pl.rows_per_block - 1) / pl.rows_per_block;
   int sms = 0;
   const cudaError_t e = sm_count(&sms);
@@ -121,7 +126,7 @@ int run_decode(const SbDecodeParams *p, void *stream) {
   k.part_l = reinterpret_cast<float *>(reinterpret_cast<char *>(p->workspace) + pl.part_o);
   k.status = p->status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_decode_simt(k, p->dtype, s);
+  cudaError_t e = pl.path == SB_PATH_SIMT ? launch_decode_simt(k, p->dtype, s) : launch_decode_tc(k, p->dtype, s);
   if (e == cudaSuccess) e = launch_decode_join(k, p->dtype, s);
   *launches = 2;
   return e == cudaSuccess ? SB_OK : fail(SB_ERR_CUDA, "decode launch: %s", cudaGetErrorString(e));

@@ -107,6 +107,28 @@ def test_decode_infinite_scores(cuda_device, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("heads,new", [(2, 5), (12, 9)])
+@pytest.mark.parametrize("length", [100, 113, 131])
+def test_decode_keys_that_a_row_does_not_attend_to(cuda_device, dtype, heads, new, length):
+    """Keys and values of the newest tokens that are no numbers: they show in the rows that attend to them and in no other."""
+    import stickbreaking_attention_b200 as sb
+    q, (k, v, table, lens) = make(15, [length, 40], heads, 2, 64, 16, dtype, new=new)
+    for bad in (2, 4):                                        # the token from which on rows see it (keys before a query)
+        k2, v2 = k.clone(), v.clone()
+        pos = length - new + bad - 1
+        at = table[0, pos // 16].long()
+        k2[at, 0, pos % 16] = float("nan")
+        v2[at, 1, pos % 16] = float("inf")
+        o, rem = run_decode(sb, cuda_device, q, (k2, v2, table, lens))
+        half = heads // 2
+        assert not bool(torch.isfinite(o[0, :, bad:]).any(-1)[:half].any()) and bool(rem[0, :half, bad:].isnan().all())
+        assert not bool(torch.isfinite(o[0, half:, bad:]).any())
+        fine = lambda t: t[:, :, :bad]
+        R.check_decode((fine(o), fine(rem)), R.decode(fine(q), k, v, table, lens - (new - bad)))
+
+
+@gpu
 def test_decode_padded_batch(cuda_device):
     """More new tokens than a sequence has: rows in front of it, and empty sequences, give o = 0, rem = 1."""
     import stickbreaking_attention_b200 as sb
