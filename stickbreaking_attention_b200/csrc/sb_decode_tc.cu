@@ -178,8 +178,9 @@ template <typename T, int kD, int kN> struct TcWarp {
     }
   }
 
-  // O^T += V^T P^T, P as two 16-bit numbers; `b`: [row block][keys 2 m, 2 m + 1][high, low]
-  __device__ __forceinline__ void add_values(uint32_t values, const uint32_t (&b)[kN][2][2]) {
+  // O^T += V^T P^T, P as two 16-bit numbers; `b`: [row block][keys 2 m, 2 m + 1][high, low].  kSome: only for the queries whose
+  // limits are in [low, high).
+  template <bool kSome> __device__ __forceinline__ void add_values(uint32_t values, const uint32_t (&b)[kN][2][2], int low, int high) {
     const int lane = threadIdx.x & 31;
     const int r = 2 * (lane & 7) + (lane >> 4), c = (lane >> 3) & 1;
 #pragma unroll
@@ -188,23 +189,14 @@ template <typename T, int kD, int kN> struct TcWarp {
       ldsm4_t(values + chunk_at<kD>(r, 2 * i + c), a);
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        mma<T>(acc[i][n], a, b[n][0][0], b[n][1][0]);
-        mma<T>(acc[i][n], a, b[n][0][1], b[n][1][1]);
-      }
-    }
-  }
-  // The two 16-bit parts of the weights, moved from (key, query) to (query, key); only queries with limits in [low, high).
-  __device__ __forceinline__ void split(const float (&a)[kN][4], uint32_t (&b)[kN][2][2], int low, int high) {
+        float o[4];
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      const bool x = limit[n][0] >= low && limit[n][0] < high, y = limit[n][1] >= low && limit[n][1] < high;
+        for (int j = 0; j < 4; ++j) o[j] = acc[i][n][j];
+        mma<T>(o, a, b[n][0][0], b[n][1][0]);
+        mma<T>(o, a, b[n][0][1], b[n][1][1]);
 #pragma unroll
-      for (int key = 0; key < 2; ++key) {
-        const float a0 = x ? a[n][2 * key] : 0.0f, a1 = y ? a[n][2 * key + 1] : 0.0f;
-        const uint32_t hi = pack<T>(a0, a1);
-        const float2 back = unpack<T>(hi);
-        b[n][key][0] = transpose8x8(hi);
-        b[n][key][1] = transpose8x8(pack<T>(a0 - back.x, a1 - back.y));
+        for (int j = 0; j < 4; ++j)
+          if (!kSome || (limit[n][j & 1] >= low && limit[n][j & 1] < high)) acc[i][n][j] = o[j];
       }
     }
   }
@@ -255,24 +247,31 @@ template <typename T, int kD, int kN> struct TcWarp {
         left[n][j] += (double)__shfl_sync(0xffffffffu, later + both, lane & 3);
       }
     }
-    const uint32_t values = stage + S::kHalf;
+    // the two 16-bit parts of the weights, moved from (key, query) to (query, key)
     uint32_t b[kN][2][2];
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int key = 0; key < 2; ++key) {
+        const uint32_t hi = pack<T>(a[n][2 * key], a[n][2 * key + 1]);
+        const float2 back = unpack<T>(hi);
+        b[n][key][0] = transpose8x8(hi);
+        b[n][key][1] = transpose8x8(pack<T>(a[n][2 * key] - back.x, a[n][2 * key + 1] - back.y));
+      }
+    const uint32_t values = stage + S::kHalf;
     if (key0 + kTileKeys <= w.edge) {
-      split(a, b, 0, 0x7fffffff);
-      add_values(values, b);
+      add_values<false>(values, b, 0, 0);
       return;
     }
     // Some rows do not attend to some keys of the tile.  Those keys' values are taken out, not multiplied by 0 (they may be no
     // numbers): the rows take their turns from the longest reach down, and the values that are out of reach become zeros.
-    split(a, b, key0 + kTileKeys, 0x7fffffff);
-    add_values(values, b);
+    add_values<true>(values, b, key0 + kTileKeys, 0x7fffffff);
     for (int reach = min(w.k1, key0 + kTileKeys - 1); reach >= max(w.edge, key0 + 1); --reach) {
       __syncwarp();
       if (lane < S::kChunks)
         asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(values + chunk_at<kD>(reach - key0, lane)), "r"(0) : "memory");
       __syncwarp();
-      split(a, b, reach, reach + 1);
-      add_values(values, b);
+      add_values<true>(values, b, reach, reach + 1);
     }
   }
 };
