@@ -2,19 +2,24 @@
 //
 // A run of keys is summed up, per query row, by (o, L): o = sum of a_j v_j with the stick whole at the newest end of the run,
 // L = log2 of the stick that is left at its oldest end.  Two neighbouring runs join to (o_new + 2^L_new o_old, L_new + L_old),
-// and this is associative, so the cache of a sequence can be cut anywhere: into pieces for blocks, into ranges for warps.
+// and this is associative, so the cache of a sequence can be cut anywhere.
 //
 // An item is (sequence, key head, block of query rows); its keys are counted in units of kUnit.  The units of all items lie
-// one behind the other on one axis, which is cut into equal chunks, one per block: a batch of ragged lengths is spread evenly
-// whatever the lengths are, and only the device has to know them.  An item that a cut goes through leaves a piece per block in
-// the workspace (two slots per block) for the join kernel.
+// one behind the other on one axis, which is cut into equal chunks, one per WARP of the grid: a batch of ragged lengths is
+// spread evenly whatever the lengths are, only the device has to know them, and no warp ever waits for another.  A warp walks
+// through the pieces of its chunk without a pause: its loads run a ring of stages ahead of its arithmetic and go on into the next
+// piece while the last one's results are being written.  (With a block per chunk, its warps joined behind every piece, a piece
+// cost 8 us more than its bytes: 64 sequences x 16 heads x 512..4096 keys 201 us, 24 short ones with 4 new tokens 60 us.)
+//
+// An item that a cut goes through leaves a piece per chunk in the workspace (two slots per chunk) for the join kernel, and a
+// note of where they are.
 #pragma once
 
 #include "sb_common.cuh"
 
 namespace sb {
 
-constexpr int kUnit = 64;
+constexpr int kUnit = 64, kTileKeys = 16;
 // A weight below 2^-150 is exactly 0 in fp32, the smallest of whose numbers is 2^-149.
 constexpr float kStickGone = -150.0f;
 
@@ -32,10 +37,13 @@ struct DecodeParams {
   const int *seq_lens;
   int batch, heads, kv_heads, new_tokens, head_dim, page_size, num_pages, max_pages;
   int rows, row_blocks, rows_per_block;   // query rows of a key head = heads / kv_heads * new_tokens, and how they are cut
+  int items_per_seq;      // kv_heads * row_blocks
   int attend_current, dense;
   float scale;
-  int chunks, min_units;  // blocks of the main kernel; units that a block takes at least
+  int chunks;             // warps of the main kernel
+  int by_item;            // notes are numbered by item, where there are fewer items than chunks; else by chunk
   float *part_o, *part_l; // [2 * chunks][rows_per_block][head_dim], [2 * chunks][rows_per_block]
+  int4 *notes;            // [min(items, chunks)]: an item that was cut: sequence, item of it, first chunk, pieces (0: none)
   int *status;
 };
 
@@ -51,20 +59,57 @@ __device__ __forceinline__ int row_limit(const DecodeParams &p, int keys, int r)
   return max(keys - (p.new_tokens - 1 - r % p.new_tokens), 0);
 }
 
-struct Place {            // a position on the axis of units
-  long long units, chunk; // of the whole axis, and per block
-  int seq;
-  long long first;        // where the units of `seq` begin
+// One chunk's part of one item: keys [k0, k1) for the query rows [row0, row0 + rows) of key head `head`.
+struct Piece {
+  int seq, head, row0, rows, keys, k0, k1;
+  int edge;               // some row does not attend to the keys from here on (k1 and more if there is no such row)
 };
 
-// By all threads of the block (a multiple of 32, at most 1024); contains barriers.  Where unit `chunk_index * chunk + shift`
-// lies.  `shared`: 40 long longs.
+// Where a chunk is on its way through the items.
+struct Cursor {
+  int seq, item, u0, n, keys;   // item of the sequence, unit of the item, units of every item of the sequence, seq_keys
+  long long rest;               // units from here to the chunk's end
+  __device__ __forceinline__ void read_seq(const DecodeParams &p) {
+    keys = seq_keys(p, seq);
+    n = units_of(keys);
+  }
+  __device__ __forceinline__ int count() const { return (int)min((long long)(n - u0), rest); }
+  __device__ __forceinline__ void advance(const DecodeParams &p) {
+    rest -= count();
+    u0 = 0;
+    if (++item == p.items_per_seq) {
+      item = 0;
+      ++seq;
+      if (rest > 0) read_seq(p);
+    }
+  }
+  __device__ __forceinline__ Piece piece(const DecodeParams &p) const {
+    Piece w;
+    w.seq = seq;
+    w.keys = max(keys, 0);
+    w.head = item / p.row_blocks;
+    w.row0 = (item - w.head * p.row_blocks) * p.rows_per_block;
+    w.rows = min(p.rows - w.row0, p.rows_per_block);
+    // the first and the last token among the rows: what none of them attends to is not read, what some do not is looked at per row
+    const int tok = w.row0 % p.new_tokens, last = tok + w.rows - 1;
+    const int high = min(last, p.new_tokens - 1), low = last >= p.new_tokens ? 0 : tok;
+    w.k0 = u0 * kUnit;
+    w.k1 = max(min((u0 + count()) * kUnit, w.keys - (p.new_tokens - 1 - high)), w.k0);
+    w.edge = w.keys - (p.new_tokens - 1 - low);
+    return w;
+  }
+};
+__device__ __forceinline__ int tiles_of(const Piece &w) { return (w.k1 - w.k0 + kTileKeys - 1) / kTileKeys; }
+
+// The block's warps' chunks: warp w has chunk w * blocks + block, so that few units are spread over many SMs.  By all threads
+// of the block; contains barriers.  `shared`: 32 + 4 * warps long longs.
 template <int kThreads>
-__device__ __forceinline__ Place find_place(const DecodeParams &p, int chunk_index, int shift, long long *shared) {
-  const int per_item = p.kv_heads * p.row_blocks, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+__device__ __forceinline__ Cursor find_chunk(const DecodeParams &p, int &chunk, long long &size, long long *shared) {
+  constexpr int kWarps = kThreads / 32;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int each = (p.batch + kThreads - 1) / kThreads, b0 = min(t * each, p.batch), b1 = min(b0 + each, p.batch);
   long long own = 0;
-  for (int b = b0; b < b1; ++b) own += (long long)per_item * units_of(seq_keys(p, b));
+  for (int b = b0; b < b1; ++b) own += (long long)p.items_per_seq * units_of(seq_keys(p, b));
   long long sum = own;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -74,70 +119,49 @@ __device__ __forceinline__ Place find_place(const DecodeParams &p, int chunk_ind
   if (lane == 31) shared[warp] = sum;
   __syncthreads();
   long long before = 0, total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     if (w == warp) before = total;
     total += shared[w];
   }
   before += sum - own;
-  Place at;
-  at.units = total;
-  at.chunk = max((total + p.chunks - 1) / p.chunks, (long long)p.min_units);
-  const long long unit = chunk_index * at.chunk + shift;
-  if (unit >= before && unit < before + own) {
-    int b = b0;
+  size = (total + p.chunks - 1) / p.chunks;
+  for (int w = 0; w < kWarps; ++w) {
+    const long long unit = (w * (long long)gridDim.x + blockIdx.x) * size;
+    if (unit < before || unit >= before + own) continue;
+    long long first = before;
+    int b = b0, n;
     for (;; ++b) {
-      const long long n = (long long)per_item * units_of(seq_keys(p, b));
-      if (unit < before + n) break;
-      before += n;
+      n = units_of(seq_keys(p, b));
+      const long long all = (long long)p.items_per_seq * n;
+      if (unit < first + all) break;
+      first += all;
     }
-    shared[32] = b;
-    shared[33] = before;
+    const long long item = (unit - first) / n;
+    shared[32 + 4 * w] = b;
+    shared[33 + 4 * w] = item;
+    shared[34 + 4 * w] = unit - first - item * n;
   }
   __syncthreads();
-  at.seq = (int)shared[32];
-  at.first = shared[33];
-  return at;
+  Cursor c;
+  chunk = warp * gridDim.x + blockIdx.x;
+  c.rest = max(min(size, total - chunk * size), 0LL);
+  c.seq = c.item = c.u0 = c.n = c.keys = 0;
+  if (c.rest > 0) {
+    c.seq = (int)shared[32 + 4 * warp];
+    c.item = (int)shared[33 + 4 * warp];
+    c.u0 = (int)shared[34 + 4 * warp];
+    c.read_seq(p);
+  }
+  return c;
 }
 
-// One block's part of one item: keys [k0, k1) for the query rows [row0, row0 + rows) of key head `head`.
-struct Piece {
-  int seq, head, row0, rows, keys, k0, k1;
-  int edge;               // some row does not attend to the keys from here on (k1 and more if there is no such row)
-  int slot;               // where it is left for the join kernel, -1: it is the whole item
-  bool bad;               // the sequence's length was refused
-};
-
-// The piece at `unit` of a block's units [.., end); returns the units it takes.
-__device__ __forceinline__ int next_piece(const DecodeParams &p, const Place &at, int chunk_index, long long unit, long long begin,
-                                          long long end, int keys, Piece &w) {
-  w.bad = keys < 0;
-  w.keys = max(keys, 0);
-  const int n = units_of(keys);
-  const long long in_seq = unit - at.first;
-  const int item = (int)(in_seq / n), u0 = (int)(in_seq - (long long)item * n);
-  const int count = (int)min((long long)(n - u0), end - unit);
-  w.seq = at.seq;
-  w.head = item / p.row_blocks;
-  w.row0 = (item - w.head * p.row_blocks) * p.rows_per_block;
-  w.rows = min(p.rows - w.row0, p.rows_per_block);
-  // the first and the last token among the rows: what none of them attends to is not read, what some do not is looked at per row
-  const int tok = w.row0 % p.new_tokens, last = tok + w.rows - 1;
-  const int high = min(last, p.new_tokens - 1), low = last >= p.new_tokens ? 0 : tok;
-  w.k0 = u0 * kUnit;
-  w.k1 = max(min((u0 + count) * kUnit, w.keys - (p.new_tokens - 1 - high)), w.k0);
-  w.edge = w.keys - (p.new_tokens - 1 - low);
-  const bool whole = u0 == 0 && count == n;
-  w.slot = whole ? -1 : 2 * chunk_index + (u0 > 0 && unit == begin ? 0 : 1);
-  return count;
+__device__ __forceinline__ long long row_offset(const DecodeParams &p, const TensorRef &t, int seq, int head, int row) {
+  const int g = row / p.new_tokens, tok = row - g * p.new_tokens;
+  return seq * t.sb + (head * (long long)(p.heads / p.kv_heads) + g) * t.sh + tok * t.st;
 }
-
-__device__ __forceinline__ long long row_offset(const DecodeParams &p, const TensorRef &t, const Piece &w, int r) {
-  const int row = w.row0 + r, g = row / p.new_tokens, tok = row - g * p.new_tokens;
-  return w.seq * t.sb + (w.head * (long long)(p.heads / p.kv_heads) + g) * t.sh + tok * t.st;
-}
-__device__ __forceinline__ long long rem_index(const DecodeParams &p, const Piece &w, int r) {
-  const int row = w.row0 + r, g = row / p.new_tokens, tok = row - g * p.new_tokens;
-  return ((long long)w.seq * p.heads + w.head * (p.heads / p.kv_heads) + g) * p.new_tokens + tok;
+__device__ __forceinline__ long long rem_index(const DecodeParams &p, int seq, int head, int row) {
+  const int g = row / p.new_tokens, tok = row - g * p.new_tokens;
+  return ((long long)seq * p.heads + head * (p.heads / p.kv_heads) + g) * p.new_tokens + tok;
 }
 
 // The page that holds a key, or -1 (and the status word) for an entry of the table that is none.
@@ -151,50 +175,148 @@ __device__ __forceinline__ int page_of(const DecodeParams &p, int seq, int index
   return -1;
 }
 
-// The epilogue of a piece, by all threads of the block behind a barrier: joins the warps' sums (warp 0 has the newest keys),
-// warp n's at sums + n * warp_stride as [rows][width] times `unscale`, and writes the result or leaves it for the join kernel.
-template <typename T, int kThreads, int kWarps, int kRows>
-__device__ __forceinline__ void finish_piece(const DecodeParams &p, const Piece &w, const float *sums, int warp_stride, int width,
-                                             float unscale, const float (&left_of)[kWarps][kRows]) {
-  for (int e = threadIdx.x; e < w.rows * p.head_dim; e += kThreads) {
-    const int r = e / p.head_dim, c = e - r * p.head_dim;
-    float o = 0.0f, left = 0.0f;
-    for (int n = 0; n < kWarps; ++n) {
-      const float stick = exp2f(left);
-      if (stick == 0.0f) break;
-      o += stick * sums[n * warp_stride + r * width + c];
-      left += left_of[n][r];
-    }
-    o *= unscale;
-    if (w.slot < 0)
-      reinterpret_cast<T *>(p.o.ptr)[row_offset(p, p.o, w, r) + c] = from_f32<T>(o);
-    else
-      p.part_o[((long long)w.slot * p.rows_per_block + r) * p.head_dim + c] = o;
-  }
-  for (int r = threadIdx.x; r < w.rows; r += kThreads) {
-    float left = 0.0f;
-    for (int n = 0; n < kWarps; ++n) left += left_of[n][r];
-    if (w.slot < 0)
-      reinterpret_cast<T *>(p.rem)[rem_index(p, w, r)] = from_f32<T>(exp2f(left));
-    else
-      p.part_l[(long long)w.slot * p.rows_per_block + r] = left;
-  }
-  if (w.bad && threadIdx.x == 0 && p.status != nullptr) {
-    p.status[0] = SB_DEV_BAD_SEQ_LEN;
-    p.status[1] = w.seq;
-  }
-}
-
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int n> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
 
+// A warp's loads, newest tile of a piece first, on into the next pieces.  The page of a tile is looked up when the tile before
+// it is copied.
+template <typename E> struct Feed {
+  const DecodeParams &p;
+  Cursor c;
+  Piece w;
+  int left = 0, number = 0;     // tiles of the piece that are still to be copied; how many pieces came before it
+  int page = -1;                // that lane l & 15's key of the next tile is in
+  uint32_t bad = 0;             // a bit per stage: a page that is none
+
+  __device__ __forceinline__ Feed(const DecodeParams &p_, const Cursor &at) : p(p_), c(at) {
+    if (c.rest > 0) {
+      w = c.piece(p);
+      left = tiles_of(w);
+      E::prefetch_rows(p, w);
+      seek();
+    }
+  }
+  __device__ __forceinline__ void seek() {
+    while (left == 0) {
+      c.advance(p);
+      if (c.rest == 0) return;
+      w = c.piece(p);
+      left = tiles_of(w);
+      ++number;
+      E::prefetch_rows(p, w);
+    }
+    const int key = w.k0 + (left - 1) * kTileKeys + (threadIdx.x & 15);
+    page = key < w.k1 ? page_of(p, w.seq, key / p.page_size) : -1;
+  }
+  __device__ __forceinline__ void copy(int stage, char *to) {
+    if (left == 0) return;
+    const int key0 = w.k0 + --left * kTileKeys, key = key0 + (threadIdx.x & 15);
+    const bool wrong = __any_sync(0xffffffffu, key < w.k1 && page < 0);
+    bad = (bad & ~(1u << stage)) | (uint32_t)wrong << stage;
+    E::copy(p, w, page, key - key / p.page_size * p.page_size, to);
+    seek();
+  }
+  // what is left of piece `which` is not wanted; how many of its tiles that is
+  __device__ __forceinline__ int drop(int which) {
+    if (number != which || left == 0) return 0;
+    const int dropped = left;
+    left = 0;
+    seek();
+    return dropped;
+  }
+};
+
+// The main kernel.  E, the engine: the shape of a stage (kWarps, kStages, kStage bytes), copy (16 keys and values of one
+// key head), start, tile (adds a stage up, keys newest first), gone (the rows' sticks are used up), finish (writes the sums out).
+template <typename E>
+__device__ __forceinline__ void decode_chunks(const DecodeParams &p, char *ring, long long *shared) {
+  int chunk;
+  long long size;
+  Cursor c = find_chunk<E::kWarps * 32>(p, chunk, size, shared);
+  const int lane = threadIdx.x & 31;
+  if (!p.by_item && lane == 0) p.notes[chunk] = make_int4(0, 0, 0, 0);
+  if (c.rest == 0) return;
+  char *stages = ring + (threadIdx.x >> 5) * E::kStages * E::kStage;
+  Feed<E> feed(p, c);
+#pragma unroll
+  for (int i = 0; i < E::kStages - 1; ++i) {
+    feed.copy(i, stages + i * E::kStage);
+    cp_async_commit();
+  }
+  int at = 0, into = E::kStages - 1, number = 0;
+  for (bool first = true; c.rest > 0; first = false, ++number) {
+    const Piece w = c.piece(p);
+    E sum;
+    sum.start(p, w);
+    bool bad = c.keys < 0, done = false;
+    for (int left = tiles_of(w); left > 0; --left) {
+      cp_async_wait<E::kStages - 2>();
+      __syncwarp();
+      // (before the copy: it may set the same bit for a stage ahead only)
+      const bool wrong = feed.bad >> at & 1;
+      feed.copy(into, stages + into * E::kStage);
+      cp_async_commit();
+      if (!done) {
+        bad |= wrong;
+        sum.tile(p, w, stages + at * E::kStage, w.k0 + (left - 1) * kTileKeys);
+        if (!p.dense && sum.gone()) {
+          done = true;           // the tiles that are on their way still come by
+          left -= feed.drop(number);
+        }
+      }
+      at = at == E::kStages - 1 ? 0 : at + 1;
+      into = into == E::kStages - 1 ? 0 : into + 1;
+    }
+    const int count = c.count();
+    const bool whole = c.u0 == 0 && count == c.n;
+    const int slot = whole ? -1 : 2 * chunk + (first && c.u0 > 0 ? 0 : 1);
+    sum.finish(p, w, slot, bad);
+    if (c.u0 == 0 && lane == 0) {
+      const int pieces = whole ? 0 : 1 + (int)((c.n - count + size - 1) / size);
+      if (p.by_item) p.notes[c.seq * p.items_per_seq + c.item] = make_int4(c.seq, c.item, chunk, pieces);
+      else if (!whole) p.notes[chunk] = make_int4(c.seq, c.item, chunk, pieces);
+    }
+    if (c.keys < 0 && lane == 0 && p.status != nullptr) {
+      p.status[0] = SB_DEV_BAD_SEQ_LEN;
+      p.status[1] = c.seq;
+    }
+    c.advance(p);
+  }
+  cp_async_wait<0>();
+}
+
+// The result of row `row` of a piece's item: element `col` of it, or what is left of its stick.
+template <typename T> __device__ __forceinline__ void put_o(const DecodeParams &p, const Piece &w, int slot, int r, int col, float o) {
+  if (slot < 0)
+    reinterpret_cast<T *>(p.o.ptr)[row_offset(p, p.o, w.seq, w.head, w.row0 + r) + col] = from_f32<T>(o);
+  else
+    p.part_o[((long long)slot * p.rows_per_block + r) * p.head_dim + col] = o;
+}
+template <typename T> __device__ __forceinline__ void put_rem(const DecodeParams &p, const Piece &w, int slot, int r, float left) {
+  if (slot < 0)
+    reinterpret_cast<T *>(p.rem)[rem_index(p, w.seq, w.head, w.row0 + r)] = from_f32<T>(exp2f(left));
+  else
+    p.part_l[(long long)slot * p.rows_per_block + r] = left;
+}
+// The rows of q that a piece will want: on their way to L2 while the piece before it is worked on.
+template <int kBytes> __device__ __forceinline__ void prefetch_q(const DecodeParams &p, const Piece &w, int esize) {
+  const int lane = threadIdx.x & 31;
+  const int lines = (p.head_dim * esize + kBytes - 1) / kBytes;
+  for (int e = lane; e < w.rows * lines; e += 32) {
+    const int r = e / lines, l = e - r * lines;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p.q.ptr + row_offset(p, p.q, w.seq, w.head, w.row0 + r) * esize + l * kBytes));
+  }
+}
+
 cudaError_t launch_decode_simt(const DecodeParams &p, int dtype, cudaStream_t s);
-cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s);
 cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s);
-int decode_tc_rows(int rows, int head_dim);
-int decode_simt_rows(int rows, int head_dim);   // query rows per item
+cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s);
+int decode_tc_rows(int rows, int head_dim);     // query rows per item
+int decode_simt_rows(int rows, int head_dim);
+int decode_tc_warps(int head_dim);              // warps per block; one block per SM
+int decode_simt_warps(int head_dim);
 
 }  // namespace sb

@@ -29,15 +29,12 @@ using ptx::ex2;
 using ptx::rcp;
 using ptx::smem_u32;
 
-constexpr int kTileKeys = 16;
-
 template <int kD> struct TcShape {                                  // kD: head_dim rounded up to 64, 128, 256
   static constexpr int kChunks = kD / 8;                            // 16-byte chunks of a row
   static constexpr int kHalf = kTileKeys * kD * 2;                  // bytes of a stage's keys (or values)
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kWarps = kD <= 128 ? 8 : 4;
   static constexpr int kStages = kD <= 64 ? 6 : 3;
-  static constexpr int kThreads = kWarps * 32;
   static constexpr int kBytes = kWarps * kStages * kStage;          // 192 KiB
 };
 
@@ -102,61 +99,44 @@ template <int kD> __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return (uint32_t)(r * kD * 2 + ((c ^ ((r >> 1) & 7)) << 4));
 }
 
-// The copies of one warp.  `page_at` is the table's entry for the next tile, read a tile ahead.
-template <int kD> struct Loader {
+// The tensor-core engine.  kN: blocks of 8 query rows.
+template <typename T, int kD, int kN> struct TcEngine : TcShape<kD> {
   using S = TcShape<kD>;
-  const DecodeParams &p;
-  const Piece &w;
-  const char *k, *v;      // the key head's first row of page 0
-  int page = -1;          // of the next tile's key that this lane looks up
-  bool bad = false;
-
-  __device__ __forceinline__ Loader(const DecodeParams &p_, const Piece &w_)
-      : p(p_), w(w_), k(p_.k.ptr + w_.head * p_.k.sh * 2), v(p_.v.ptr + w_.head * p_.v.sh * 2) {}
-  // lane l & 15 looks up key l & 15 of the tile
-  __device__ __forceinline__ void look_up(int key0) {
-    const int key = key0 + (threadIdx.x & 15);
-    page = -1;
-    if (key < w.k1) page = page_of(p, w.seq, key / p.page_size);
-  }
-  __device__ __forceinline__ void copy(int key0, uint32_t stage) {
-    const int lane = threadIdx.x & 31, key = key0 + (lane & 15);
-    bad = bad || (key < w.k1 && page < 0);
-    const long long slot = key - key / p.page_size * p.page_size;
-    const bool value = lane >= 16;               // lanes 16..31 hold the values' offsets
-    long long at = page < 0 ? -1 : (page * (value ? p.v.sp : p.k.sp) + slot * (value ? p.v.st : p.k.st)) * 2;
-    constexpr int kAtOnce = 32 / S::kChunks > 0 ? 32 / S::kChunks : 1;      // rows of one instruction
-    constexpr int kSplit = S::kChunks > 32 ? S::kChunks / 32 : 1;
-    static_assert(kSplit == 1, "a row is at most 32 chunks");
-    const int c = lane % S::kChunks, r0 = lane / S::kChunks;
-    const bool col = c * 8 < p.head_dim;
-#pragma unroll
-    for (int i = 0; i < kTileKeys / kAtOnce; ++i) {
-      const int r = i * kAtOnce + r0;
-      const long long ak = __shfl_sync(0xffffffffu, at, r), av = __shfl_sync(0xffffffffu, at, r + 16);
-      const uint32_t to = stage + chunk_at<kD>(r, c);
-      const bool take = ak >= 0 && col;
-      cp_async16(to, take ? k + ak + c * 16 : k, take);
-      cp_async16(to + S::kHalf, take ? v + av + c * 16 : v, take);
-    }
-  }
-};
-
-// A warp's keys, newest first.  kN: blocks of 8 query rows.
-template <typename T, int kD, int kN> struct TcWarp {
-  using S = TcShape<kD>;
+  using S::kHalf;
   uint32_t q[kN][kD / 16][2];
   float acc[kD / 16][kN][4];
   double left[kN][2];
   int limit[kN][2];
   bool real[kN][2];
 
+  __device__ static __forceinline__ void prefetch_rows(const DecodeParams &p, const Piece &w) { prefetch_q<128>(p, w, 2); }
+
+  // Rows behind the piece's end, and columns behind head_dim, are zeros.
+  __device__ static __forceinline__ void copy(const DecodeParams &p, const Piece &w, int page, int slot, char *to) {
+    const int lane = threadIdx.x & 31;
+    const bool value = lane >= 16;               // lanes 16..31 hold the values' offsets
+    const PagedRef &t = value ? p.v : p.k;
+    const long long at = page < 0 ? -1 : (page * t.sp + w.head * t.sh + slot * t.st) * 2;
+    constexpr int kAtOnce = 32 / S::kChunks;     // rows of one instruction
+    const int c = lane % S::kChunks, r0 = lane / S::kChunks;
+    const bool col = c * 8 < p.head_dim;
+    const uint32_t stage = smem_u32(to);
+#pragma unroll
+    for (int i = 0; i < kTileKeys / kAtOnce; ++i) {
+      const int r = i * kAtOnce + r0;
+      const long long ak = __shfl_sync(0xffffffffu, at, r), av = __shfl_sync(0xffffffffu, at, r + 16);
+      const bool take = ak >= 0 && col;
+      cp_async16(stage + chunk_at<kD>(r, c), take ? p.k.ptr + ak + c * 16 : p.k.ptr, take);
+      cp_async16(stage + kHalf + chunk_at<kD>(r, c), take ? p.v.ptr + av + c * 16 : p.v.ptr, take);
+    }
+  }
+
   __device__ __forceinline__ void start(const DecodeParams &p, const Piece &w) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       const int r = n * 8 + g;
-      const unsigned short *row = reinterpret_cast<const unsigned short *>(p.q.ptr) + row_offset(p, p.q, w, min(r, w.rows - 1));
+      const unsigned short *row = reinterpret_cast<const unsigned short *>(p.q.ptr) + row_offset(p, p.q, w.seq, w.head, w.row0 + min(r, w.rows - 1));
 #pragma unroll
       for (int i = 0; i < kD / 16; ++i)
 #pragma unroll
@@ -201,7 +181,8 @@ template <typename T, int kD, int kN> struct TcWarp {
     }
   }
 
-  __device__ __forceinline__ void tile(const DecodeParams &p, const Piece &w, uint32_t stage, int key0) {
+  __device__ __forceinline__ void tile(const DecodeParams &p, const Piece &w, char *to, int key0) {
+    const uint32_t stage = smem_u32(to);
     const int lane = threadIdx.x & 31, g = lane >> 2;
     float s[kN][4];
 #pragma unroll
@@ -258,7 +239,7 @@ template <typename T, int kD, int kN> struct TcWarp {
         b[n][key][0] = transpose8x8(hi);
         b[n][key][1] = transpose8x8(pack<T>(a[n][2 * key] - back.x, a[n][2 * key + 1] - back.y));
       }
-    const uint32_t values = stage + S::kHalf;
+    const uint32_t values = stage + kHalf;
     if (key0 + kTileKeys <= w.edge) {
       add_values<false>(values, b, 0, 0);
       return;
@@ -274,95 +255,51 @@ template <typename T, int kD, int kN> struct TcWarp {
       add_values<true>(values, b, reach, reach + 1);
     }
   }
+
+  __device__ __forceinline__ bool gone() const {
+    bool all = true;
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) all = all && (!real[n][j] || left[n][j] < (double)kStickGone);
+    return __all_sync(0xffffffffu, all);
+  }
+
+  __device__ __forceinline__ void finish(const DecodeParams &p, const Piece &w, int slot, bool bad) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = n * 8 + t * 2 + j;
+        if (r >= w.rows) continue;
+#pragma unroll
+        for (int i = 0; i < kD / 16; ++i)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int c = i * 16 + half * 8 + g;
+            if (c < p.head_dim) put_o<T>(p, w, slot, r, c, bad ? nan : acc[i][n][half * 2 + j] * (1.0f / kScaleP<T>));
+          }
+        if (g == 0) put_rem<T>(p, w, slot, r, bad ? nan : (float)left[n][j]);
+      }
+  }
 };
 
 template <typename T, int kD, int kN>
-__global__ void __launch_bounds__(TcShape<kD>::kThreads, 1) decode_tc_kernel(const __grid_constant__ DecodeParams p) {
-  using S = TcShape<kD>;
+__global__ void __launch_bounds__(TcShape<kD>::kWarps * 32, 1) decode_tc_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) char ring[];
-  __shared__ long long place[40];
-  __shared__ float left_of[S::kWarps][kN * 8];
+  __shared__ long long shared[32 + 4 * TcShape<kD>::kWarps];
   enter_kernel<true>();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Place at = find_place<S::kThreads>(p, blockIdx.x, 0, place);
-  const long long begin = blockIdx.x * at.chunk, end = min(begin + at.chunk, at.units);
-  const uint32_t stages = smem_u32(ring) + warp * S::kStages * S::kStage;
-  float *sums = reinterpret_cast<float *>(ring + warp * S::kStages * S::kStage);
-  for (long long unit = begin; unit < end;) {
-    const int keys = seq_keys(p, at.seq);
-    const long long seq_units = (long long)p.kv_heads * p.row_blocks * units_of(keys);
-    if (unit >= at.first + seq_units) {
-      at.first += seq_units;
-      ++at.seq;
-      continue;
-    }
-    Piece w;
-    unit += next_piece(p, at, blockIdx.x, unit, begin, end, keys, w);
-
-    // the warps' ranges, warp 0 the newest
-    const int tiles = (w.k1 - w.k0 + kTileKeys - 1) / kTileKeys, share = (tiles + S::kWarps - 1) / S::kWarps;
-    const int t1 = max(tiles - warp * share, 0), t0 = max(t1 - share, 0);
-    Loader<kD> load(p, w);
-    if (t1 > t0) load.look_up(w.k0 + (t1 - 1) * kTileKeys);
-#pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) {
-      const int t = t1 - 1 - i;
-      if (t >= t0) load.copy(w.k0 + t * kTileKeys, stages + i * S::kStage);
-      if (t > t0) load.look_up(w.k0 + (t - 1) * kTileKeys);
-      cp_async_commit();
-    }
-    TcWarp<T, kD, kN> sum;
-    sum.start(p, w);
-    int at_stage = 0;
-    for (int t = t1 - 1; t >= t0; --t) {
-      cp_async_wait<S::kStages - 2>();
-      __syncwarp();
-      const int ahead = t - (S::kStages - 1), into = at_stage == 0 ? S::kStages - 1 : at_stage - 1;
-      if (ahead >= t0) load.copy(w.k0 + ahead * kTileKeys, stages + into * S::kStage);
-      if (ahead > t0) load.look_up(w.k0 + (ahead - 1) * kTileKeys);
-      cp_async_commit();
-      sum.tile(p, w, stages + at_stage * S::kStage, w.k0 + t * kTileKeys);
-      at_stage = at_stage == S::kStages - 1 ? 0 : at_stage + 1;
-      if (!p.dense) {
-        bool gone = true;
-#pragma unroll
-        for (int n = 0; n < kN; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) gone = gone && (!sum.real[n][j] || sum.left[n][j] < (double)kStickGone);
-        if (__all_sync(0xffffffffu, gone)) break;
-      }
-    }
-    cp_async_wait<0>();
-    const bool bad = __any_sync(0xffffffffu, load.bad) || w.bad;
-    __syncwarp();
-    // the warp's sums into its own stages: [row][kD]
-    const int g = lane >> 2, tt = lane & 3;
-    const float nan = __int_as_float(0x7fffffff);
-#pragma unroll
-    for (int n = 0; n < kN; ++n) {
-#pragma unroll
-      for (int i = 0; i < kD / 16; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          sums[(n * 8 + tt * 2 + (j & 1)) * kD + i * 16 + g + (j >> 1) * 8] = bad ? nan : sum.acc[i][n][j];
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (g == 0) left_of[warp][n * 8 + tt * 2 + j] = bad ? nan : (float)sum.left[n][j];
-    }
-    __syncthreads();
-    finish_piece<T, S::kThreads, S::kWarps, kN * 8>(p, w, reinterpret_cast<const float *>(ring), S::kStages * S::kStage / 4, kD,
-                                                    1.0f / kScaleP<T>, left_of);
-    __syncthreads();
-  }
+  decode_chunks<TcEngine<T, kD, kN>>(p, ring, shared);
 }
 
 template <typename T, int kD, int kN> cudaError_t launch_one(const DecodeParams &p, cudaStream_t s) {
   using S = TcShape<kD>;
-  static_assert(kN * 8 * kD * 4 <= S::kStages * S::kStage, "a warp's sums fit into its stages");
   const auto kernel = decode_tc_kernel<T, kD, kN>;
   const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3(p.chunks), S::kThreads, S::kBytes, s, p);
+  return launch_kernel(kernel, dim3(p.chunks / S::kWarps), S::kWarps * 32, S::kBytes, s, p);
 }
 template <typename T> cudaError_t launch_shape(const DecodeParams &p, cudaStream_t s) {
   const int n = p.rows_per_block / 8;
@@ -378,6 +315,7 @@ int decode_tc_rows(int rows, int head_dim) {
   const int most = head_dim <= 64 ? 32 : head_dim <= 128 ? 16 : 8;
   return rows <= 8 || most == 8 ? 8 : rows <= 16 || most == 16 ? 16 : 32;
 }
+int decode_tc_warps(int head_dim) { return head_dim <= 128 ? TcShape<128>::kWarps : TcShape<256>::kWarps; }
 
 cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s) {
   return dtype == SB_DTYPE_BF16 ? launch_shape<__nv_bfloat16>(p, s) : launch_shape<__half>(p, s);

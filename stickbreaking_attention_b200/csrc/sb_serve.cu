@@ -35,8 +35,9 @@ int check_pool(int dtype, int kv_heads, int head_dim, int page_size, int num_pag
 }
 
 struct DecodePlan {
-  int path, rows, rows_per_block, row_blocks, chunks, min_units;
-  size_t part_o, bytes;
+  int path, rows, rows_per_block, row_blocks, chunks;
+  bool by_item;
+  size_t part_o, part_l, bytes;
 };
 
 int check_decode(const SbDecodeParams *p) {
@@ -66,11 +67,13 @@ int plan_decode(const SbDecodeParams *p, DecodePlan &pl) {
   int sms = 0;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return fail(SB_ERR_CUDA, "SM count: %s", cudaGetErrorString(e));
-  pl.chunks = sms;
-  pl.min_units = 4;
-  const size_t slots = 2 * (size_t)pl.chunks * pl.rows_per_block;
-  pl.part_o = slots * p->head_dim * sizeof(float);
-  pl.bytes = (pl.part_o + slots * sizeof(float) + 255) / 256 * 256;
+  pl.chunks = sms * (tc ? decode_tc_warps(p->head_dim) : decode_simt_warps(p->head_dim));
+  const long long items = (long long)p->batch * p->kv_heads * pl.row_blocks;
+  pl.by_item = items < pl.chunks;
+  const size_t slots = 2 * (size_t)pl.chunks * pl.rows_per_block, notes = (size_t)(pl.by_item ? items : pl.chunks) * sizeof(int4);
+  pl.part_o = (notes + 255) / 256 * 256;
+  pl.part_l = pl.part_o + slots * p->head_dim * sizeof(float);
+  pl.bytes = (pl.part_l + slots * sizeof(float) + 255) / 256 * 256;
   return SB_OK;
 }
 
@@ -121,9 +124,12 @@ int run_decode(const SbDecodeParams *p, void *stream) {
   k.dense = (p->flags & SB_FLAG_DENSE_ROW_PASS) ? 1 : 0;
   k.scale = p->logit_scale;
   k.chunks = pl.chunks;
-  k.min_units = pl.min_units;
-  k.part_o = reinterpret_cast<float *>(p->workspace);
-  k.part_l = reinterpret_cast<float *>(reinterpret_cast<char *>(p->workspace) + pl.part_o);
+  k.by_item = pl.by_item;
+  k.items_per_seq = p->kv_heads * pl.row_blocks;
+  char *ws = reinterpret_cast<char *>(p->workspace);
+  k.notes = reinterpret_cast<int4 *>(ws);
+  k.part_o = reinterpret_cast<float *>(ws + pl.part_o);
+  k.part_l = reinterpret_cast<float *>(ws + pl.part_l);
   k.status = p->status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = pl.path == SB_PATH_SIMT ? launch_decode_simt(k, p->dtype, s) : launch_decode_tc(k, p->dtype, s);
