@@ -49,9 +49,12 @@ template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtSh
   double left[kPairs];
   int limit[kPairs];
 
-  __device__ static __forceinline__ void prefetch_rows(const DecodeParams &p, const Piece &w) { prefetch_q<128>(p, w, sizeof(T)); }
+  __device__ static __forceinline__ void prefetch_rows(const DecodeParams &p, const Piece &w) { prefetch_q(p, w, sizeof(T)); }
 
-  // Rows behind the piece's end, and columns behind head_dim, are zeros.
+  __device__ static __forceinline__ void copy_run(const DecodeParams &p, const Piece &w, int page, int slot, char *to) {
+    copy(p, w, page, slot + (threadIdx.x & 15), to);
+  }
+  // Rows without a page, and columns behind head_dim, are zeros.
   __device__ static __forceinline__ void copy(const DecodeParams &p, const Piece &w, int page, int slot, char *to) {
     const int lane = threadIdx.x & 31;
     for (int j = 0; j < kTileKeys; ++j) {
@@ -172,12 +175,15 @@ template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtSh
     const int lane = threadIdx.x & 31;
     const float nan = __int_as_float(0x7fffffff);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+    for (int r = 0; r < kRows; ++r) {
+      if (r >= w.rows) break;
+      const RowOut<T> out(p, w, slot, r);
 #pragma unroll
       for (int i = 0; i < kCols; ++i) {
         const int c = col_of<kCols>(lane, i);
-        if (r < w.rows && c < p.head_dim) put_o<T>(p, w, slot, r, c, bad ? nan : acc[r][i]);
+        if (c < p.head_dim) out.put(c, bad ? nan : acc[r][i]);
       }
+    }
 #pragma unroll
     for (int pr = 0; pr < kPairs; ++pr)
       if (lane < 2 && 2 * pr + lane < w.rows) put_rem<T>(p, w, slot, 2 * pr + lane, bad ? nan : (float)(left[pr] * kLog2eD));
@@ -187,95 +193,88 @@ template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtSh
 template <typename E>
 __global__ void __launch_bounds__(E::kWarps * 32, 1) decode_simt_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) char ring[];
-  __shared__ long long shared[32 + 4 * E::kWarps];
+  __shared__ ChunkShared<E::kWarps> shared;
   enter_kernel<true>();
   decode_chunks<E>(p, ring, shared);
 }
 
-// Joins the pieces of the items that were cut: a block per note (and share of the item's columns).  Its warps take the pieces
-// in turns, 32 * 4 elements at a time.
-constexpr int kJoinElements = 128, kJoinPieces = 256, kMostRows = 32;
-template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_constant__ DecodeParams p) {
-  constexpr int kWarps = kThreads / 32;
-  __shared__ float stick[kJoinPieces][kMostRows];      // of each piece: what of the stick its newest end still has
-  __shared__ float left[kMostRows];                    // log2 of what the pieces so far have left of it
-  __shared__ float sums[kWarps][kJoinElements];
+// Joins the pieces of the items that were cut, 128 elements (rows x columns) of an item at a time, four neighbours per lane, newest piece first.
+// Each warp has elements of its own (kTogether false), or all warps of a block have the same and take a run of the pieces each,
+// whose sums are joined like pieces: for items of very many pieces.
+constexpr int kJoinElements = 128;
+template <typename T, int kWarps, bool kTogether>
+__global__ void __launch_bounds__(kWarps * 32) decode_join_kernel(const __grid_constant__ DecodeParams p) {
   enter_kernel<true>();
   const int4 note = p.notes[blockIdx.x];
   if (note.w == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int head = note.y / p.row_blocks, row0 = (note.y - head * p.row_blocks) * p.rows_per_block;
+  const int head = p.row_blocks == 1 ? note.y : note.y / p.row_blocks, row0 = (note.y - head * p.row_blocks) * p.rows_per_block;
   const int rows = min(p.rows - row0, p.rows_per_block), elements = rows * p.head_dim;
-  const auto slot_of = [&](int i) {       // i-th piece from the newest on: the oldest is its chunk's last, the others their chunk's first
-    const int c = note.z + note.w - 1 - i;
-    return 2 * (long long)c + (i == note.w - 1 ? 1 : 0);
-  };
+  const int e0 = (kTogether ? blockIdx.y : blockIdx.y * kWarps + warp) * kJoinElements + lane * 4;
+  if (!kTogether && e0 - lane * 4 >= elements) return;
+  int r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = min(e0 + j, elements - 1) / p.head_dim;
   const long long part = (long long)p.rows_per_block * p.head_dim;
-  for (int e0 = blockIdx.y * kJoinElements; e0 < elements; e0 += gridDim.y * kJoinElements) {
-    float o[4] = {};
-    for (int base = 0; base < note.w; base += kJoinPieces) {
-      const int n = min(note.w - base, kJoinPieces);
-      __syncthreads();
-      for (int e = threadIdx.x; e < n * rows; e += kThreads) {
-        const int i = e / rows, r = e - i * rows;
-        stick[i][r] = p.part_l[slot_of(base + i) * p.rows_per_block + r];
+  float o[4] = {}, left[4] = {};
+  const int share = kTogether ? (note.w + kWarps - 1) / kWarps : note.w;
+  const int begin = kTogether ? min(warp * share, note.w) : 0, end = min(begin + share, note.w);
+  constexpr int kDeep = 8;
+  for (int i0 = begin; i0 < end; i0 += kDeep) {
+    float x[kDeep][4], l[kDeep][4];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const int i = min(i0 + k, end - 1), c = note.z + note.w - 1 - i;
+      const long long slot = 2 * (long long)c + (i == note.w - 1 ? 1 : 0);      // the oldest is its chunk's last piece, the others their chunk's first
+      const float *src = p.part_o + slot * part;
+      if (p.head_dim % 4 == 0) {
+        const float4 v = *reinterpret_cast<const float4 *>(src + min(e0, elements - 4));
+        x[k][0] = v.x; x[k][1] = v.y; x[k][2] = v.z; x[k][3] = v.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[k][j] = src[min(e0 + j, elements - 1)];
       }
-      if (base == 0 && threadIdx.x < kMostRows) left[threadIdx.x] = 0.0f;
-      __syncthreads();
-      for (int r = warp; r < rows; r += kWarps) {      // exclusive sums over the pieces
-        float before = left[r];
-        for (int i0 = 0; i0 < n; i0 += 32) {
-          const float own = i0 + lane < n ? stick[i0 + lane][r] : 0.0f;
-          float sum = own;
+      l[k][0] = p.part_l[slot * p.rows_per_block + r[0]];
 #pragma unroll
-          for (int d = 1; d < 32; d <<= 1) {
-            const float other = __shfl_up_sync(0xffffffffu, sum, d);
-            if (lane >= d) sum += other;
-          }
-          float excl = __shfl_up_sync(0xffffffffu, sum, 1);
-          if (lane == 0) excl = 0.0f;
-          if (i0 + lane < n) stick[i0 + lane][r] = exp2f(before + excl);
-          before += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        __syncwarp();
-        if (lane == 0) left[r] = before;
-      }
-      __syncthreads();
-      constexpr int kDeep = 8;
-      for (int i0 = warp; i0 < n; i0 += kDeep * kWarps) {
-        float x[kDeep][4];
-#pragma unroll
-        for (int k = 0; k < kDeep; ++k) {
-          const int i = i0 + k * kWarps;
-          const float *src = p.part_o + slot_of(base + min(i, n - 1)) * part + e0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[k][j] = i < n && e0 + lane + 32 * j < elements ? src[lane + 32 * j] : 0.0f;
-        }
-#pragma unroll
-        for (int k = 0; k < kDeep; ++k)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int i = i0 + k * kWarps, e = e0 + lane + 32 * j;
-            if (i >= n || e >= elements) continue;
-            const float s = stick[i][e / p.head_dim];
-            if (s != 0.0f) o[j] += s * x[k][j];        // (0 times what is no number stays out)
-          }
-      }
+      for (int j = 1; j < 4; ++j) l[k][j] = p.head_dim % 4 == 0 ? l[k][0] : p.part_l[slot * p.rows_per_block + r[j]];
     }
-    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sums[warp][lane + 32 * j] = o[j];
-    __syncthreads();
-    for (int e = threadIdx.x; e < kJoinElements && e0 + e < elements; e += kThreads) {
-      float sum = 0.0f;
-      for (int n = 0; n < kWarps; ++n) sum += sums[n][e];
-      const int r = (e0 + e) / p.head_dim, c = e0 + e - r * p.head_dim;
-      reinterpret_cast<T *>(p.o.ptr)[row_offset(p, p.o, note.x, head, row0 + r) + c] = from_f32<T>(sum);
+    for (int k = 0; k < kDeep; ++k) {
+      if (i0 + k >= end) break;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float stick = exp2f(left[j]);
+        if (stick != 0.0f) o[j] += stick * x[k][j];        // (0 times what is no number stays out)
+        left[j] += l[k][j];
+      }
     }
   }
-  if (blockIdx.y == 0 && threadIdx.x < rows)
-    reinterpret_cast<T *>(p.rem)[rem_index(p, note.x, head, row0 + threadIdx.x)] = from_f32<T>(exp2f(left[threadIdx.x]));
+  if constexpr (kTogether) {
+    __shared__ float4 sums[kWarps][32], lefts[kWarps][32];
+    sums[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+    lefts[warp][lane] = make_float4(left[0], left[1], left[2], left[3]);
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = left[j] = 0.0f;
+    for (int n = 0; n < kWarps; ++n) {
+      const float4 x = sums[n][lane], l = lefts[n][lane];
+      const float xs[4] = {x.x, x.y, x.z, x.w}, ls[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float stick = exp2f(left[j]);
+        if (stick != 0.0f) o[j] += stick * xs[j];
+        left[j] += ls[j];
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int e = e0 + j, col = e - r[j] * p.head_dim;
+    if (e >= elements) continue;
+    reinterpret_cast<T *>(p.o.ptr)[row_offset(p, p.o, note.x, head, row0 + r[j]) + col] = from_f32<T>(o[j]);
+    if (col == 0) reinterpret_cast<T *>(p.rem)[rem_index(p, note.x, head, row0 + r[j])] = from_f32<T>(exp2f(left[j]));
+  }
 }
 
 template <typename E> cudaError_t launch_engine(const DecodeParams &p, cudaStream_t s) {
@@ -316,20 +315,21 @@ cudaError_t launch_decode_simt(const DecodeParams &p, int dtype, cudaStream_t s)
   }
 }
 
-// Few items are cut into many pieces each: a large block per item, and several of them where one could not read fast enough.
-// Where there are at least as many items as chunks most have two pieces at most, and few have any.
 cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s) {
   const long long items = (long long)p.batch * p.items_per_seq;
   const int notes = (int)(p.by_item ? items : p.chunks);
   const int tiles = (p.rows_per_block * p.head_dim + kJoinElements - 1) / kJoinElements;
-  const int split = p.by_item ? std::max(1, std::min(tiles, 256 / notes)) : 1;
-  auto go = [&](auto kernel, int threads) { return launch_kernel(kernel, dim3(notes, split), threads, 0, s, p); };
-  const bool wide = p.by_item && p.chunks >= 16 * items;
+  constexpr int kWide = 16, kNarrow = 4;
+  const bool wide = p.by_item && p.chunks >= kWide * items;      // sixteen pieces and more of an item, on the average
+  const dim3 grid(notes, wide ? tiles : (tiles + kNarrow - 1) / kNarrow);
+  auto go = [&](auto kernel, int threads) { return launch_kernel(kernel, grid, threads, 0, s, p); };
+#define SB_JOIN(T) wide ? go(decode_join_kernel<T, kWide, true>, kWide * 32) : go(decode_join_kernel<T, kNarrow, false>, kNarrow * 32)
   switch (dtype) {
-    case SB_DTYPE_F32: return wide ? go(decode_join_kernel<float, 512>, 512) : go(decode_join_kernel<float, 128>, 128);
-    case SB_DTYPE_BF16: return wide ? go(decode_join_kernel<__nv_bfloat16, 512>, 512) : go(decode_join_kernel<__nv_bfloat16, 128>, 128);
-    default: return wide ? go(decode_join_kernel<__half, 512>, 512) : go(decode_join_kernel<__half, 128>, 128);
+    case SB_DTYPE_F32: return SB_JOIN(float);
+    case SB_DTYPE_BF16: return SB_JOIN(__nv_bfloat16);
+    default: return SB_JOIN(__half);
   }
+#undef SB_JOIN
 }
 
 }  // namespace sb

@@ -19,7 +19,7 @@
 
 namespace sb {
 
-constexpr int kUnit = 64, kTileKeys = 16;
+constexpr int kUnit = 64, kTileKeys = 16;      // (units are 64 keys or, in huge batches, so many more that 31 bits count them)
 // A weight below 2^-150 is exactly 0 in fp32, the smallest of whose numbers is 2^-149.
 constexpr float kStickGone = -150.0f;
 
@@ -38,7 +38,9 @@ struct DecodeParams {
   int batch, heads, kv_heads, new_tokens, head_dim, page_size, num_pages, max_pages;
   int rows, row_blocks, rows_per_block;   // query rows of a key head = heads / kv_heads * new_tokens, and how they are cut
   int items_per_seq;      // kv_heads * row_blocks
+  int page_shift;         // page_size = 1 << page_shift, or -1
   int attend_current, dense;
+  int unit_shift;         // a unit is 1 << unit_shift keys
   float scale;
   int chunks;             // warps of the main kernel
   int by_item;            // notes are numbered by item, where there are fewer items than chunks; else by chunk
@@ -53,10 +55,15 @@ __device__ __forceinline__ int seq_keys(const DecodeParams &p, int b) {
   if (len < 0 || len > (long long)p.max_pages * p.page_size) return -1;
   return max(len - (p.attend_current ? 0 : 1), 0);
 }
-__device__ __forceinline__ int units_of(int keys) { return max((max(keys, 0) + kUnit - 1) / kUnit, 1); }
+__device__ __forceinline__ int units_of(const DecodeParams &p, int keys) {
+  return keys <= 0 ? 1 : (int)(((unsigned)keys + (1u << p.unit_shift) - 1) >> p.unit_shift);
+}
+__device__ __forceinline__ int page_index(const DecodeParams &p, int key) {
+  return p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+}
 // Keys that query row r (= head of the group * new_tokens + token) attends to are those before this one.
 __device__ __forceinline__ int row_limit(const DecodeParams &p, int keys, int r) {
-  return max(keys - (p.new_tokens - 1 - r % p.new_tokens), 0);
+  return p.new_tokens == 1 ? keys : max(keys - (p.new_tokens - 1 - r % p.new_tokens), 0);
 }
 
 // One chunk's part of one item: keys [k0, k1) for the query rows [row0, row0 + rows) of key head `head`.
@@ -68,12 +75,12 @@ struct Piece {
 // Where a chunk is on its way through the items.
 struct Cursor {
   int seq, item, u0, n, keys;   // item of the sequence, unit of the item, units of every item of the sequence, seq_keys
-  long long rest;               // units from here to the chunk's end
+  int rest;                     // units from here to the chunk's end
   __device__ __forceinline__ void read_seq(const DecodeParams &p) {
     keys = seq_keys(p, seq);
-    n = units_of(keys);
+    n = units_of(p, keys);
   }
-  __device__ __forceinline__ int count() const { return (int)min((long long)(n - u0), rest); }
+  __device__ __forceinline__ int count() const { return min(n - u0, rest); }
   __device__ __forceinline__ void advance(const DecodeParams &p) {
     rest -= count();
     u0 = 0;
@@ -87,14 +94,14 @@ struct Cursor {
     Piece w;
     w.seq = seq;
     w.keys = max(keys, 0);
-    w.head = item / p.row_blocks;
+    w.head = p.row_blocks == 1 ? item : item / p.row_blocks;
     w.row0 = (item - w.head * p.row_blocks) * p.rows_per_block;
     w.rows = min(p.rows - w.row0, p.rows_per_block);
     // the first and the last token among the rows: what none of them attends to is not read, what some do not is looked at per row
-    const int tok = w.row0 % p.new_tokens, last = tok + w.rows - 1;
+    const int tok = p.new_tokens == 1 ? 0 : w.row0 % p.new_tokens, last = tok + w.rows - 1;
     const int high = min(last, p.new_tokens - 1), low = last >= p.new_tokens ? 0 : tok;
-    w.k0 = u0 * kUnit;
-    w.k1 = max(min((u0 + count()) * kUnit, w.keys - (p.new_tokens - 1 - high)), w.k0);
+    w.k0 = u0 << p.unit_shift;
+    w.k1 = max(min(u0 + count() == n ? w.keys : (u0 + count()) << p.unit_shift, w.keys - (p.new_tokens - 1 - high)), w.k0);
     w.edge = w.keys - (p.new_tokens - 1 - low);
     return w;
   }
@@ -102,77 +109,66 @@ struct Cursor {
 __device__ __forceinline__ int tiles_of(const Piece &w) { return (w.k1 - w.k0 + kTileKeys - 1) / kTileKeys; }
 
 // The block's warps' chunks: warp w has chunk w * blocks + block, so that few units are spread over many SMs.  By all threads
-// of the block; contains barriers.  `shared`: 32 + 4 * warps long longs.
-template <int kThreads>
-__device__ __forceinline__ Cursor find_chunk(const DecodeParams &p, int &chunk, long long &size, long long *shared) {
-  constexpr int kWarps = kThreads / 32;
+// of the block; contains barriers.
+template <int kWarps> struct ChunkShared {
+  int sum[kWarps], before[kWarps * 32 + 1];    // units of each warp's sequences; units before each thread's
+};
+template <int kWarps>
+__device__ __forceinline__ Cursor find_chunk(const DecodeParams &p, int &chunk, int &size, ChunkShared<kWarps> &shared) {
+  constexpr int kThreads = kWarps * 32;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int each = (p.batch + kThreads - 1) / kThreads, b0 = min(t * each, p.batch), b1 = min(b0 + each, p.batch);
-  long long own = 0;
-  for (int b = b0; b < b1; ++b) own += (long long)p.items_per_seq * units_of(seq_keys(p, b));
-  long long sum = own;
+  int own = 0;
+  for (int b = b0; b < b1; ++b) own += p.items_per_seq * units_of(p, seq_keys(p, b));
+  int sum = own;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long other = __shfl_up_sync(0xffffffffu, sum, d);
+    const int other = __shfl_up_sync(0xffffffffu, sum, d);
     if (lane >= d) sum += other;
   }
-  if (lane == 31) shared[warp] = sum;
+  if (lane == 31) shared.sum[warp] = sum;
   __syncthreads();
-  long long before = 0, total = 0;
+  int before = sum - own, total = 0;
+#pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w == warp) before = total;
-    total += shared[w];
+    if (w < warp) before += shared.sum[w];
+    total += shared.sum[w];
   }
-  before += sum - own;
-  size = (total + p.chunks - 1) / p.chunks;
-  for (int w = 0; w < kWarps; ++w) {
-    const long long unit = (w * (long long)gridDim.x + blockIdx.x) * size;
-    if (unit < before || unit >= before + own) continue;
-    long long first = before;
-    int b = b0, n;
-    for (;; ++b) {
-      n = units_of(seq_keys(p, b));
-      const long long all = (long long)p.items_per_seq * n;
-      if (unit < first + all) break;
-      first += all;
-    }
-    const long long item = (unit - first) / n;
-    shared[32 + 4 * w] = b;
-    shared[33 + 4 * w] = item;
-    shared[34 + 4 * w] = unit - first - item * n;
-  }
+  shared.before[t] = before;
+  if (t == 0) shared.before[kThreads] = total;
   __syncthreads();
-  Cursor c;
+  size = (total - 1) / p.chunks + 1;
   chunk = warp * gridDim.x + blockIdx.x;
-  c.rest = max(min(size, total - chunk * size), 0LL);
-  c.seq = c.item = c.u0 = c.n = c.keys = 0;
-  if (c.rest > 0) {
-    c.seq = (int)shared[32 + 4 * warp];
-    c.item = (int)shared[33 + 4 * warp];
-    c.u0 = (int)shared[34 + 4 * warp];
-    c.read_seq(p);
+  Cursor c;
+  c.rest = c.seq = c.item = c.u0 = c.n = c.keys = 0;
+  if (chunk > (total - 1) / size) return c;
+  const int unit = chunk * size;
+  c.rest = min(size, total - unit);
+  int owner = 0;                               // the thread whose units this one is among
+#pragma unroll
+  for (int i = 0; i < kThreads; i += 32) {
+    const uint32_t vote = __ballot_sync(0xffffffffu, shared.before[i + lane] <= unit && shared.before[i + lane + 1] > unit);
+    if (vote != 0) owner = i + __ffs(vote) - 1;
   }
+  int first = shared.before[owner];
+  for (c.seq = owner * each;; ++c.seq) {
+    c.read_seq(p);
+    const int all = p.items_per_seq * c.n;
+    if (unit - first < all) break;
+    first += all;
+  }
+  c.item = (unit - first) / c.n;
+  c.u0 = unit - first - c.item * c.n;
   return c;
 }
 
 __device__ __forceinline__ long long row_offset(const DecodeParams &p, const TensorRef &t, int seq, int head, int row) {
-  const int g = row / p.new_tokens, tok = row - g * p.new_tokens;
+  const int g = p.new_tokens == 1 ? row : row / p.new_tokens, tok = row - g * p.new_tokens;
   return seq * t.sb + (head * (long long)(p.heads / p.kv_heads) + g) * t.sh + tok * t.st;
 }
 __device__ __forceinline__ long long rem_index(const DecodeParams &p, int seq, int head, int row) {
-  const int g = row / p.new_tokens, tok = row - g * p.new_tokens;
+  const int g = p.new_tokens == 1 ? row : row / p.new_tokens, tok = row - g * p.new_tokens;
   return ((long long)seq * p.heads + head * (p.heads / p.kv_heads) + g) * p.new_tokens + tok;
-}
-
-// The page that holds a key, or -1 (and the status word) for an entry of the table that is none.
-__device__ __forceinline__ int page_of(const DecodeParams &p, int seq, int index) {
-  const int page = p.page_table[seq * p.table_stride + index];
-  if ((unsigned)page < (unsigned)p.num_pages) return page;
-  if (p.status != nullptr) {
-    p.status[0] = SB_DEV_BAD_PAGE;
-    p.status[1] = seq;
-  }
-  return -1;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool take) {
@@ -181,42 +177,66 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool t
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int n> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
 
-// A warp's loads, newest tile of a piece first, on into the next pieces.  The page of a tile is looked up when the tile before
-// it is copied.
+// A warp's loads, newest tile of a piece first, on into the next pieces.  32 entries of the page table are kept in a register of
+// the warp and read anew, ahead of their use, where a tile needs others.
 template <typename E> struct Feed {
   const DecodeParams &p;
   Cursor c;
   Piece w;
   int left = 0, number = 0;     // tiles of the piece that are still to be copied; how many pieces came before it
-  int page = -1;                // that lane l & 15's key of the next tile is in
+  int window = 0, top = -1;     // lane l has entry top - l of the sequence's row
   uint32_t bad = 0;             // a bit per stage: a page that is none
 
-  __device__ __forceinline__ Feed(const DecodeParams &p_, const Cursor &at) : p(p_), c(at) {
-    if (c.rest > 0) {
-      w = c.piece(p);
-      left = tiles_of(w);
-      E::prefetch_rows(p, w);
-      seek();
-    }
+  __device__ __forceinline__ Feed(const DecodeParams &p_, const Cursor &at) : p(p_), c(at) { open(); }
+  __device__ __forceinline__ void open() {
+    top = -1;
+    if (c.rest == 0) return;
+    w = c.piece(p);
+    left = tiles_of(w);
+    E::prefetch_rows(p, w);
   }
+  // By all lanes, before each copy but ahead of the one before it: the next tile's pages.
   __device__ __forceinline__ void seek() {
     while (left == 0) {
-      c.advance(p);
       if (c.rest == 0) return;
-      w = c.piece(p);
-      left = tiles_of(w);
+      c.advance(p);
       ++number;
-      E::prefetch_rows(p, w);
+      open();
     }
-    const int key = w.k0 + (left - 1) * kTileKeys + (threadIdx.x & 15);
-    page = key < w.k1 ? page_of(p, w.seq, key / p.page_size) : -1;
+    const int key0 = w.k0 + (left - 1) * kTileKeys;
+    const int low = page_index(p, key0);
+    if (top < 0 || low < top - 31) {
+      top = page_index(p, min(key0 + kTileKeys, w.k1) - 1);
+      const int entry = top - (int)(threadIdx.x & 31);
+      window = entry >= 0 ? p.page_table[w.seq * p.table_stride + entry] : -1;
+    }
+  }
+  // Lane l's key of the tile (l & 15): its page, -1 for none, and whether it should have one.
+  __device__ __forceinline__ int page_of(int key) {
+    const int page = __shfl_sync(0xffffffffu, window, top - page_index(p, min(key, w.k1 - 1)));
+    return (unsigned)page < (unsigned)p.num_pages ? page : -1;
   }
   __device__ __forceinline__ void copy(int stage, char *to) {
     if (left == 0) return;
-    const int key0 = w.k0 + --left * kTileKeys, key = key0 + (threadIdx.x & 15);
-    const bool wrong = __any_sync(0xffffffffu, key < w.k1 && page < 0);
+    const int key0 = w.k0 + --left * kTileKeys;
+    bool wrong;
+    if (p.page_shift >= 4 && key0 + kTileKeys <= w.k1) {         // a whole tile in one page
+      const int page = page_of(key0);
+      wrong = page < 0;
+      if (!wrong) E::copy_run(p, w, page, key0 & ((1 << p.page_shift) - 1), to);
+      else E::copy(p, w, -1, 0, to);
+    } else {
+      const int key = key0 + (threadIdx.x & 15);
+      int page = page_of(key);
+      wrong = __any_sync(0xffffffffu, page < 0);
+      if (key >= w.k1) page = -1;
+      E::copy(p, w, page, key - page_index(p, key) * p.page_size, to);
+    }
+    if (wrong && (threadIdx.x & 31) == 0 && p.status != nullptr) {
+      p.status[0] = SB_DEV_BAD_PAGE;
+      p.status[1] = w.seq;
+    }
     bad = (bad & ~(1u << stage)) | (uint32_t)wrong << stage;
-    E::copy(p, w, page, key - key / p.page_size * p.page_size, to);
     seek();
   }
   // what is left of piece `which` is not wanted; how many of its tiles that is
@@ -231,70 +251,87 @@ template <typename E> struct Feed {
 
 // The main kernel.  E, the engine: the shape of a stage (kWarps, kStages, kStage bytes), copy (16 keys and values of one
 // key head), start, tile (adds a stage up, keys newest first), gone (the rows' sticks are used up), finish (writes the sums out).
-template <typename E>
-__device__ __forceinline__ void decode_chunks(const DecodeParams &p, char *ring, long long *shared) {
-  int chunk;
-  long long size;
-  Cursor c = find_chunk<E::kWarps * 32>(p, chunk, size, shared);
+// One loop and one place for each of these: a short call runs through the code once, and its length counts there.
+template <typename E> __device__ __forceinline__ void decode_chunks(const DecodeParams &p, char *ring, ChunkShared<E::kWarps> &shared) {
+  int chunk, size;
+  Cursor c = find_chunk<E::kWarps>(p, chunk, size, shared);
   const int lane = threadIdx.x & 31;
   if (!p.by_item && lane == 0) p.notes[chunk] = make_int4(0, 0, 0, 0);
   if (c.rest == 0) return;
   char *stages = ring + (threadIdx.x >> 5) * E::kStages * E::kStage;
   Feed<E> feed(p, c);
-#pragma unroll
-  for (int i = 0; i < E::kStages - 1; ++i) {
-    feed.copy(i, stages + i * E::kStage);
-    cp_async_commit();
-  }
-  int at = 0, into = E::kStages - 1, number = 0;
-  for (bool first = true; c.rest > 0; first = false, ++number) {
-    const Piece w = c.piece(p);
-    E sum;
-    sum.start(p, w);
-    bool bad = c.keys < 0, done = false;
-    for (int left = tiles_of(w); left > 0; --left) {
-      cp_async_wait<E::kStages - 2>();
+  feed.seek();
+  Piece w;
+  E sum;
+  int at = 0, into = 0, fill = E::kStages, number = 0, left = 0;
+  bool fresh = true, bad = false, done = false, first = true;
+  for (;;) {
+    if (fill > 0) {              // a stage is free
       __syncwarp();
-      // (before the copy: it may set the same bit for a stage ahead only)
-      const bool wrong = feed.bad >> at & 1;
       feed.copy(into, stages + into * E::kStage);
       cp_async_commit();
+      into = into == E::kStages - 1 ? 0 : into + 1;
+      if (--fill > 0) continue;
+    }
+    if (fresh) {
+      w = c.piece(p);
+      sum.start(p, w);
+      left = tiles_of(w);
+      bad = c.keys < 0;
+      fresh = done = false;
+    }
+    if (left > 0) {
+      cp_async_wait<E::kStages - 1>();
+      __syncwarp();
       if (!done) {
-        bad |= wrong;
+        bad |= feed.bad >> at & 1;
         sum.tile(p, w, stages + at * E::kStage, w.k0 + (left - 1) * kTileKeys);
         if (!p.dense && sum.gone()) {
           done = true;           // the tiles that are on their way still come by
           left -= feed.drop(number);
         }
       }
+      --left;
       at = at == E::kStages - 1 ? 0 : at + 1;
-      into = into == E::kStages - 1 ? 0 : into + 1;
+      fill = 1;
     }
+    if (left > 0) continue;
     const int count = c.count();
     const bool whole = c.u0 == 0 && count == c.n;
-    const int slot = whole ? -1 : 2 * chunk + (first && c.u0 > 0 ? 0 : 1);
-    sum.finish(p, w, slot, bad);
-    if (c.u0 == 0 && lane == 0) {
-      const int pieces = whole ? 0 : 1 + (int)((c.n - count + size - 1) / size);
-      if (p.by_item) p.notes[c.seq * p.items_per_seq + c.item] = make_int4(c.seq, c.item, chunk, pieces);
-      else if (!whole) p.notes[chunk] = make_int4(c.seq, c.item, chunk, pieces);
-    }
-    if (c.keys < 0 && lane == 0 && p.status != nullptr) {
-      p.status[0] = SB_DEV_BAD_SEQ_LEN;
-      p.status[1] = c.seq;
+    sum.finish(p, w, whole ? -1 : 2 * chunk + (first && c.u0 > 0 ? 0 : 1), bad);
+    if (lane == 0) {
+      if (c.u0 == 0) {
+        const int pieces = whole ? 0 : 1 + (c.n - count + size - 1) / size;
+        if (p.by_item) p.notes[c.seq * p.items_per_seq + c.item] = make_int4(c.seq, c.item, chunk, pieces);
+        else if (!whole) p.notes[chunk] = make_int4(c.seq, c.item, chunk, pieces);
+      }
+      if (c.keys < 0 && p.status != nullptr) {
+        p.status[0] = SB_DEV_BAD_SEQ_LEN;
+        p.status[1] = c.seq;
+      }
     }
     c.advance(p);
+    if (c.rest == 0) break;
+    ++number;
+    first = false;
+    fresh = true;
   }
   cp_async_wait<0>();
 }
 
-// The result of row `row` of a piece's item: element `col` of it, or what is left of its stick.
-template <typename T> __device__ __forceinline__ void put_o(const DecodeParams &p, const Piece &w, int slot, int r, int col, float o) {
-  if (slot < 0)
-    reinterpret_cast<T *>(p.o.ptr)[row_offset(p, p.o, w.seq, w.head, w.row0 + r) + col] = from_f32<T>(o);
-  else
-    p.part_o[((long long)slot * p.rows_per_block + r) * p.head_dim + col] = o;
-}
+// Where row r of a piece's result goes: to o and rem where the piece is the whole item, else to its slot of the workspace.
+template <typename T> struct RowOut {
+  T *o;
+  float *part;
+  __device__ __forceinline__ RowOut(const DecodeParams &p, const Piece &w, int slot, int r) {
+    o = reinterpret_cast<T *>(p.o.ptr) + row_offset(p, p.o, w.seq, w.head, w.row0 + r);
+    part = slot < 0 ? nullptr : p.part_o + ((long long)slot * p.rows_per_block + r) * p.head_dim;
+  }
+  __device__ __forceinline__ void put(int col, float x) const {
+    if (part == nullptr) o[col] = from_f32<T>(x);
+    else part[col] = x;
+  }
+};
 template <typename T> __device__ __forceinline__ void put_rem(const DecodeParams &p, const Piece &w, int slot, int r, float left) {
   if (slot < 0)
     reinterpret_cast<T *>(p.rem)[rem_index(p, w.seq, w.head, w.row0 + r)] = from_f32<T>(exp2f(left));
@@ -302,13 +339,11 @@ template <typename T> __device__ __forceinline__ void put_rem(const DecodeParams
     p.part_l[(long long)slot * p.rows_per_block + r] = left;
 }
 // The rows of q that a piece will want: on their way to L2 while the piece before it is worked on.
-template <int kBytes> __device__ __forceinline__ void prefetch_q(const DecodeParams &p, const Piece &w, int esize) {
+__device__ __forceinline__ void prefetch_q(const DecodeParams &p, const Piece &w, int esize) {
   const int lane = threadIdx.x & 31;
-  const int lines = (p.head_dim * esize + kBytes - 1) / kBytes;
-  for (int e = lane; e < w.rows * lines; e += 32) {
-    const int r = e / lines, l = e - r * lines;
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(p.q.ptr + row_offset(p, p.q, w.seq, w.head, w.row0 + r) * esize + l * kBytes));
-  }
+  if (lane >= w.rows) return;
+  const char *row = p.q.ptr + row_offset(p, p.q, w.seq, w.head, w.row0 + lane) * esize;
+  for (int at = 0; at < p.head_dim * esize; at += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + at));
 }
 
 cudaError_t launch_decode_simt(const DecodeParams &p, int dtype, cudaStream_t s);
@@ -316,7 +351,7 @@ cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s);
 cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s);
 int decode_tc_rows(int rows, int head_dim);     // query rows per item
 int decode_simt_rows(int rows, int head_dim);
-int decode_tc_warps(int head_dim);              // warps per block; one block per SM
+int decode_tc_warps(int rows, int head_dim);    // warps per block for so many rows per item; one block per SM
 int decode_simt_warps(int head_dim);
 
 }  // namespace sb

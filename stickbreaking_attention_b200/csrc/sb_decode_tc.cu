@@ -29,12 +29,14 @@ using ptx::ex2;
 using ptx::rcp;
 using ptx::smem_u32;
 
-template <int kD> struct TcShape {                                  // kD: head_dim rounded up to 64, 128, 256
+// kD: head_dim rounded up to 64, 128, 256; kN: blocks of 8 query rows.  As many warps as their registers allow: a tile is a
+// chain of some 800 cycles (scores, scan over keys, weights, values), and other warps' tiles are what fills them.
+template <int kD, int kN> struct TcShape {
   static constexpr int kChunks = kD / 8;                            // 16-byte chunks of a row
   static constexpr int kHalf = kTileKeys * kD * 2;                  // bytes of a stage's keys (or values)
   static constexpr int kStage = 2 * kHalf;
-  static constexpr int kWarps = kD <= 128 ? 8 : 4;
-  static constexpr int kStages = kD <= 64 ? 6 : 3;
+  static constexpr int kWarps = kD == 256 ? 6 : kD / 64 * kN <= 2 ? 12 : 8;
+  static constexpr int kStages = 192 * 1024 / (kWarps * kStage);
   static constexpr int kBytes = kWarps * kStages * kStage;          // 192 KiB
 };
 
@@ -100,8 +102,8 @@ template <int kD> __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 }
 
 // The tensor-core engine.  kN: blocks of 8 query rows.
-template <typename T, int kD, int kN> struct TcEngine : TcShape<kD> {
-  using S = TcShape<kD>;
+template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
+  using S = TcShape<kD, kN>;
   using S::kHalf;
   uint32_t q[kN][kD / 16][2];
   float acc[kD / 16][kN][4];
@@ -109,15 +111,32 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD> {
   int limit[kN][2];
   bool real[kN][2];
 
-  __device__ static __forceinline__ void prefetch_rows(const DecodeParams &p, const Piece &w) { prefetch_q<128>(p, w, 2); }
+  __device__ static __forceinline__ void prefetch_rows(const DecodeParams &p, const Piece &w) { prefetch_q(p, w, 2); }
 
-  // Rows behind the piece's end, and columns behind head_dim, are zeros.
+  // 16 rows from slot `slot` of one page on; columns behind head_dim are zeros.
+  __device__ static __forceinline__ void copy_run(const DecodeParams &p, const Piece &w, int page, int slot, char *to) {
+    const int lane = threadIdx.x & 31;
+    constexpr int kAtOnce = 32 / S::kChunks;     // rows of one instruction
+    const int c = lane % S::kChunks, r0 = lane / S::kChunks;
+    const bool col = c * 8 < p.head_dim;
+    const char *k = p.k.ptr + (page * p.k.sp + w.head * p.k.sh + (slot + r0) * p.k.st) * 2 + (col ? c * 16 : 0);
+    const char *v = p.v.ptr + (page * p.v.sp + w.head * p.v.sh + (slot + r0) * p.v.st) * 2 + (col ? c * 16 : 0);
+    const long long k_step = kAtOnce * 2 * p.k.st, v_step = kAtOnce * 2 * p.v.st;
+    const uint32_t stage = smem_u32(to);
+#pragma unroll
+    for (int i = 0; i < kTileKeys / kAtOnce; ++i) {
+      const uint32_t at = stage + chunk_at<kD>(i * kAtOnce + r0, c);
+      cp_async16(at, k + i * k_step, col);
+      cp_async16(at + kHalf, v + i * v_step, col);
+    }
+  }
+  // Lane l has the page (-1: none, zeros) and slot of row l & 15.
   __device__ static __forceinline__ void copy(const DecodeParams &p, const Piece &w, int page, int slot, char *to) {
     const int lane = threadIdx.x & 31;
     const bool value = lane >= 16;               // lanes 16..31 hold the values' offsets
     const PagedRef &t = value ? p.v : p.k;
     const long long at = page < 0 ? -1 : (page * t.sp + w.head * t.sh + slot * t.st) * 2;
-    constexpr int kAtOnce = 32 / S::kChunks;     // rows of one instruction
+    constexpr int kAtOnce = 32 / S::kChunks;
     const int c = lane % S::kChunks, r0 = lane / S::kChunks;
     const bool col = c * 8 < p.head_dim;
     const uint32_t stage = smem_u32(to);
@@ -136,13 +155,13 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD> {
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       const int r = n * 8 + g;
-      const unsigned short *row = reinterpret_cast<const unsigned short *>(p.q.ptr) + row_offset(p, p.q, w.seq, w.head, w.row0 + min(r, w.rows - 1));
+      const char *row = p.q.ptr + 2 * row_offset(p, p.q, w.seq, w.head, w.row0 + min(r, w.rows - 1));
 #pragma unroll
       for (int i = 0; i < kD / 16; ++i)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int c = i * 16 + half * 8 + t * 2;
-          q[n][i][half] = r < w.rows && c < p.head_dim ? row[c] | (uint32_t)row[c + 1] << 16 : 0;
+          q[n][i][half] = r < w.rows && c < p.head_dim ? *reinterpret_cast<const uint32_t *>(row + 2 * c) : 0;
         }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -184,11 +203,11 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD> {
   __device__ __forceinline__ void tile(const DecodeParams &p, const Piece &w, char *to, int key0) {
     const uint32_t stage = smem_u32(to);
     const int lane = threadIdx.x & 31, g = lane >> 2;
-    float s[kN][4];
+    float s[kN][4], odd[kN][4];           // two chains of products
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
+      for (int j = 0; j < 4; ++j) s[n][j] = odd[n][j] = 0.0f;
     {
       const int r = 2 * (lane & 7) + ((lane >> 3) & 1), c = lane >> 4;
 #pragma unroll
@@ -196,7 +215,7 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD> {
         uint32_t a[4];
         ldsm4(stage + chunk_at<kD>(r, 2 * i + c), a);
 #pragma unroll
-        for (int n = 0; n < kN; ++n) mma<T>(s[n], a, q[n][i][0], q[n][i][1]);
+        for (int n = 0; n < kN; ++n) mma<T>(i & 1 ? odd[n] : s[n], a, q[n][i][0], q[n][i][1]);
       }
     }
     const float scale = p.scale * kLog2e;
@@ -208,7 +227,7 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD> {
         float beta[2], broken[2];
 #pragma unroll
         for (int key = 0; key < 2; ++key) {
-          const float x = s[n][2 * key + j] * scale, l = log2_1p(ex2(-fabsf(x)));
+          const float x = (s[n][2 * key + j] + odd[n][2 * key + j]) * scale, l = log2_1p(ex2(-fabsf(x)));
           const bool in = key0 + 2 * g + key < limit[n][j];
           beta[key] = in ? fminf(x, 0.0f) - l : -INFINITY;
           broken[key] = in ? -(fmaxf(x, 0.0f) + l) : 0.0f;
@@ -274,12 +293,13 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD> {
       for (int j = 0; j < 2; ++j) {
         const int r = n * 8 + t * 2 + j;
         if (r >= w.rows) continue;
+        const RowOut<T> out(p, w, slot, r);
 #pragma unroll
         for (int i = 0; i < kD / 16; ++i)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int c = i * 16 + half * 8 + g;
-            if (c < p.head_dim) put_o<T>(p, w, slot, r, c, bad ? nan : acc[i][n][half * 2 + j] * (1.0f / kScaleP<T>));
+            if (c < p.head_dim) out.put(c, bad ? nan : acc[i][n][half * 2 + j] * (1.0f / kScaleP<T>));
           }
         if (g == 0) put_rem<T>(p, w, slot, r, bad ? nan : (float)left[n][j]);
       }
@@ -287,15 +307,15 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD> {
 };
 
 template <typename T, int kD, int kN>
-__global__ void __launch_bounds__(TcShape<kD>::kWarps * 32, 1) decode_tc_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(TcShape<kD, kN>::kWarps * 32, 1) decode_tc_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) char ring[];
-  __shared__ long long shared[32 + 4 * TcShape<kD>::kWarps];
+  __shared__ ChunkShared<TcShape<kD, kN>::kWarps> shared;
   enter_kernel<true>();
   decode_chunks<TcEngine<T, kD, kN>>(p, ring, shared);
 }
 
 template <typename T, int kD, int kN> cudaError_t launch_one(const DecodeParams &p, cudaStream_t s) {
-  using S = TcShape<kD>;
+  using S = TcShape<kD, kN>;
   const auto kernel = decode_tc_kernel<T, kD, kN>;
   const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kBytes);
   if (e != cudaSuccess) return e;
@@ -315,7 +335,11 @@ int decode_tc_rows(int rows, int head_dim) {
   const int most = head_dim <= 64 ? 32 : head_dim <= 128 ? 16 : 8;
   return rows <= 8 || most == 8 ? 8 : rows <= 16 || most == 16 ? 16 : 32;
 }
-int decode_tc_warps(int head_dim) { return head_dim <= 128 ? TcShape<128>::kWarps : TcShape<256>::kWarps; }
+int decode_tc_warps(int rows, int head_dim) {
+  if (head_dim > 128) return TcShape<256, 1>::kWarps;
+  if (head_dim > 64) return rows == 8 ? TcShape<128, 1>::kWarps : TcShape<128, 2>::kWarps;
+  return rows == 8 ? TcShape<64, 1>::kWarps : rows == 16 ? TcShape<64, 2>::kWarps : TcShape<64, 4>::kWarps;
+}
 
 cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s) {
   return dtype == SB_DTYPE_BF16 ? launch_shape<__nv_bfloat16>(p, s) : launch_shape<__half>(p, s);

@@ -35,7 +35,7 @@ int check_pool(int dtype, int kv_heads, int head_dim, int page_size, int num_pag
 }
 
 struct DecodePlan {
-  int path, rows, rows_per_block, row_blocks, chunks;
+  int path, rows, rows_per_block, row_blocks, chunks, unit_shift;
   bool by_item;
   size_t part_o, part_l, bytes;
 };
@@ -55,11 +55,12 @@ int check_decode(const SbDecodeParams *p) {
 }
 
 int plan_decode(const SbDecodeParams *p, DecodePlan &pl) {
-  // whole 16-byte chunks in every row of the cache
+  // whole 16-byte chunks in every row of the cache, pairs of elements in q
   auto chunks = [](const SbCache &c) {
     return reinterpret_cast<uintptr_t>(c.ptr) % 16 == 0 && c.stride_page % 8 == 0 && c.stride_h % 8 == 0 && c.stride_t % 8 == 0;
   };
-  const bool tc = p->dtype != SB_DTYPE_F32 && !(p->flags & SB_FLAG_FORCE_SIMT) && p->head_dim % 8 == 0 && chunks(p->k) && chunks(p->v);
+  const bool q_pairs = reinterpret_cast<uintptr_t>(p->q.ptr) % 4 == 0 && p->q.stride_b % 2 == 0 && p->q.stride_h % 2 == 0 && p->q.stride_t % 2 == 0;
+  const bool tc = q_pairs && p->dtype != SB_DTYPE_F32 && !(p->flags & SB_FLAG_FORCE_SIMT) && p->head_dim % 8 == 0 && chunks(p->k) && chunks(p->v);
   pl.path = tc ? SB_PATH_TCGEN05 : SB_PATH_SIMT;
   pl.rows = p->heads / p->kv_heads * p->new_tokens;
   pl.rows_per_block = tc ? decode_tc_rows(pl.rows, p->head_dim) : decode_simt_rows(pl.rows, p->head_dim);
@@ -67,9 +68,12 @@ int plan_decode(const SbDecodeParams *p, DecodePlan &pl) {
   int sms = 0;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return fail(SB_ERR_CUDA, "SM count: %s", cudaGetErrorString(e));
-  pl.chunks = sms * (tc ? decode_tc_warps(p->head_dim) : decode_simt_warps(p->head_dim));
+  pl.chunks = sms * (tc ? decode_tc_warps(pl.rows_per_block, p->head_dim) : decode_simt_warps(p->head_dim));
   const long long items = (long long)p->batch * p->kv_heads * pl.row_blocks;
   pl.by_item = items < pl.chunks;
+  if (items > (1LL << 30)) return fail(SB_ERR_ARGUMENT, "batch * kv_heads too large");
+  pl.unit_shift = 6;                         // the units of all items have to be counted in 31 bits
+  while (items * (((long long)p->max_pages * p->page_size >> pl.unit_shift) + 1) > 0x7fffffffLL) ++pl.unit_shift;
   const size_t slots = 2 * (size_t)pl.chunks * pl.rows_per_block, notes = (size_t)(pl.by_item ? items : pl.chunks) * sizeof(int4);
   pl.part_o = (notes + 255) / 256 * 256;
   pl.part_l = pl.part_o + slots * p->head_dim * sizeof(float);
@@ -125,6 +129,10 @@ int run_decode(const SbDecodeParams *p, void *stream) {
   k.scale = p->logit_scale;
   k.chunks = pl.chunks;
   k.by_item = pl.by_item;
+  k.unit_shift = pl.unit_shift;
+  k.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (p->page_size == 1 << i) k.page_shift = i;
   k.items_per_seq = p->kv_heads * pl.row_blocks;
   char *ws = reinterpret_cast<char *>(p->workspace);
   k.notes = reinterpret_cast<int4 *>(ws);

@@ -414,7 +414,11 @@ std::tuple<Tensor, Tensor> decode(const Tensor &q_in, const Tensor &k, const Ten
   check_table(table, lens, k);
   TORCH_CHECK_VALUE(lens.size(0) == q_in.size(0), "seq_lens must have an entry for each sequence of q");
   c10::cuda::CUDAGuard guard(k.device());
-  const Tensor q = q_in.size(3) <= 1 || q_in.stride(3) == 1 ? q_in : q_in.contiguous();
+  // rows of pairs of elements (only an odd slice has others), so that the kernel does not depend on where q comes from
+  bool pairs = q_in.size(3) <= 1 || q_in.stride(3) == 1;
+  if (pairs && q_in.element_size() == 2 && q_in.size(3) % 8 == 0)
+    pairs = reinterpret_cast<uintptr_t>(q_in.data_ptr()) % 4 == 0 && stride_of(q_in, 0) % 2 == 0 && stride_of(q_in, 1) % 2 == 0 && stride_of(q_in, 2) % 2 == 0;
+  const Tensor q = pairs ? q_in : q_in.contiguous();
   const Tensor o = empty_as(q), rem = empty_cuda(q.sizes().slice(0, 3), q.scalar_type(), q);
   SbDecodeParams p;
   memset(&p, 0, sizeof(p));
