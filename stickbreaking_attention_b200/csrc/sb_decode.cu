@@ -40,13 +40,15 @@ template <int kCols> __device__ __forceinline__ int col_of(int lane, int i) {
 
 // The CUDA-core engine.  kRows: query rows (1, 2, 4, 8); kVec: bytes of a copy (fp32: 16 or 4; 16-bit types: 0, converted on the
 // way).  Lane l holds the scores of row 2 pair + (l & 1) at key l >> 1 of the tile: 16 keys and two rows fill a warp, and the scan
-// over keys takes four shuffles.  `left`: natural log of the stick that remains, 64-bit.
+// over keys takes four shuffles.  `left`: natural log of the stick that remains.
 template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtShape<kCols> {
   using S = SimtShape<kCols>;
   using S::kWidth;
+  using Ring = AsyncRing<S::kStages>;
+  static constexpr bool kBoxes = false;
   static constexpr int kPairs = (kRows + 1) / 2;
   float q[kRows][kCols], acc[kRows][kCols];
-  double left[kPairs];
+  LongSum left[kPairs];
   int limit[kPairs];
 
   __device__ static __forceinline__ void prefetch_rows(const DecodeParams &p, const Piece &w) { prefetch_q(p, w, sizeof(T)); }
@@ -93,7 +95,7 @@ template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtSh
     }
 #pragma unroll
     for (int pr = 0; pr < kPairs; ++pr) {
-      left[pr] = 0.0;
+      left[pr] = LongSum();
       limit[pr] = row_limit(p, w.keys, w.row0 + min(2 * pr + (lane & 1), w.rows - 1));
     }
   }
@@ -145,8 +147,8 @@ template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtSh
       }
       float later = __shfl_down_sync(0xffffffffu, sum, 2);
       if (lane >= 30) later = 0.0f;
-      a[pr] = in ? expf((fminf(x, 0.0f) - l1) + ((float)left[pr] + later)) : 0.0f;
-      left[pr] += (double)__shfl_sync(0xffffffffu, sum, lane & 1);
+      a[pr] = in ? expf((fminf(x, 0.0f) - l1) + (left[pr].sum + later)) : 0.0f;
+      left[pr].add(__shfl_sync(0xffffffffu, sum, lane & 1));
     }
     // a value that a row does not attend to is left out, not multiplied by 0: it may be no number
     const bool edge = key0 + kTileKeys > w.edge;
@@ -167,7 +169,7 @@ template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtSh
   __device__ __forceinline__ bool gone() const {
     bool all = true;
 #pragma unroll
-    for (int pr = 0; pr < kPairs; ++pr) all = all && left[pr] < (double)kStickGone * kLn2D;
+    for (int pr = 0; pr < kPairs; ++pr) all = all && left[pr].sum < kStickGone * (float)kLn2D;
     return __all_sync(0xffffffffu, all);
   }
 
@@ -186,7 +188,7 @@ template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtSh
     }
 #pragma unroll
     for (int pr = 0; pr < kPairs; ++pr)
-      if (lane < 2 && 2 * pr + lane < w.rows) put_rem<T>(p, w, slot, 2 * pr + lane, bad ? nan : (float)(left[pr] * kLog2eD));
+      if (lane < 2 && 2 * pr + lane < w.rows) put_rem<T>(p, w, slot, 2 * pr + lane, bad ? nan : left[pr].sum * kLog2e);
   }
 };
 
@@ -195,86 +197,105 @@ __global__ void __launch_bounds__(E::kWarps * 32, 1) decode_simt_kernel(const __
   extern __shared__ __align__(128) char ring[];
   __shared__ ChunkShared<E::kWarps> shared;
   enter_kernel<true>();
-  decode_chunks<E>(p, ring, shared);
+  decode_chunks<E>(p, ring, shared, typename E::Ring());
 }
 
-// Joins the pieces of the items that were cut, 128 elements (rows x columns) of an item at a time, four neighbours per lane, newest piece first.
-// Each warp has elements of its own (kTogether false), or all warps of a block have the same and take a run of the pieces each,
-// whose sums are joined like pieces: for items of very many pieces.
-constexpr int kJoinElements = 128;
-template <typename T, int kWarps, bool kTogether>
+// Joins the pieces of the items that were cut, up to 128 columns of one row at a time, newest piece first.  Each warp has such a
+// part of its own (kTogether 1), or kTogether warps have the same one and take a run of its pieces each, whose sums are joined
+// like pieces.  The sticks of 32 pieces are one scan over the lanes, which leaves a product and a sum per piece and column.
+constexpr int kJoinCols = 128, kJoinDeep = 8;
+
+// Eight pieces' columns in flight together.  (One statement: left to itself the compiler loads a few, adds them up, and only then
+// loads the next, which is a trip to L2 each.)
+__device__ __forceinline__ void load_eight(const float *const (&at)[8], float (&x)[8][4]) {
+  asm volatile(
+      "ld.global.f32 %0, [%32];\n\tld.global.f32 %1, [%32+128];\n\tld.global.f32 %2, [%32+256];\n\tld.global.f32 %3, [%32+384];\n\t"
+      "ld.global.f32 %4, [%33];\n\tld.global.f32 %5, [%33+128];\n\tld.global.f32 %6, [%33+256];\n\tld.global.f32 %7, [%33+384];\n\t"
+      "ld.global.f32 %8, [%34];\n\tld.global.f32 %9, [%34+128];\n\tld.global.f32 %10, [%34+256];\n\tld.global.f32 %11, [%34+384];\n\t"
+      "ld.global.f32 %12, [%35];\n\tld.global.f32 %13, [%35+128];\n\tld.global.f32 %14, [%35+256];\n\tld.global.f32 %15, [%35+384];\n\t"
+      "ld.global.f32 %16, [%36];\n\tld.global.f32 %17, [%36+128];\n\tld.global.f32 %18, [%36+256];\n\tld.global.f32 %19, [%36+384];\n\t"
+      "ld.global.f32 %20, [%37];\n\tld.global.f32 %21, [%37+128];\n\tld.global.f32 %22, [%37+256];\n\tld.global.f32 %23, [%37+384];\n\t"
+      "ld.global.f32 %24, [%38];\n\tld.global.f32 %25, [%38+128];\n\tld.global.f32 %26, [%38+256];\n\tld.global.f32 %27, [%38+384];\n\t"
+      "ld.global.f32 %28, [%39];\n\tld.global.f32 %29, [%39+128];\n\tld.global.f32 %30, [%39+256];\n\tld.global.f32 %31, [%39+384];"
+      : "=f"(x[0][0]), "=f"(x[0][1]), "=f"(x[0][2]), "=f"(x[0][3]), "=f"(x[1][0]), "=f"(x[1][1]), "=f"(x[1][2]), "=f"(x[1][3]),
+        "=f"(x[2][0]), "=f"(x[2][1]), "=f"(x[2][2]), "=f"(x[2][3]), "=f"(x[3][0]), "=f"(x[3][1]), "=f"(x[3][2]), "=f"(x[3][3]),
+        "=f"(x[4][0]), "=f"(x[4][1]), "=f"(x[4][2]), "=f"(x[4][3]), "=f"(x[5][0]), "=f"(x[5][1]), "=f"(x[5][2]), "=f"(x[5][3]),
+        "=f"(x[6][0]), "=f"(x[6][1]), "=f"(x[6][2]), "=f"(x[6][3]), "=f"(x[7][0]), "=f"(x[7][1]), "=f"(x[7][2]), "=f"(x[7][3])
+      : "l"(at[0]), "l"(at[1]), "l"(at[2]), "l"(at[3]), "l"(at[4]), "l"(at[5]), "l"(at[6]), "l"(at[7])
+      : "memory");
+}
+
+template <typename T, int kWarps, int kTogether>
 __global__ void __launch_bounds__(kWarps * 32) decode_join_kernel(const __grid_constant__ DecodeParams p) {
   enter_kernel<true>();
   const int4 note = p.notes[blockIdx.x];
   if (note.w == 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, team = warp / kTogether, member = warp % kTogether;
   const int head = p.row_blocks == 1 ? note.y : note.y / p.row_blocks, row0 = (note.y - head * p.row_blocks) * p.rows_per_block;
-  const int rows = min(p.rows - row0, p.rows_per_block), elements = rows * p.head_dim;
-  const int e0 = (kTogether ? blockIdx.y : blockIdx.y * kWarps + warp) * kJoinElements + lane * 4;
-  if (!kTogether && e0 - lane * 4 >= elements) return;
-  int r[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) r[j] = min(e0 + j, elements - 1) / p.head_dim;
+  const int rows = min(p.rows - row0, p.rows_per_block), segments = (p.head_dim + kJoinCols - 1) / kJoinCols;
+  const int job = blockIdx.y * (kWarps / kTogether) + team, r = segments == 1 ? job : job >> 1, col0 = segments == 1 ? 0 : (job & 1) * kJoinCols;
+  const bool real = r < rows;
+  if (kTogether == 1 && !real) return;
+  const int share = (note.w + kTogether - 1) / kTogether;
+  const int begin = real ? min(member * share, note.w) : 0, end = real ? min(begin + share, note.w) : 0;
+  // i-th piece from the newest on: the oldest is its chunk's last, the others are their chunk's first
+  const auto slot_of = [&](int i) { return 2LL * (note.z + note.w - 1 - i) + (i == note.w - 1 ? 1 : 0); };
   const long long part = (long long)p.rows_per_block * p.head_dim;
-  float o[4] = {}, left[4] = {};
-  const int share = kTogether ? (note.w + kWarps - 1) / kWarps : note.w;
-  const int begin = kTogether ? min(warp * share, note.w) : 0, end = min(begin + share, note.w);
-  constexpr int kDeep = 8;
-  for (int i0 = begin; i0 < end; i0 += kDeep) {
-    float x[kDeep][4], l[kDeep][4];
+  const float *const parts = p.part_o + r * p.head_dim + col0 + lane;
+  float o[4] = {}, left = 0.0f;
+  for (int i0 = begin; i0 < end; i0 += 32) {
+    const int n = min(end - i0, 32);
+    const float own = lane < n ? p.part_l[slot_of(i0 + lane) * p.rows_per_block + r] : 0.0f;
+    float x[kJoinDeep][4];
+    const float *at[kJoinDeep];
+    float sum = own;
 #pragma unroll
-    for (int k = 0; k < kDeep; ++k) {
-      const int i = min(i0 + k, end - 1), c = note.z + note.w - 1 - i;
-      const long long slot = 2 * (long long)c + (i == note.w - 1 ? 1 : 0);      // the oldest is its chunk's last piece, the others their chunk's first
-      const float *src = p.part_o + slot * part;
-      if (p.head_dim % 4 == 0) {
-        const float4 v = *reinterpret_cast<const float4 *>(src + min(e0, elements - 4));
-        x[k][0] = v.x; x[k][1] = v.y; x[k][2] = v.z; x[k][3] = v.w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[k][j] = src[min(e0 + j, elements - 1)];
-      }
-      l[k][0] = p.part_l[slot * p.rows_per_block + r[0]];
-#pragma unroll
-      for (int j = 1; j < 4; ++j) l[k][j] = p.head_dim % 4 == 0 ? l[k][0] : p.part_l[slot * p.rows_per_block + r[j]];
+    for (int d = 1; d < 32; d <<= 1) {
+      const float other = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += other;
     }
+    float before = __shfl_up_sync(0xffffffffu, sum, 1);
+    if (lane == 0) before = 0.0f;
+    const float stick = lane < n ? exp2_all(left + before) : 0.0f;      // what is left of the stick at the piece's newest end
+    left += __shfl_sync(0xffffffffu, sum, 31);
+    for (int k0 = 0; k0 < n; k0 += kJoinDeep) {
 #pragma unroll
-    for (int k = 0; k < kDeep; ++k) {
-      if (i0 + k >= end) break;
+      for (int k = 0; k < kJoinDeep; ++k) at[k] = parts + slot_of(min(i0 + k0 + k, end - 1)) * part;
+      load_eight(at, x);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float stick = exp2f(left[j]);
-        if (stick != 0.0f) o[j] += stick * x[k][j];        // (0 times what is no number stays out)
-        left[j] += l[k][j];
+      for (int k = 0; k < kJoinDeep; ++k) {
+        const float w = __shfl_sync(0xffffffffu, stick, (k0 + k) & 31);
+        const bool in = k0 + k < n && w != 0.0f;                        // (0 times what is no number stays out)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += in ? w * x[k][j] : 0.0f;
       }
     }
   }
-  if constexpr (kTogether) {
-    __shared__ float4 sums[kWarps][32], lefts[kWarps][32];
-    sums[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
-    lefts[warp][lane] = make_float4(left[0], left[1], left[2], left[3]);
+  if constexpr (kTogether > 1) {
+    __shared__ float sums[kWarps][4][32], lefts[kWarps];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[warp][j][lane] = o[j];
+    if (lane == 0) lefts[warp] = left;
     __syncthreads();
-    if (warp != 0) return;
+    if (member != 0 || !real) return;
+    left = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = left[j] = 0.0f;
-    for (int n = 0; n < kWarps; ++n) {
-      const float4 x = sums[n][lane], l = lefts[n][lane];
-      const float xs[4] = {x.x, x.y, x.z, x.w}, ls[4] = {l.x, l.y, l.z, l.w};
+    for (int j = 0; j < 4; ++j) o[j] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float stick = exp2f(left[j]);
-        if (stick != 0.0f) o[j] += stick * xs[j];
-        left[j] += ls[j];
-      }
+    for (int n = 0; n < kTogether; ++n) {
+      const float w = exp2_all(left);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += w != 0.0f ? w * sums[warp + n][j][lane] : 0.0f;
+      left += lefts[warp + n];
     }
   }
+  T *const out = reinterpret_cast<T *>(p.o.ptr) + row_offset(p, p.o, note.x, head, row0 + r);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int e = e0 + j, col = e - r[j] * p.head_dim;
-    if (e >= elements) continue;
-    reinterpret_cast<T *>(p.o.ptr)[row_offset(p, p.o, note.x, head, row0 + r[j]) + col] = from_f32<T>(o[j]);
-    if (col == 0) reinterpret_cast<T *>(p.rem)[rem_index(p, note.x, head, row0 + r[j])] = from_f32<T>(exp2f(left[j]));
+    const int c = col0 + lane + 32 * j;
+    if (c < p.head_dim) out[c] = from_f32<T>(o[j]);
   }
+  if (lane == 0 && col0 == 0) reinterpret_cast<T *>(p.rem)[rem_index(p, note.x, head, row0 + r)] = from_f32<T>(exp2f(left));
 }
 
 template <typename E> cudaError_t launch_engine(const DecodeParams &p, cudaStream_t s) {
@@ -315,15 +336,21 @@ cudaError_t launch_decode_simt(const DecodeParams &p, int dtype, cudaStream_t s)
   }
 }
 
+// The columns behind head_dim that a part reads (up to 127) lie in the next row, or behind the last one in the padding that the
+// workspace has there.  Few items are cut into many pieces each, and 32 warps share a part; where there are at least as many
+// items as chunks most have two pieces at most.
 cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s) {
   const long long items = (long long)p.batch * p.items_per_seq;
   const int notes = (int)(p.by_item ? items : p.chunks);
-  const int tiles = (p.rows_per_block * p.head_dim + kJoinElements - 1) / kJoinElements;
-  constexpr int kWide = 16, kNarrow = 4;
-  const bool wide = p.by_item && p.chunks >= kWide * items;      // sixteen pieces and more of an item, on the average
-  const dim3 grid(notes, wide ? tiles : (tiles + kNarrow - 1) / kNarrow);
-  auto go = [&](auto kernel, int threads) { return launch_kernel(kernel, grid, threads, 0, s, p); };
-#define SB_JOIN(T) wide ? go(decode_join_kernel<T, kWide, true>, kWide * 32) : go(decode_join_kernel<T, kNarrow, false>, kNarrow * 32)
+  const int jobs = p.rows_per_block * ((p.head_dim + kJoinCols - 1) / kJoinCols);
+  const int together = !p.by_item ? 1 : p.chunks >= 16 * items ? 32 : 4;
+  auto go = [&](auto kernel, int warps, int per_block) {
+    return launch_kernel(kernel, dim3(notes, (jobs + per_block - 1) / per_block), warps * 32, 0, s, p);
+  };
+#define SB_JOIN(T)                                               \
+  together == 32  ? go(decode_join_kernel<T, 32, 32>, 32, 1)     \
+  : together == 4 ? go(decode_join_kernel<T, 4, 4>, 4, 1)        \
+                  : go(decode_join_kernel<T, 4, 1>, 4, 4)
   switch (dtype) {
     case SB_DTYPE_F32: return SB_JOIN(float);
     case SB_DTYPE_BF16: return SB_JOIN(__nv_bfloat16);

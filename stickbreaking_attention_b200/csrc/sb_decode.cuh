@@ -4,8 +4,8 @@
 // L = log2 of the stick that is left at its oldest end.  Two neighbouring runs join to (o_new + 2^L_new o_old, L_new + L_old),
 // and this is associative, so the cache of a sequence can be cut anywhere.
 //
-// An item is (sequence, key head, block of query rows); its keys are counted in units of kUnit.  The units of all items lie
-// one behind the other on one axis, which is cut into equal chunks, one per WARP of the grid: a batch of ragged lengths is
+// An item is (sequence, key head, block of query rows); its keys are counted in units of one tile, 16 keys (or, in huge
+// batches, of so many that 31 bits count them).  The units of all items lie one behind the other on one axis, which is cut into equal chunks, one per WARP of the grid: a batch of ragged lengths is
 // spread evenly whatever the lengths are, only the device has to know them, and no warp ever waits for another.  A warp walks
 // through the pieces of its chunk without a pause: its loads run a ring of stages ahead of its arithmetic and go on into the next
 // piece while the last one's results are being written.  (With a block per chunk, its warps joined behind every piece, a piece
@@ -19,7 +19,7 @@
 
 namespace sb {
 
-constexpr int kUnit = 64, kTileKeys = 16;      // (units are 64 keys or, in huge batches, so many more that 31 bits count them)
+constexpr int kTileKeys = 16;
 // A weight below 2^-150 is exactly 0 in fp32, the smallest of whose numbers is 2^-149.
 constexpr float kStickGone = -150.0f;
 
@@ -38,13 +38,17 @@ struct DecodeParams {
   int batch, heads, kv_heads, new_tokens, head_dim, page_size, num_pages, max_pages;
   int rows, row_blocks, rows_per_block;   // query rows of a key head = heads / kv_heads * new_tokens, and how they are cut
   int items_per_seq;      // kv_heads * row_blocks
-  int page_shift;         // page_size = 1 << page_shift, or -1
+  int page_shift;         // page_size = 1 << page_shift, or -1: then key / page_size = (key * page_magic >> 32) >> page_post
+  unsigned page_magic;
+  int page_post;
   int attend_current, dense;
   int unit_shift;         // a unit is 1 << unit_shift keys
   float scale;
   int chunks;             // warps of the main kernel
   int by_item;            // notes are numbered by item, where there are fewer items than chunks; else by chunk
-  float *part_o, *part_l; // [2 * chunks][rows_per_block][head_dim], [2 * chunks][rows_per_block]
+  float *part_o, *part_l; // per slot (2 * chunks of them): rows_per_block x part_cols sums, rows_per_block x L
+  int part_cols;
+  int box_rows;           // tensor-core kernel with tensor maps: rows of a box (8, 16)
   int4 *notes;            // [min(items, chunks)]: an item that was cut: sequence, item of it, first chunk, pieces (0: none)
   int *status;
 };
@@ -59,7 +63,7 @@ __device__ __forceinline__ int units_of(const DecodeParams &p, int keys) {
   return keys <= 0 ? 1 : (int)(((unsigned)keys + (1u << p.unit_shift) - 1) >> p.unit_shift);
 }
 __device__ __forceinline__ int page_index(const DecodeParams &p, int key) {
-  return p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+  return p.page_shift >= 0 ? key >> p.page_shift : (int)(__umulhi((unsigned)key, p.page_magic) >> p.page_post);
 }
 // Keys that query row r (= head of the group * new_tokens + token) attends to are those before this one.
 __device__ __forceinline__ int row_limit(const DecodeParams &p, int keys, int r) {
@@ -177,6 +181,16 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool t
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int n> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
 
+// How a warp waits for the copies of its stages: cp.async ones in groups, of which the newest kStages - 1 may still be on their way.
+template <int kStages> struct AsyncRing {
+  __device__ __forceinline__ void filled() { cp_async_commit(); }
+  __device__ __forceinline__ bool wait(int) {
+    cp_async_wait<kStages - 1>();
+    return true;
+  }
+  __device__ __forceinline__ void end(bool) { cp_async_wait<0>(); }
+};
+
 // A warp's loads, newest tile of a piece first, on into the next pieces.  32 entries of the page table are kept in a register of
 // the warp and read anew, ahead of their use, where a tile needs others.
 template <typename E> struct Feed {
@@ -216,11 +230,23 @@ template <typename E> struct Feed {
     const int page = __shfl_sync(0xffffffffu, window, top - page_index(p, min(key, w.k1 - 1)));
     return (unsigned)page < (unsigned)p.num_pages ? page : -1;
   }
-  __device__ __forceinline__ void copy(int stage, char *to) {
+  // `ring`: how the engine's copies are waited for.
+  __device__ __forceinline__ void copy(int stage, char *to, typename E::Ring &ring) {
     if (left == 0) return;
     const int key0 = w.k0 + --left * kTileKeys;
     bool wrong;
-    if (p.page_shift >= 4 && key0 + kTileKeys <= w.k1) {         // a whole tile in one page
+    if constexpr (E::kBoxes) {
+      const int low = page_index(p, key0), page = page_of(key0), slot = key0 - low * p.page_size;
+      wrong = page < 0;
+      if (p.box_rows == kTileKeys) {                              // the tile is in one page
+        E::copy_boxes(p, w, page, slot, page, slot, !wrong, false, to, ring, stage);
+      } else {                                                    // two times eight rows
+        const bool two = key0 + 8 < w.k1;
+        const int next = page_index(p, key0 + 8), second = page_of(key0 + 8);
+        wrong = wrong || (two && second < 0);
+        E::copy_boxes(p, w, page, slot, second, key0 + 8 - next * p.page_size, !wrong, two, to, ring, stage);
+      }
+    } else if (p.page_shift >= 4 && key0 + kTileKeys <= w.k1) {   // a whole tile in one page
       const int page = page_of(key0);
       wrong = page < 0;
       if (!wrong) E::copy_run(p, w, page, key0 & ((1 << p.page_shift) - 1), to);
@@ -252,24 +278,25 @@ template <typename E> struct Feed {
 // The main kernel.  E, the engine: the shape of a stage (kWarps, kStages, kStage bytes), copy (16 keys and values of one
 // key head), start, tile (adds a stage up, keys newest first), gone (the rows' sticks are used up), finish (writes the sums out).
 // One loop and one place for each of these: a short call runs through the code once, and its length counts there.
-template <typename E> __device__ __forceinline__ void decode_chunks(const DecodeParams &p, char *ring, ChunkShared<E::kWarps> &shared) {
+template <typename E>
+__device__ __forceinline__ void decode_chunks(const DecodeParams &p, char *memory, ChunkShared<E::kWarps> &shared, typename E::Ring ring) {
   int chunk, size;
   Cursor c = find_chunk<E::kWarps>(p, chunk, size, shared);
   const int lane = threadIdx.x & 31;
   if (!p.by_item && lane == 0) p.notes[chunk] = make_int4(0, 0, 0, 0);
   if (c.rest == 0) return;
-  char *stages = ring + (threadIdx.x >> 5) * E::kStages * E::kStage;
+  char *stages = memory + (threadIdx.x >> 5) * E::kStages * E::kStage;
   Feed<E> feed(p, c);
   feed.seek();
   Piece w;
   E sum;
   int at = 0, into = 0, fill = E::kStages, number = 0, left = 0;
-  bool fresh = true, bad = false, done = false, first = true;
+  bool fresh = true, bad = false, done = false, first = true, failed = false;
   for (;;) {
     if (fill > 0) {              // a stage is free
       __syncwarp();
-      feed.copy(into, stages + into * E::kStage);
-      cp_async_commit();
+      feed.copy(into, stages + into * E::kStage, ring);
+      ring.filled();
       into = into == E::kStages - 1 ? 0 : into + 1;
       if (--fill > 0) continue;
     }
@@ -281,9 +308,19 @@ template <typename E> __device__ __forceinline__ void decode_chunks(const Decode
       fresh = done = false;
     }
     if (left > 0) {
-      cp_async_wait<E::kStages - 1>();
+      if (!failed && !ring.wait(at)) {       // a copy that does not come: nothing of this warp counts any more
+        failed = true;
+        if (p.status != nullptr) {
+          p.status[0] = SB_DEV_WAIT_TIMEOUT;
+          p.status[1] = at;
+        }
+      }
       __syncwarp();
-      if (!done) {
+      if (failed) {
+        bad = true;
+        feed.left = 0;
+        feed.c.rest = 0;
+      } else if (!done) {
         bad |= feed.bad >> at & 1;
         sum.tile(p, w, stages + at * E::kStage, w.k0 + (left - 1) * kTileKeys);
         if (!p.dense && sum.gone()) {
@@ -316,7 +353,7 @@ template <typename E> __device__ __forceinline__ void decode_chunks(const Decode
     first = false;
     fresh = true;
   }
-  cp_async_wait<0>();
+  ring.end(failed);
 }
 
 // Where row r of a piece's result goes: to o and rem where the piece is the whole item, else to its slot of the workspace.
@@ -325,7 +362,7 @@ template <typename T> struct RowOut {
   float *part;
   __device__ __forceinline__ RowOut(const DecodeParams &p, const Piece &w, int slot, int r) {
     o = reinterpret_cast<T *>(p.o.ptr) + row_offset(p, p.o, w.seq, w.head, w.row0 + r);
-    part = slot < 0 ? nullptr : p.part_o + ((long long)slot * p.rows_per_block + r) * p.head_dim;
+    part = slot < 0 ? nullptr : p.part_o + ((long long)slot * p.rows_per_block + r) * p.part_cols;
   }
   __device__ __forceinline__ void put(int col, float x) const {
     if (part == nullptr) o[col] = from_f32<T>(x);
@@ -346,11 +383,31 @@ __device__ __forceinline__ void prefetch_q(const DecodeParams &p, const Piece &w
   for (int at = 0; at < p.head_dim * esize; at += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + at));
 }
 
+// 2^x down to the smallest numbers (ptx::ex2 gives 0 for what is below 2^-126; weights go down to 2^-149, where a stick counts as
+// used up), to 2^-22 of itself.
+__device__ __forceinline__ float exp2_all(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A sum of many terms in 32 bits whose rounding errors are kept and added to the next term.
+struct LongSum {
+  float sum = 0.0f, lost = 0.0f;
+  __device__ __forceinline__ void add(float x) {
+    const float y = x + lost, s = sum + y;
+    lost = isinf(s) ? 0.0f : y - (s - sum);
+    sum = s;
+  }
+};
+
 cudaError_t launch_decode_simt(const DecodeParams &p, int dtype, cudaStream_t s);
 cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s);
-cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s);
+cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s);      // of the CUDA-core kernel's pieces
+cudaError_t launch_decode_tc_join(const DecodeParams &p, int dtype, cudaStream_t s);
 int decode_tc_rows(int rows, int head_dim);     // query rows per item
 int decode_simt_rows(int rows, int head_dim);
+int decode_tc_cols(int head_dim);               // columns of a piece in the workspace
 int decode_tc_warps(int rows, int head_dim);    // warps per block for so many rows per item; one block per SM
 int decode_simt_warps(int head_dim);
 

@@ -2,24 +2,30 @@
 //
 // What bounds it: every key and value is read once from HBM and takes part in 4 * rows operations per element, `rows` (query
 // heads per key head times new tokens) being 1 to 16 here: 1 to 16 operations per byte, where the GPU's ratio is 250.  So the
-// kernel is built around the copies: each warp has a ring of 16-key stages of its own, filled with cp.async, and no barrier
-// with other warps inside a piece; 192 KiB of stages per SM keep more bytes in flight than the latency of HBM needs (some 50 KiB).
+// kernel is built around the copies: each warp has a ring of 16-key stages of its own, and no barrier with other warps; 192 KiB of
+// stages per SM keep more bytes in flight than the latency of HBM needs (some 50 KiB).  Where pages hold a multiple of 8 tokens the
+// stages are filled by TMA, 64 columns x 16 (or two times 8) rows of one page and key head at a time, issued by one lane; other
+// pages take cp.async, a lane per 16 bytes.
 //
 // The products are mma.sync ones with the keys as the rows of the tile: S^T = K Q^T, O^T = V^T P^T, 16 keys by 8 queries.  A
 // tcgen05 tile takes 64 or 128 rows of one operand from shared memory that whole warps have to hand over; with 8 queries it
 // would be no less empty, and the products are not what takes the time.
 //
-// Row m of the score tile is key 2 m for m < 8, key 2 (m - 8) + 1 otherwise: a thread then holds two neighbouring keys of
-// two queries, and the sums over later keys take four shuffles per query.  Base 2 throughout:
+// A thread holds rows g and g + 8 of the score tile.  They are keys 2 g and 2 g + 1 of the 16 (for g >= 4 the other way round), so
+// that the sums over later keys take four shuffles per query; and the eight rows that one ldmatrix reads are eight different ones
+// modulo 8, which is what the 128-byte swizzle of TMA needs to put them into different banks.  Base 2 throughout:
 //   x = s log2(e) <q, k>,  u = 2^-|x|,  l = log2(1 + u);  log2 beta = min(x, 0) - l,  log2(1 - beta) = -max(x, 0) - l.
 // l comes from the series 2 atanh(u / (2 + u)) = 2 (w + w^3 / 3 + w^5 / 5 + ...), to 2^-22 of itself also where u is small: what
 // thousands of keys break off adds up.
 //
 // P enters the second product as the sum of two 16-bit numbers (16 or 22 bits): rounded once it would double the error that the
 // output's own rounding makes, and the second product of the pair is free.  In fp16 it is scaled by 2^15, since a weight of 1e-5
-// has few bits left there.  Scores, sums and the output's accumulators are 32-bit, the stick between tiles 64-bit.
+// has few bits left there.  Scores, sums and the output's accumulators are 32-bit, the stick between tiles 32-bit with what its sums lost.
+#include <cstring>
+#include <type_traits>
+
 #include "sb_decode.cuh"
-#include "sb_ptx.cuh"
+#include "sb_tc_common.cuh"
 
 namespace sb {
 
@@ -77,13 +83,6 @@ template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t x) { retur
 template <typename T> constexpr float kScaleP = 1.0f;
 template <> constexpr float kScaleP<__half> = 32768.0f;
 
-// (ptx::ex2 gives 0 for what is below 2^-126; weights go down to 2^-149, where the stick counts as used up)
-__device__ __forceinline__ float weight(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // log2(1 + u), 0 <= u <= 1; NaN for NaN.
 __device__ __forceinline__ float log2_1p(float u) {
   const float w = u * rcp(2.0f + u), t = w * w;
@@ -95,24 +94,75 @@ __device__ __forceinline__ float log2_1p(float u) {
   return 2.0f * kLog2e * w * s;
 }
 
-// Where chunk c of row r of a stage's keys or values lies: the eight even (or odd) rows that one ldmatrix reads are in eight
-// different places of the 128 bytes that the banks span.
-template <int kD> __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
-  return (uint32_t)(r * kD * 2 + ((c ^ ((r >> 1) & 7)) << 4));
+// Where chunk c of row r of a stage's keys or values lies: blocks of 64 columns, rows of 128 bytes, swizzled.
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return (uint32_t)((c >> 3) * (kTileKeys * 128) + r * 128 + (((c ^ r) & 7) << 4));
 }
+// The key of the tile that row g (second false) or g + 8 of a product's operand is.
+__device__ __forceinline__ int key_of(int g, bool second) { return 2 * g + (second != (g >= 4)); }
+
+struct Maps {
+  CUtensorMap k, v;
+};
 
 // The tensor-core engine.  kN: blocks of 8 query rows.
-template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
+// kTma: the stages are filled by TMA, an mbarrier per stage; else by cp.async.
+template <typename T, int kD, int kN, bool kTma> struct TcEngine : TcShape<kD, kN> {
   using S = TcShape<kD, kN>;
   using S::kHalf;
+  static constexpr bool kBoxes = kTma;
+  struct TmaRing {
+    const Maps *maps;
+    uint32_t bars;             // the warp's, one per stage
+    uint32_t phases = 0;       // a bit per stage: the parity to wait for next
+    uint32_t open = 0;         // a bit per stage: copies that nobody has waited for
+    __device__ __forceinline__ void filled() {}
+    __device__ __forceinline__ bool wait(int stage) {
+      const bool ok = ptx::mbar_wait(bars + 8 * stage, phases >> stage & 1);
+      phases ^= 1u << stage;
+      open &= ~(1u << stage);
+      return __all_sync(0xffffffffu, ok);
+    }
+    // the block's memory is not given back while copies into it are on their way
+    __device__ __forceinline__ void end(bool failed) {
+      for (int i = 0; i < S::kStages; ++i)
+        if (open >> i & 1) ptx::mbar_wait(bars + 8 * i, phases >> i & 1);
+      (void)failed;
+    }
+  };
+  using Ring = std::conditional_t<kTma, TmaRing, AsyncRing<S::kStages>>;
   uint32_t q[kN][kD / 16][2];
   float acc[kD / 16][kN][4];
-  double left[kN][2];
+  LongSum left[kN][2];
   int limit[kN][2];
   bool real[kN][2];
 
   __device__ static __forceinline__ void prefetch_rows(const DecodeParams &p, const Piece &w) { prefetch_q(p, w, 2); }
 
+  // Eight or sixteen rows from slot `slot` of page `page` on, and (two) eight more from another place.  Rows behind the page's end and
+  // columns behind head_dim are zeros.  !real: nothing, the stage counts as filled.
+  __device__ static __forceinline__ void copy_boxes(const DecodeParams &p, const Piece &w, int page, int slot, int page2, int slot2, bool real,
+                                                    bool two, char *to, TmaRing &ring, int stage_index) {
+    ring.open |= 1u << stage_index;
+    if ((threadIdx.x & 31) != 0) return;
+    const uint32_t bar = ring.bars + 8 * stage_index, stage = smem_u32(to);
+    if (!real) {
+      ptx::mbar_arrive(bar);
+      return;
+    }
+    const int rows = two ? kTileKeys : p.box_rows;
+    ptx::mbar_arrive_expect_tx(bar, 2 * kD * 2 * rows);
+#pragma unroll
+    for (int c = 0; c < kD / 64; ++c) {
+      const uint32_t at = stage + c * (kTileKeys * 128);
+      ptx::tma_load_4d(at, &ring.maps->k, bar, c * 64, slot, w.head, page);
+      ptx::tma_load_4d(at + kHalf, &ring.maps->v, bar, c * 64, slot, w.head, page);
+      if (two) {
+        ptx::tma_load_4d(at + 8 * 128, &ring.maps->k, bar, c * 64, slot2, w.head, page2);
+        ptx::tma_load_4d(at + 8 * 128 + kHalf, &ring.maps->v, bar, c * 64, slot2, w.head, page2);
+      }
+    }
+  }
   // 16 rows from slot `slot` of one page on; columns behind head_dim are zeros.
   __device__ static __forceinline__ void copy_run(const DecodeParams &p, const Piece &w, int page, int slot, char *to) {
     const int lane = threadIdx.x & 31;
@@ -125,7 +175,7 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
     const uint32_t stage = smem_u32(to);
 #pragma unroll
     for (int i = 0; i < kTileKeys / kAtOnce; ++i) {
-      const uint32_t at = stage + chunk_at<kD>(i * kAtOnce + r0, c);
+      const uint32_t at = stage + chunk_at(i * kAtOnce + r0, c);
       cp_async16(at, k + i * k_step, col);
       cp_async16(at + kHalf, v + i * v_step, col);
     }
@@ -145,8 +195,8 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
       const int r = i * kAtOnce + r0;
       const long long ak = __shfl_sync(0xffffffffu, at, r), av = __shfl_sync(0xffffffffu, at, r + 16);
       const bool take = ak >= 0 && col;
-      cp_async16(stage + chunk_at<kD>(r, c), take ? p.k.ptr + ak + c * 16 : p.k.ptr, take);
-      cp_async16(stage + kHalf + chunk_at<kD>(r, c), take ? p.v.ptr + av + c * 16 : p.v.ptr, take);
+      cp_async16(stage + chunk_at(r, c), take ? p.k.ptr + ak + c * 16 : p.k.ptr, take);
+      cp_async16(stage + kHalf + chunk_at(r, c), take ? p.v.ptr + av + c * 16 : p.v.ptr, take);
     }
   }
 
@@ -166,7 +216,7 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int query = n * 8 + t * 2 + j;
-        left[n][j] = 0.0;
+        left[n][j] = LongSum();
         real[n][j] = query < w.rows;
         limit[n][j] = row_limit(p, w.keys, w.row0 + min(query, w.rows - 1));
       }
@@ -177,15 +227,15 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
     }
   }
 
-  // O^T += V^T P^T, P as two 16-bit numbers; `b`: [row block][keys 2 m, 2 m + 1][high, low].  kSome: only for the queries whose
+  // O^T += V^T P^T, P as two 16-bit numbers; `b`: [row block][rows m, m + 8][high, low].  kSome: only for the queries whose
   // limits are in [low, high).
   template <bool kSome> __device__ __forceinline__ void add_values(uint32_t values, const uint32_t (&b)[kN][2][2], int low, int high) {
     const int lane = threadIdx.x & 31;
-    const int r = 2 * (lane & 7) + (lane >> 4), c = (lane >> 3) & 1;
+    const int r = key_of(lane & 7, lane >> 4), c = (lane >> 3) & 1;
 #pragma unroll
     for (int i = 0; i < kD / 16; ++i) {
       uint32_t a[4];
-      ldsm4_t(values + chunk_at<kD>(r, 2 * i + c), a);
+      ldsm4_t(values + chunk_at(r, 2 * i + c), a);
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
         float o[4];
@@ -209,11 +259,11 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[n][j] = odd[n][j] = 0.0f;
     {
-      const int r = 2 * (lane & 7) + ((lane >> 3) & 1), c = lane >> 4;
+      const int r = key_of(lane & 7, lane >> 3 & 1), c = lane >> 4;
 #pragma unroll
       for (int i = 0; i < kD / 16; ++i) {
         uint32_t a[4];
-        ldsm4(stage + chunk_at<kD>(r, 2 * i + c), a);
+        ldsm4(stage + chunk_at(r, 2 * i + c), a);
 #pragma unroll
         for (int n = 0; n < kN; ++n) mma<T>(i & 1 ? odd[n] : s[n], a, q[n][i][0], q[n][i][1]);
       }
@@ -223,15 +273,15 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {                  // queries 2 t + j; keys 2 g (s[n][j]) and 2 g + 1 (s[n][2 + j])
+      for (int j = 0; j < 2; ++j) {                  // queries 2 t + j; rows g (s[n][j]) and g + 8 (s[n][2 + j])
         float beta[2], broken[2];
 #pragma unroll
-        for (int key = 0; key < 2; ++key) {
-          const float x = (s[n][2 * key + j] + odd[n][2 * key + j]) * scale, l = log2_1p(ex2(-fabsf(x)));
-          const bool in = key0 + 2 * g + key < limit[n][j];
-          beta[key] = in ? fminf(x, 0.0f) - l : -INFINITY;
-          broken[key] = in ? -(fmaxf(x, 0.0f) + l) : 0.0f;
-          if (in && x != x) beta[key] = broken[key] = x;      // (fminf and fmaxf drop a NaN)
+        for (int row = 0; row < 2; ++row) {
+          const float x = (s[n][2 * row + j] + odd[n][2 * row + j]) * scale, l = log2_1p(ex2(-fabsf(x)));
+          const bool in = key0 + key_of(g, row) < limit[n][j];
+          beta[row] = in ? fminf(x, 0.0f) - l : -INFINITY;
+          broken[row] = in ? -(fmaxf(x, 0.0f) + l) : 0.0f;
+          if (in && x != x) beta[row] = broken[row] = x;      // (fminf and fmaxf drop a NaN)
         }
         const float both = broken[0] + broken[1];
         float later = __shfl_down_sync(0xffffffffu, both, 4);
@@ -241,10 +291,11 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
           const float other = __shfl_down_sync(0xffffffffu, later, d);
           if (lane + d < 32) later += other;
         }
-        const float base = (float)left[n][j] + later;
-        a[n][2 + j] = weight(beta[1] + base) * kScaleP<T>;
-        a[n][j] = weight(beta[0] + (base + broken[1])) * kScaleP<T>;
-        left[n][j] += (double)__shfl_sync(0xffffffffu, later + both, lane & 3);
+        const float base = left[n][j].sum + later;
+        // the older key of the two comes behind the newer one
+        a[n][j] = exp2_all(beta[0] + (base + (g < 4 ? broken[1] : 0.0f))) * kScaleP<T>;
+        a[n][2 + j] = exp2_all(beta[1] + (base + (g < 4 ? 0.0f : broken[0]))) * kScaleP<T>;
+        left[n][j].add(__shfl_sync(0xffffffffu, later + both, lane & 3));
       }
     }
     // the two 16-bit parts of the weights, moved from (key, query) to (query, key)
@@ -252,11 +303,11 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int key = 0; key < 2; ++key) {
-        const uint32_t hi = pack<T>(a[n][2 * key], a[n][2 * key + 1]);
+      for (int row = 0; row < 2; ++row) {
+        const uint32_t hi = pack<T>(a[n][2 * row], a[n][2 * row + 1]);
         const float2 back = unpack<T>(hi);
-        b[n][key][0] = transpose8x8(hi);
-        b[n][key][1] = transpose8x8(pack<T>(a[n][2 * key] - back.x, a[n][2 * key + 1] - back.y));
+        b[n][row][0] = transpose8x8(hi);
+        b[n][row][1] = transpose8x8(pack<T>(a[n][2 * row] - back.x, a[n][2 * row + 1] - back.y));
       }
     const uint32_t values = stage + kHalf;
     if (key0 + kTileKeys <= w.edge) {
@@ -265,14 +316,19 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
     }
     // Some rows do not attend to some keys of the tile.  Those keys' values are taken out, not multiplied by 0 (they may be no
     // numbers): the rows take their turns from the longest reach down, and the values that are out of reach become zeros.
-    add_values<true>(values, b, key0 + kTileKeys, 0x7fffffff);
+    const auto clear = [&](int row) {
+      if (lane < S::kChunks)
+        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(values + chunk_at(row, lane)), "r"(0) : "memory");
+    };
+    if (w.k1 >= key0 + kTileKeys) add_values<true>(values, b, key0 + kTileKeys, 0x7fffffff);
+    for (int key = w.k1 + 1; key < key0 + kTileKeys; ++key) clear(key - key0);
     for (int reach = min(w.k1, key0 + kTileKeys - 1); reach >= max(w.edge, key0 + 1); --reach) {
       __syncwarp();
-      if (lane < S::kChunks)
-        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(values + chunk_at<kD>(reach - key0, lane)), "r"(0) : "memory");
+      clear(reach - key0);
       __syncwarp();
       add_values<true>(values, b, reach, reach + 1);
     }
+    if constexpr (kTma) ptx::fence_proxy_async_smem();      // the stage's next copies come behind these stores
   }
 
   __device__ __forceinline__ bool gone() const {
@@ -280,52 +336,203 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) all = all && (!real[n][j] || left[n][j] < (double)kStickGone);
+      for (int j = 0; j < 2; ++j) all = all && (!real[n][j] || left[n][j].sum < kStickGone);
     return __all_sync(0xffffffffu, all);
   }
 
+  // A piece that is not the whole item leaves its accumulators as they lie in the registers, 16 bytes a lane, for the join kernel.
   __device__ __forceinline__ void finish(const DecodeParams &p, const Piece &w, int slot, bool bad) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const float nan = __int_as_float(0x7fffffff);
+    if (bad) {
 #pragma unroll
-    for (int n = 0; n < kN; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = n * 8 + t * 2 + j;
-        if (r >= w.rows) continue;
-        const RowOut<T> out(p, w, slot, r);
+      for (int n = 0; n < kN; ++n) {
 #pragma unroll
         for (int i = 0; i < kD / 16; ++i)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int c = i * 16 + half * 8 + g;
-            if (c < p.head_dim) out.put(c, bad ? nan : acc[i][n][half * 2 + j] * (1.0f / kScaleP<T>));
-          }
-        if (g == 0) put_rem<T>(p, w, slot, r, bad ? nan : (float)left[n][j]);
+          for (int j = 0; j < 4; ++j) acc[i][n][j] = nan;
+        left[n][0].sum = left[n][1].sum = nan;
       }
+    }
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const int r = n * 8 + t * 2;
+      if (r >= w.rows) continue;
+      if (slot < 0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (r + j >= w.rows) continue;
+          T *const out = reinterpret_cast<T *>(p.o.ptr) + row_offset(p, p.o, w.seq, w.head, w.row0 + r + j);
+#pragma unroll
+          for (int i = 0; i < kD / 16; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int c = i * 16 + half * 8 + g;
+              if (c < p.head_dim) out[c] = from_f32<T>(acc[i][n][half * 2 + j] * (1.0f / kScaleP<T>));
+            }
+          if (g == 0) put_rem<T>(p, w, slot, r + j, left[n][j].sum);
+        }
+      } else {
+        float4 *const part = reinterpret_cast<float4 *>(p.part_o + (long long)slot * (kN * 8 * kD)) + n * (kD / 16) * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < kD / 16; ++i) part[i * 32] = make_float4(acc[i][n][0], acc[i][n][1], acc[i][n][2], acc[i][n][3]);
+        if (g == 0) *reinterpret_cast<float2 *>(p.part_l + (long long)slot * (kN * 8) + r) = make_float2(left[n][0].sum, left[n][1].sum);
+      }
+    }
   }
 };
 
-template <typename T, int kD, int kN>
-__global__ void __launch_bounds__(TcShape<kD, kN>::kWarps * 32, 1) decode_tc_kernel(const __grid_constant__ DecodeParams p) {
-  extern __shared__ __align__(128) char ring[];
-  __shared__ ChunkShared<TcShape<kD, kN>::kWarps> shared;
-  enter_kernel<true>();
-  decode_chunks<TcEngine<T, kD, kN>>(p, ring, shared);
+template <typename T, int kD, int kN, bool kTma>
+__global__ void __launch_bounds__(TcShape<kD, kN>::kWarps * 32, 1)
+    decode_tc_kernel(const __grid_constant__ DecodeParams p, const __grid_constant__ Maps maps) {
+  using S = TcShape<kD, kN>;
+  using E = TcEngine<T, kD, kN, kTma>;
+  extern __shared__ __align__(1024) char ring[];
+  __shared__ ChunkShared<S::kWarps> shared;
+  if constexpr (kTma) {
+    __shared__ uint64_t bars[S::kWarps][S::kStages];
+    const uint32_t mine = smem_u32(bars[threadIdx.x >> 5]);
+    if ((threadIdx.x & 31) == 0) {
+      ptx::prefetch_tensormap(&maps.k);
+      ptx::prefetch_tensormap(&maps.v);
+      for (int i = 0; i < S::kStages; ++i) ptx::mbar_init(mine + 8 * i, 1);
+      ptx::fence_barrier_init();
+      ptx::fence_proxy_async_smem();
+    }
+    __syncwarp();
+    enter_kernel<true>();
+    decode_chunks<E>(p, ring, shared, typename E::Ring{&maps, mine});
+  } else {
+    enter_kernel<true>();
+    decode_chunks<E>(p, ring, shared, typename E::Ring());
+  }
 }
 
-template <typename T, int kD, int kN> cudaError_t launch_one(const DecodeParams &p, cudaStream_t s) {
+// Joins the pieces of the items that were cut, newest first, 8 rows x 16 columns at a time as a warp's registers held them: a lane has two
+// rows and two columns.  Each warp has such a part of its own (kTogether 1), or kTogether warps have the same one and take a run
+// of its pieces each, whose sums are joined like pieces.
+constexpr int kJoinDeep = 8;
+// Eight pieces in flight together.  (One statement: left to itself the compiler loads a few, adds them up, and only then loads the
+// next, which is a trip to L2 each.)
+__device__ __forceinline__ void load_eight(const float4 *const (&at)[8], float4 (&x)[8]) {
+  asm volatile(
+      "ld.global.v4.f32 {%0,%1,%2,%3}, [%32];\n\tld.global.v4.f32 {%4,%5,%6,%7}, [%33];\n\t"
+      "ld.global.v4.f32 {%8,%9,%10,%11}, [%34];\n\tld.global.v4.f32 {%12,%13,%14,%15}, [%35];\n\t"
+      "ld.global.v4.f32 {%16,%17,%18,%19}, [%36];\n\tld.global.v4.f32 {%20,%21,%22,%23}, [%37];\n\t"
+      "ld.global.v4.f32 {%24,%25,%26,%27}, [%38];\n\tld.global.v4.f32 {%28,%29,%30,%31}, [%39];"
+      : "=f"(x[0].x), "=f"(x[0].y), "=f"(x[0].z), "=f"(x[0].w), "=f"(x[1].x), "=f"(x[1].y), "=f"(x[1].z), "=f"(x[1].w),
+        "=f"(x[2].x), "=f"(x[2].y), "=f"(x[2].z), "=f"(x[2].w), "=f"(x[3].x), "=f"(x[3].y), "=f"(x[3].z), "=f"(x[3].w),
+        "=f"(x[4].x), "=f"(x[4].y), "=f"(x[4].z), "=f"(x[4].w), "=f"(x[5].x), "=f"(x[5].y), "=f"(x[5].z), "=f"(x[5].w),
+        "=f"(x[6].x), "=f"(x[6].y), "=f"(x[6].z), "=f"(x[6].w), "=f"(x[7].x), "=f"(x[7].y), "=f"(x[7].z), "=f"(x[7].w)
+      : "l"(at[0]), "l"(at[1]), "l"(at[2]), "l"(at[3]), "l"(at[4]), "l"(at[5]), "l"(at[6]), "l"(at[7])
+      : "memory");
+}
+__device__ __forceinline__ void load_eight(const float2 *const (&at)[8], float2 (&x)[8]) {
+  asm volatile(
+      "ld.global.v2.f32 {%0,%1}, [%16];\n\tld.global.v2.f32 {%2,%3}, [%17];\n\tld.global.v2.f32 {%4,%5}, [%18];\n\tld.global.v2.f32 {%6,%7}, [%19];\n\t"
+      "ld.global.v2.f32 {%8,%9}, [%20];\n\tld.global.v2.f32 {%10,%11}, [%21];\n\tld.global.v2.f32 {%12,%13}, [%22];\n\tld.global.v2.f32 {%14,%15}, [%23];"
+      : "=f"(x[0].x), "=f"(x[0].y), "=f"(x[1].x), "=f"(x[1].y), "=f"(x[2].x), "=f"(x[2].y), "=f"(x[3].x), "=f"(x[3].y),
+        "=f"(x[4].x), "=f"(x[4].y), "=f"(x[5].x), "=f"(x[5].y), "=f"(x[6].x), "=f"(x[6].y), "=f"(x[7].x), "=f"(x[7].y)
+      : "l"(at[0]), "l"(at[1]), "l"(at[2]), "l"(at[3]), "l"(at[4]), "l"(at[5]), "l"(at[6]), "l"(at[7])
+      : "memory");
+}
+// Adds a run of keys (x, l) behind what is summed up in (o, left).  (0 times what is no number stays out.)
+__device__ __forceinline__ void add_behind(float4 &o, float2 &left, const float4 &x, const float2 &l) {
+  const float a = exp2_all(left.x), b = exp2_all(left.y);
+  o.x += a != 0.0f ? a * x.x : 0.0f;
+  o.y += b != 0.0f ? b * x.y : 0.0f;
+  o.z += a != 0.0f ? a * x.z : 0.0f;
+  o.w += b != 0.0f ? b * x.w : 0.0f;
+  left.x += l.x;
+  left.y += l.y;
+}
+
+template <typename T, int kWarps, int kTogether>
+__global__ void __launch_bounds__(kWarps * 32) decode_tc_join_kernel(const __grid_constant__ DecodeParams p) {
+  enter_kernel<true>();
+  const int4 note = p.notes[blockIdx.x];
+  if (note.w == 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, team = warp / kTogether, member = warp % kTogether;
+  const int head = p.row_blocks == 1 ? note.y : note.y / p.row_blocks, row0 = (note.y - head * p.row_blocks) * p.rows_per_block;
+  const int rows = min(p.rows - row0, p.rows_per_block), blocks = p.part_cols / 16;
+  const int job = blockIdx.y * (kWarps / kTogether) + team, n = job / blocks, i = job - n * blocks;
+  const int r = n * 8 + (lane & 3) * 2, c = i * 16 + (lane >> 2);
+  const bool real = r < rows && i * 16 < p.head_dim;      // (columns behind head_dim are there, as zeros)
+  const int share = (note.w + kTogether - 1) / kTogether;
+  const int begin = min(member * share, note.w), end = min(begin + share, note.w);
+  // k-th piece from the newest on: the oldest is its chunk's last, the others are their chunk's first
+  const auto slot_of = [&](int k) { return 2LL * (note.z + note.w - 1 - k) + (k == note.w - 1 ? 1 : 0); };
+  const int slot_size = p.rows_per_block * p.part_cols;
+  const float4 *const parts = reinterpret_cast<const float4 *>(p.part_o) + job * 32 + lane;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float2 left = make_float2(0.0f, 0.0f);
+  if (real) {
+    for (int k0 = begin; k0 < end; k0 += kJoinDeep) {
+      const float4 *at[kJoinDeep];
+      const float2 *l_at[kJoinDeep];
+      float4 x[kJoinDeep];
+      float2 l[kJoinDeep];
+#pragma unroll
+      for (int k = 0; k < kJoinDeep; ++k) {
+        const long long slot = slot_of(min(k0 + k, end - 1));
+        at[k] = parts + slot * (slot_size / 4);
+        l_at[k] = reinterpret_cast<const float2 *>(p.part_l + slot * p.rows_per_block + r);
+      }
+      load_eight(at, x);
+      load_eight(l_at, l);
+#pragma unroll
+      for (int k = 0; k < kJoinDeep; ++k)
+        if (k0 + k < end) add_behind(o, left, x[k], l[k]);
+    }
+  }
+  if constexpr (kTogether > 1) {
+    __shared__ float4 sums[kWarps][32];
+    __shared__ float2 lefts[kWarps][32];
+    sums[warp][lane] = o;
+    lefts[warp][lane] = left;
+    __syncthreads();
+    if (member != 0) return;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    left = make_float2(0.0f, 0.0f);
+#pragma unroll 8
+    for (int m = 0; m < kTogether; ++m) add_behind(o, left, sums[warp + m][lane], lefts[warp + m][lane]);
+  }
+  if (!real) return;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    if (r + j >= rows) break;
+    T *const out = reinterpret_cast<T *>(p.o.ptr) + row_offset(p, p.o, note.x, head, row0 + r + j);
+    if (c < p.head_dim) out[c] = from_f32<T>((j ? o.y : o.x) * (1.0f / kScaleP<T>));
+    if (c + 8 < p.head_dim) out[c + 8] = from_f32<T>((j ? o.w : o.z) * (1.0f / kScaleP<T>));
+    if (c == 0) reinterpret_cast<T *>(p.rem)[rem_index(p, note.x, head, row0 + r + j)] = from_f32<T>(exp2f(j ? left.y : left.x));
+  }
+}
+
+template <typename T, int kD, int kN, bool kTma> cudaError_t launch_one(const DecodeParams &p, const Maps &maps, cudaStream_t s) {
   using S = TcShape<kD, kN>;
-  const auto kernel = decode_tc_kernel<T, kD, kN>;
+  const auto kernel = decode_tc_kernel<T, kD, kN, kTma>;
   const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3(p.chunks / S::kWarps), S::kWarps * 32, S::kBytes, s, p);
+  return launch_kernel(kernel, dim3(p.chunks / S::kWarps), S::kWarps * 32, S::kBytes, s, p, maps);
 }
-template <typename T> cudaError_t launch_shape(const DecodeParams &p, cudaStream_t s) {
+template <typename T, bool kTma> cudaError_t launch_shape(const DecodeParams &p, const Maps &maps, cudaStream_t s) {
   const int n = p.rows_per_block / 8;
-  if (p.head_dim <= 64) return n == 1 ? launch_one<T, 64, 1>(p, s) : n == 2 ? launch_one<T, 64, 2>(p, s) : launch_one<T, 64, 4>(p, s);
-  if (p.head_dim <= 128) return n == 1 ? launch_one<T, 128, 1>(p, s) : launch_one<T, 128, 2>(p, s);
-  return launch_one<T, 256, 1>(p, s);
+  if (p.head_dim <= 64)
+    return n == 1 ? launch_one<T, 64, 1, kTma>(p, maps, s) : n == 2 ? launch_one<T, 64, 2, kTma>(p, maps, s) : launch_one<T, 64, 4, kTma>(p, maps, s);
+  if (p.head_dim <= 128) return n == 1 ? launch_one<T, 128, 1, kTma>(p, maps, s) : launch_one<T, 128, 2, kTma>(p, maps, s);
+  return launch_one<T, 256, 1, kTma>(p, maps, s);
+}
+template <typename T> cudaError_t launch_type(const DecodeParams &p, const Maps &maps, cudaStream_t s) {
+  return p.box_rows != 0 ? launch_shape<T, true>(p, maps, s) : launch_shape<T, false>(p, maps, s);
+}
+
+// (head_dim, slots, heads, pages); the stride of an axis of one element is the caller's to leave as it likes.
+cudaError_t cache_map(CUtensorMap *map, const PagedRef &t, const DecodeParams &p, int dtype) {
+  const long long st = p.page_size > 1 ? t.st : (p.head_dim + 7) / 8 * 8, sh = p.kv_heads > 1 ? t.sh : st * p.page_size,
+                  sp = p.num_pages > 1 ? t.sp : sh * p.kv_heads;
+  const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.page_size, (cuuint64_t)p.kv_heads, (cuuint64_t)p.num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sp * 2};
+  return encode_tile_map(map, t.ptr, dims, strides, p.box_rows, dtype);
 }
 
 }  // namespace
@@ -335,14 +542,38 @@ int decode_tc_rows(int rows, int head_dim) {
   const int most = head_dim <= 64 ? 32 : head_dim <= 128 ? 16 : 8;
   return rows <= 8 || most == 8 ? 8 : rows <= 16 || most == 16 ? 16 : 32;
 }
+int decode_tc_cols(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 int decode_tc_warps(int rows, int head_dim) {
   if (head_dim > 128) return TcShape<256, 1>::kWarps;
   if (head_dim > 64) return rows == 8 ? TcShape<128, 1>::kWarps : TcShape<128, 2>::kWarps;
   return rows == 8 ? TcShape<64, 1>::kWarps : rows == 16 ? TcShape<64, 2>::kWarps : TcShape<64, 4>::kWarps;
 }
 
-cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s) {
-  return dtype == SB_DTYPE_BF16 ? launch_shape<__nv_bfloat16>(p, s) : launch_shape<__half>(p, s);
+cudaError_t launch_decode_tc(const DecodeParams &params, int dtype, cudaStream_t s) {
+  DecodeParams p = params;
+  p.box_rows = p.page_size % 16 == 0 ? 16 : p.page_size % 8 == 0 ? 8 : 0;
+  Maps maps;
+  memset(&maps, 0, sizeof(maps));
+  cudaError_t e = cudaSuccess;
+  if (p.box_rows != 0 && ((e = cache_map(&maps.k, p.k, p, dtype)) != cudaSuccess || (e = cache_map(&maps.v, p.v, p, dtype)) != cudaSuccess)) return e;
+  return dtype == SB_DTYPE_BF16 ? launch_type<__nv_bfloat16>(p, maps, s) : launch_type<__half>(p, maps, s);
+}
+
+// Few items are cut into many pieces each, and 32 or 4 warps share a part; where there are at least as many items as chunks most
+// have two pieces at most.
+cudaError_t launch_decode_tc_join(const DecodeParams &p, int dtype, cudaStream_t s) {
+  const long long items = (long long)p.batch * p.items_per_seq;
+  const int notes = (int)(p.by_item ? items : p.chunks), jobs = p.rows_per_block / 8 * (p.part_cols / 16);
+  const int together = !p.by_item ? 1 : p.chunks >= 16 * items ? 32 : 4;
+  auto go = [&](auto kernel, int warps, int per_block) {
+    return launch_kernel(kernel, dim3(notes, (jobs + per_block - 1) / per_block), warps * 32, 0, s, p);
+  };
+#define SB_JOIN(T)                                                  \
+  together == 32  ? go(decode_tc_join_kernel<T, 32, 32>, 32, 1)     \
+  : together == 4 ? go(decode_tc_join_kernel<T, 4, 4>, 4, 1)        \
+                  : go(decode_tc_join_kernel<T, 4, 1>, 4, 4)
+  return dtype == SB_DTYPE_BF16 ? SB_JOIN(__nv_bfloat16) : SB_JOIN(__half);
+#undef SB_JOIN
 }
 
 }  // namespace sb

@@ -35,7 +35,7 @@ int check_pool(int dtype, int kv_heads, int head_dim, int page_size, int num_pag
 }
 
 struct DecodePlan {
-  int path, rows, rows_per_block, row_blocks, chunks, unit_shift;
+  int path, rows, rows_per_block, row_blocks, chunks, unit_shift, part_cols;
   bool by_item;
   size_t part_o, part_l, bytes;
 };
@@ -55,9 +55,11 @@ int check_decode(const SbDecodeParams *p) {
 }
 
 int plan_decode(const SbDecodeParams *p, DecodePlan &pl) {
-  // whole 16-byte chunks in every row of the cache, pairs of elements in q
-  auto chunks = [](const SbCache &c) {
-    return reinterpret_cast<uintptr_t>(c.ptr) % 16 == 0 && c.stride_page % 8 == 0 && c.stride_h % 8 == 0 && c.stride_t % 8 == 0;
+  // whole 16-byte chunks in every row of the cache and no axis that repeats its elements, pairs of elements in q
+  auto chunks = [p](const SbCache &c) {
+    auto axis = [](int extent, int64_t stride) { return extent <= 1 || (stride > 0 && stride % 8 == 0); };
+    return reinterpret_cast<uintptr_t>(c.ptr) % 16 == 0 && axis(p->num_pages, c.stride_page) && axis(p->kv_heads, c.stride_h) &&
+           axis(p->page_size, c.stride_t);
   };
   const bool q_pairs = reinterpret_cast<uintptr_t>(p->q.ptr) % 4 == 0 && p->q.stride_b % 2 == 0 && p->q.stride_h % 2 == 0 && p->q.stride_t % 2 == 0;
   const bool tc = q_pairs && p->dtype != SB_DTYPE_F32 && !(p->flags & SB_FLAG_FORCE_SIMT) && p->head_dim % 8 == 0 && chunks(p->k) && chunks(p->v);
@@ -71,12 +73,13 @@ int plan_decode(const SbDecodeParams *p, DecodePlan &pl) {
   pl.chunks = sms * (tc ? decode_tc_warps(pl.rows_per_block, p->head_dim) : decode_simt_warps(p->head_dim));
   const long long items = (long long)p->batch * p->kv_heads * pl.row_blocks;
   pl.by_item = items < pl.chunks;
+  pl.part_cols = tc ? decode_tc_cols(p->head_dim) : p->head_dim;
   if (items > (1LL << 30)) return fail(SB_ERR_ARGUMENT, "batch * kv_heads too large");
-  pl.unit_shift = 6;                         // the units of all items have to be counted in 31 bits
+  pl.unit_shift = 4;                         // the units of all items have to be counted in 31 bits
   while (items * (((long long)p->max_pages * p->page_size >> pl.unit_shift) + 1) > 0x7fffffffLL) ++pl.unit_shift;
   const size_t slots = 2 * (size_t)pl.chunks * pl.rows_per_block, notes = (size_t)(pl.by_item ? items : pl.chunks) * sizeof(int4);
   pl.part_o = (notes + 255) / 256 * 256;
-  pl.part_l = pl.part_o + slots * p->head_dim * sizeof(float);
+  pl.part_l = pl.part_o + (slots * pl.part_cols + 128) * sizeof(float);      // (padded: see launch_decode_join)
   pl.bytes = (pl.part_l + slots * sizeof(float) + 255) / 256 * 256;
   return SB_OK;
 }
@@ -129,10 +132,16 @@ int run_decode(const SbDecodeParams *p, void *stream) {
   k.scale = p->logit_scale;
   k.chunks = pl.chunks;
   k.by_item = pl.by_item;
+  k.part_cols = pl.part_cols;
   k.unit_shift = pl.unit_shift;
   k.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (p->page_size == 1 << i) k.page_shift = i;
+  // keys have 31 bits, so with 2^l >= page_size > 2^(l - 1) the quotient is exactly key * ceil(2^(31 + l) / page_size) >> 31 + l
+  int l = 0;
+  while ((1LL << l) < p->page_size) ++l;
+  k.page_magic = (unsigned)(((1ULL << (31 + l)) + p->page_size - 1) / p->page_size);
+  k.page_post = l - 1;
   k.items_per_seq = p->kv_heads * pl.row_blocks;
   char *ws = reinterpret_cast<char *>(p->workspace);
   k.notes = reinterpret_cast<int4 *>(ws);
@@ -141,7 +150,7 @@ int run_decode(const SbDecodeParams *p, void *stream) {
   k.status = p->status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = pl.path == SB_PATH_SIMT ? launch_decode_simt(k, p->dtype, s) : launch_decode_tc(k, p->dtype, s);
-  if (e == cudaSuccess) e = launch_decode_join(k, p->dtype, s);
+  if (e == cudaSuccess) e = pl.path == SB_PATH_SIMT ? launch_decode_join(k, p->dtype, s) : launch_decode_tc_join(k, p->dtype, s);
   *launches = 2;
   return e == cudaSuccess ? SB_OK : fail(SB_ERR_CUDA, "decode launch: %s", cudaGetErrorString(e));
 }

@@ -44,23 +44,8 @@ struct MapSlot {
 };
 constexpr int kMapSlots = 128;
 
-static cudaError_t encode_cached(CUtensorMap *map, const void *ptr, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3],
-                                 int box_rows, int dtype) {
-  static thread_local MapSlot table[kMapSlots];
-  MapKey key;
-  memset(&key, 0, sizeof(key));
-  key.ptr = ptr;
-  for (int i = 0; i < 4; ++i) key.dims[i] = dims[i];
-  for (int i = 0; i < 3; ++i) key.strides[i] = strides[i];
-  key.box_rows = (cuuint32_t)box_rows;
-  key.dtype = dtype;
-  uint64_t h = (uint64_t)(uintptr_t)ptr * 0x9E3779B97F4A7C15ull;
-  h ^= (dims[1] + 0x1000193u * box_rows + 31u * strides[0] + 17u * strides[1]) * 0xC2B2AE3D27D4EB4Full;
-  MapSlot &slot = table[(h >> 32) % kMapSlots];
-  if (slot.used && slot.key == key) {
-    *map = slot.map;
-    return cudaSuccess;
-  }
+cudaError_t encode_tile_map(CUtensorMap *map, const void *ptr, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3], int box_rows,
+                            int dtype) {
   EncodeTiledFn enc = encode_fn();
   if (enc == nullptr) return cudaErrorNotSupported;
   cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
@@ -78,6 +63,28 @@ static cudaError_t encode_cached(CUtensorMap *map, const void *ptr, const cuuint
     if (e != cudaSuccess) return e;
     if (!encode()) return cudaErrorInvalidValue;
   }
+  return cudaSuccess;
+}
+
+static cudaError_t encode_cached(CUtensorMap *map, const void *ptr, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3],
+                                 int box_rows, int dtype) {
+  static thread_local MapSlot table[kMapSlots];
+  MapKey key;
+  memset(&key, 0, sizeof(key));
+  key.ptr = ptr;
+  for (int i = 0; i < 4; ++i) key.dims[i] = dims[i];
+  for (int i = 0; i < 3; ++i) key.strides[i] = strides[i];
+  key.box_rows = (cuuint32_t)box_rows;
+  key.dtype = dtype;
+  uint64_t h = (uint64_t)(uintptr_t)ptr * 0x9E3779B97F4A7C15ull;
+  h ^= (dims[1] + 0x1000193u * box_rows + 31u * strides[0] + 17u * strides[1]) * 0xC2B2AE3D27D4EB4Full;
+  MapSlot &slot = table[(h >> 32) % kMapSlots];
+  if (slot.used && slot.key == key) {
+    *map = slot.map;
+    return cudaSuccess;
+  }
+  const cudaError_t e = encode_tile_map(map, ptr, dims, strides, box_rows, dtype);
+  if (e != cudaSuccess) return e;
   slot.key = key;
   slot.map = *map;
   slot.used = true;
