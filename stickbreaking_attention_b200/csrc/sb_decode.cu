@@ -44,8 +44,6 @@ template <int kCols> __device__ __forceinline__ int col_of(int lane, int i) {
 template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtShape<kCols> {
   using S = SimtShape<kCols>;
   using S::kWidth;
-  using Ring = AsyncRing<S::kStages>;
-  static constexpr bool kBoxes = false;
   static constexpr int kPairs = (kRows + 1) / 2;
   float q[kRows][kCols], acc[kRows][kCols];
   LongSum left[kPairs];
@@ -197,7 +195,7 @@ __global__ void __launch_bounds__(E::kWarps * 32, 1) decode_simt_kernel(const __
   extern __shared__ __align__(128) char ring[];
   __shared__ ChunkShared<E::kWarps> shared;
   enter_kernel<true>();
-  decode_chunks<E>(p, ring, shared, typename E::Ring());
+  decode_chunks<E>(p, ring, shared);
 }
 
 // Joins the pieces of the items that were cut, up to 128 columns of one row at a time, newest piece first.  Each warp has such a

@@ -48,7 +48,6 @@ struct DecodeParams {
   int by_item;            // notes are numbered by item, where there are fewer items than chunks; else by chunk
   float *part_o, *part_l; // per slot (2 * chunks of them): rows_per_block x part_cols sums, rows_per_block x L
   int part_cols;
-  int box_rows;           // tensor-core kernel with tensor maps: rows of a box (8, 16)
   int4 *notes;            // [min(items, chunks)]: an item that was cut: sequence, item of it, first chunk, pieces (0: none)
   int *status;
 };
@@ -181,16 +180,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool t
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int n> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
 
-// How a warp waits for the copies of its stages: cp.async ones in groups, of which the newest kStages - 1 may still be on their way.
-template <int kStages> struct AsyncRing {
-  __device__ __forceinline__ void filled() { cp_async_commit(); }
-  __device__ __forceinline__ bool wait(int) {
-    cp_async_wait<kStages - 1>();
-    return true;
-  }
-  __device__ __forceinline__ void end(bool) { cp_async_wait<0>(); }
-};
-
 // A warp's loads, newest tile of a piece first, on into the next pieces.  32 entries of the page table are kept in a register of
 // the warp and read anew, ahead of their use, where a tile needs others.
 template <typename E> struct Feed {
@@ -230,23 +219,11 @@ template <typename E> struct Feed {
     const int page = __shfl_sync(0xffffffffu, window, top - page_index(p, min(key, w.k1 - 1)));
     return (unsigned)page < (unsigned)p.num_pages ? page : -1;
   }
-  // `ring`: how the engine's copies are waited for.
-  __device__ __forceinline__ void copy(int stage, char *to, typename E::Ring &ring) {
+  __device__ __forceinline__ void copy(int stage, char *to) {
     if (left == 0) return;
     const int key0 = w.k0 + --left * kTileKeys;
     bool wrong;
-    if constexpr (E::kBoxes) {
-      const int low = page_index(p, key0), page = page_of(key0), slot = key0 - low * p.page_size;
-      wrong = page < 0;
-      if (p.box_rows == kTileKeys) {                              // the tile is in one page
-        E::copy_boxes(p, w, page, slot, page, slot, !wrong, false, to, ring, stage);
-      } else {                                                    // two times eight rows
-        const bool two = key0 + 8 < w.k1;
-        const int next = page_index(p, key0 + 8), second = page_of(key0 + 8);
-        wrong = wrong || (two && second < 0);
-        E::copy_boxes(p, w, page, slot, second, key0 + 8 - next * p.page_size, !wrong, two, to, ring, stage);
-      }
-    } else if (p.page_shift >= 4 && key0 + kTileKeys <= w.k1) {   // a whole tile in one page
+    if (p.page_shift >= 4 && key0 + kTileKeys <= w.k1) {          // a whole tile in one page
       const int page = page_of(key0);
       wrong = page < 0;
       if (!wrong) E::copy_run(p, w, page, key0 & ((1 << p.page_shift) - 1), to);
@@ -278,8 +255,7 @@ template <typename E> struct Feed {
 // The main kernel.  E, the engine: the shape of a stage (kWarps, kStages, kStage bytes), copy (16 keys and values of one
 // key head), start, tile (adds a stage up, keys newest first), gone (the rows' sticks are used up), finish (writes the sums out).
 // One loop and one place for each of these: a short call runs through the code once, and its length counts there.
-template <typename E>
-__device__ __forceinline__ void decode_chunks(const DecodeParams &p, char *memory, ChunkShared<E::kWarps> &shared, typename E::Ring ring) {
+template <typename E> __device__ __forceinline__ void decode_chunks(const DecodeParams &p, char *memory, ChunkShared<E::kWarps> &shared) {
   int chunk, size;
   Cursor c = find_chunk<E::kWarps>(p, chunk, size, shared);
   const int lane = threadIdx.x & 31;
@@ -291,12 +267,12 @@ __device__ __forceinline__ void decode_chunks(const DecodeParams &p, char *memor
   Piece w;
   E sum;
   int at = 0, into = 0, fill = E::kStages, number = 0, left = 0;
-  bool fresh = true, bad = false, done = false, first = true, failed = false;
+  bool fresh = true, bad = false, done = false, first = true;
   for (;;) {
     if (fill > 0) {              // a stage is free
       __syncwarp();
-      feed.copy(into, stages + into * E::kStage, ring);
-      ring.filled();
+      feed.copy(into, stages + into * E::kStage);
+      cp_async_commit();
       into = into == E::kStages - 1 ? 0 : into + 1;
       if (--fill > 0) continue;
     }
@@ -308,19 +284,9 @@ __device__ __forceinline__ void decode_chunks(const DecodeParams &p, char *memor
       fresh = done = false;
     }
     if (left > 0) {
-      if (!failed && !ring.wait(at)) {       // a copy that does not come: nothing of this warp counts any more
-        failed = true;
-        if (p.status != nullptr) {
-          p.status[0] = SB_DEV_WAIT_TIMEOUT;
-          p.status[1] = at;
-        }
-      }
+      cp_async_wait<E::kStages - 1>();
       __syncwarp();
-      if (failed) {
-        bad = true;
-        feed.left = 0;
-        feed.c.rest = 0;
-      } else if (!done) {
+      if (!done) {
         bad |= feed.bad >> at & 1;
         sum.tile(p, w, stages + at * E::kStage, w.k0 + (left - 1) * kTileKeys);
         if (!p.dense && sum.gone()) {
@@ -353,7 +319,7 @@ __device__ __forceinline__ void decode_chunks(const DecodeParams &p, char *memor
     first = false;
     fresh = true;
   }
-  ring.end(failed);
+  cp_async_wait<0>();
 }
 
 // Where row r of a piece's result goes: to o and rem where the piece is the whole item, else to its slot of the workspace.

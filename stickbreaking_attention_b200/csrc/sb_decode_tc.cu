@@ -2,30 +2,28 @@
 //
 // What bounds it: every key and value is read once from HBM and takes part in 4 * rows operations per element, `rows` (query
 // heads per key head times new tokens) being 1 to 16 here: 1 to 16 operations per byte, where the GPU's ratio is 250.  So the
-// kernel is built around the copies: each warp has a ring of 16-key stages of its own, and no barrier with other warps; 192 KiB of
-// stages per SM keep more bytes in flight than the latency of HBM needs (some 50 KiB).  Where pages hold a multiple of 8 tokens the
-// stages are filled by TMA, 64 columns x 16 (or two times 8) rows of one page and key head at a time, issued by one lane; other
-// pages take cp.async, a lane per 16 bytes.
+// kernel is built around the copies: each warp has a ring of 16-key stages of its own, filled with cp.async, and no barrier with
+// other warps; 192 KiB of stages per SM keep more bytes in flight than the latency of HBM needs (some 50 KiB).  (TMA, boxes of 64
+// columns x 16 rows issued by one lane, took the same time to within 2 %, its longer latency weighing as much as the instructions that it saves.)
 //
 // The products are mma.sync ones with the keys as the rows of the tile: S^T = K Q^T, O^T = V^T P^T, 16 keys by 8 queries.  A
 // tcgen05 tile takes 64 or 128 rows of one operand from shared memory that whole warps have to hand over; with 8 queries it
 // would be no less empty, and the products are not what takes the time.
 //
 // A thread holds rows g and g + 8 of the score tile.  They are keys 2 g and 2 g + 1 of the 16 (for g >= 4 the other way round), so
-// that the sums over later keys take four shuffles per query; and the eight rows that one ldmatrix reads are eight different ones
-// modulo 8, which is what the 128-byte swizzle of TMA needs to put them into different banks.  Base 2 throughout:
-//   x = s log2(e) <q, k>,  u = 2^-|x|,  l = log2(1 + u);  log2 beta = min(x, 0) - l,  log2(1 - beta) = -max(x, 0) - l.
-// l comes from the series 2 atanh(u / (2 + u)) = 2 (w + w^3 / 3 + w^5 / 5 + ...), to 2^-22 of itself also where u is small: what
-// thousands of keys break off adds up.
+// that the products over later keys take four shuffles per query; and the eight rows that one ldmatrix reads are eight different
+// ones modulo 8, which is what the swizzle needs to put them into different banks.  No logarithms:
+//   x = s log2(e) <q, k>,  e = 2^-|x|,  1 - beta = 1 / (1 + 2^x) = (e or 1) / (1 + e),  beta = (1 or e) / (1 + e)  (x >= 0 or not),
+//   weight = stick * (product of 1 - beta over the tile's later keys) * beta,
+// and the stick behind the tile is what was there less the tile's weights, where more than 7/8 of it are left, else the product.  The
+// difference loses nothing over thousands of keys that take 1e-5 each, whose 1 - beta are rounded in their last bits; the
+// product loses nothing where little is left.  The tile's weights are added up by one more product, with ones for values.
 //
 // P enters the second product as the sum of two 16-bit numbers (16 or 22 bits): rounded once it would double the error that the
 // output's own rounding makes, and the second product of the pair is free.  In fp16 it is scaled by 2^15, since a weight of 1e-5
-// has few bits left there.  Scores, sums and the output's accumulators are 32-bit, the stick between tiles 32-bit with what its sums lost.
-#include <cstring>
-#include <type_traits>
-
+// has few bits left there.  Scores, weights and the output's accumulators are 32-bit, the stick 32-bit with what its sums lost.
 #include "sb_decode.cuh"
-#include "sb_tc_common.cuh"
+#include "sb_ptx.cuh"
 
 namespace sb {
 
@@ -82,17 +80,8 @@ template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t x) 
 template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
 template <typename T> constexpr float kScaleP = 1.0f;
 template <> constexpr float kScaleP<__half> = 32768.0f;
-
-// log2(1 + u), 0 <= u <= 1; NaN for NaN.
-__device__ __forceinline__ float log2_1p(float u) {
-  const float w = u * rcp(2.0f + u), t = w * w;
-  float s = fmaf(t, 1.0f / 11, 1.0f / 9);
-  s = fmaf(t, s, 1.0f / 7);
-  s = fmaf(t, s, 1.0f / 5);
-  s = fmaf(t, s, 1.0f / 3);
-  s = fmaf(t, s, 1.0f);
-  return 2.0f * kLog2e * w * s;
-}
+template <typename T> constexpr uint32_t kOnes = 0x3f803f80;      // two times 1.0
+template <> constexpr uint32_t kOnes<__half> = 0x3c003c00;
 
 // Where chunk c of row r of a stage's keys or values lies: blocks of 64 columns, rows of 128 bytes, swizzled.
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
@@ -101,68 +90,18 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 // The key of the tile that row g (second false) or g + 8 of a product's operand is.
 __device__ __forceinline__ int key_of(int g, bool second) { return 2 * g + (second != (g >= 4)); }
 
-struct Maps {
-  CUtensorMap k, v;
-};
-
 // The tensor-core engine.  kN: blocks of 8 query rows.
-// kTma: the stages are filled by TMA, an mbarrier per stage; else by cp.async.
-template <typename T, int kD, int kN, bool kTma> struct TcEngine : TcShape<kD, kN> {
+template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
   using S = TcShape<kD, kN>;
   using S::kHalf;
-  static constexpr bool kBoxes = kTma;
-  struct TmaRing {
-    const Maps *maps;
-    uint32_t bars;             // the warp's, one per stage
-    uint32_t phases = 0;       // a bit per stage: the parity to wait for next
-    uint32_t open = 0;         // a bit per stage: copies that nobody has waited for
-    __device__ __forceinline__ void filled() {}
-    __device__ __forceinline__ bool wait(int stage) {
-      const bool ok = ptx::mbar_wait(bars + 8 * stage, phases >> stage & 1);
-      phases ^= 1u << stage;
-      open &= ~(1u << stage);
-      return __all_sync(0xffffffffu, ok);
-    }
-    // the block's memory is not given back while copies into it are on their way
-    __device__ __forceinline__ void end(bool failed) {
-      for (int i = 0; i < S::kStages; ++i)
-        if (open >> i & 1) ptx::mbar_wait(bars + 8 * i, phases >> i & 1);
-      (void)failed;
-    }
-  };
-  using Ring = std::conditional_t<kTma, TmaRing, AsyncRing<S::kStages>>;
   uint32_t q[kN][kD / 16][2];
   float acc[kD / 16][kN][4];
-  LongSum left[kN][2];
+  LongSum stick[kN][2];
   int limit[kN][2];
   bool real[kN][2];
 
   __device__ static __forceinline__ void prefetch_rows(const DecodeParams &p, const Piece &w) { prefetch_q(p, w, 2); }
 
-  // Eight or sixteen rows from slot `slot` of page `page` on, and (two) eight more from another place.  Rows behind the page's end and
-  // columns behind head_dim are zeros.  !real: nothing, the stage counts as filled.
-  __device__ static __forceinline__ void copy_boxes(const DecodeParams &p, const Piece &w, int page, int slot, int page2, int slot2, bool real,
-                                                    bool two, char *to, TmaRing &ring, int stage_index) {
-    ring.open |= 1u << stage_index;
-    if ((threadIdx.x & 31) != 0) return;
-    const uint32_t bar = ring.bars + 8 * stage_index, stage = smem_u32(to);
-    if (!real) {
-      ptx::mbar_arrive(bar);
-      return;
-    }
-    const int rows = two ? kTileKeys : p.box_rows;
-    ptx::mbar_arrive_expect_tx(bar, 2 * kD * 2 * rows);
-#pragma unroll
-    for (int c = 0; c < kD / 64; ++c) {
-      const uint32_t at = stage + c * (kTileKeys * 128);
-      ptx::tma_load_4d(at, &ring.maps->k, bar, c * 64, slot, w.head, page);
-      ptx::tma_load_4d(at + kHalf, &ring.maps->v, bar, c * 64, slot, w.head, page);
-      if (two) {
-        ptx::tma_load_4d(at + 8 * 128, &ring.maps->k, bar, c * 64, slot2, w.head, page2);
-        ptx::tma_load_4d(at + 8 * 128 + kHalf, &ring.maps->v, bar, c * 64, slot2, w.head, page2);
-      }
-    }
-  }
   // 16 rows from slot `slot` of one page on; columns behind head_dim are zeros.
   __device__ static __forceinline__ void copy_run(const DecodeParams &p, const Piece &w, int page, int slot, char *to) {
     const int lane = threadIdx.x & 31;
@@ -216,7 +155,7 @@ template <typename T, int kD, int kN, bool kTma> struct TcEngine : TcShape<kD, k
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int query = n * 8 + t * 2 + j;
-        left[n][j] = LongSum();
+        stick[n][j] = LongSum{1.0f, 0.0f};
         real[n][j] = query < w.rows;
         limit[n][j] = row_limit(p, w.keys, w.row0 + min(query, w.rows - 1));
       }
@@ -269,33 +208,39 @@ template <typename T, int kD, int kN, bool kTma> struct TcEngine : TcShape<kD, k
       }
     }
     const float scale = p.scale * kLog2e;
-    float a[kN][4];
+    const bool edge = key0 + kTileKeys > w.edge;     // some rows do not attend to some keys
+    float a[kN][4], rest[kN][2];                     // weights; product of 1 - beta over the tile
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {                  // queries 2 t + j; rows g (s[n][j]) and g + 8 (s[n][2 + j])
-        float beta[2], broken[2];
+        float beta[2], kept[2];
 #pragma unroll
         for (int row = 0; row < 2; ++row) {
-          const float x = (s[n][2 * row + j] + odd[n][2 * row + j]) * scale, l = log2_1p(ex2(-fabsf(x)));
-          const bool in = key0 + key_of(g, row) < limit[n][j];
-          beta[row] = in ? fminf(x, 0.0f) - l : -INFINITY;
-          broken[row] = in ? -(fmaxf(x, 0.0f) + l) : 0.0f;
-          if (in && x != x) beta[row] = broken[row] = x;      // (fminf and fmaxf drop a NaN)
+          const float x = (s[n][2 * row + j] + odd[n][2 * row + j]) * scale, e = ex2(-fabsf(x)), d = rcp(1.0f + e), ed = e * d;
+          beta[row] = x >= 0.0f ? d : ed;            // (NaN: both are)
+          kept[row] = x >= 0.0f ? ed : d;
         }
-        const float both = broken[0] + broken[1];
+        if (edge) {
+#pragma unroll
+          for (int row = 0; row < 2; ++row)
+            if (key0 + key_of(g, row) >= limit[n][j]) {
+              beta[row] = 0.0f;
+              kept[row] = 1.0f;
+            }
+        }
+        const float both = kept[0] * kept[1];
         float later = __shfl_down_sync(0xffffffffu, both, 4);
-        if (g == 7) later = 0.0f;
+        if (g == 7) later = 1.0f;
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
           const float other = __shfl_down_sync(0xffffffffu, later, d);
-          if (lane + d < 32) later += other;
+          if (lane + d < 32) later *= other;
         }
-        const float base = left[n][j].sum + later;
-        // the older key of the two comes behind the newer one
-        a[n][j] = exp2_all(beta[0] + (base + (g < 4 ? broken[1] : 0.0f))) * kScaleP<T>;
-        a[n][2 + j] = exp2_all(beta[1] + (base + (g < 4 ? 0.0f : broken[0]))) * kScaleP<T>;
-        left[n][j].add(__shfl_sync(0xffffffffu, later + both, lane & 3));
+        rest[n][j] = __shfl_sync(0xffffffffu, later * both, lane & 3);
+        const float whole = stick[n][j].sum * kScaleP<T> * later;
+        a[n][j] = beta[0] * (g < 4 ? whole * kept[1] : whole);          // the older key of the two comes behind the newer one
+        a[n][2 + j] = beta[1] * (g < 4 ? whole : whole * kept[0]);
       }
     }
     // the two 16-bit parts of the weights, moved from (key, query) to (query, key)
@@ -309,8 +254,20 @@ template <typename T, int kD, int kN, bool kTma> struct TcEngine : TcShape<kD, k
         b[n][row][0] = transpose8x8(hi);
         b[n][row][1] = transpose8x8(pack<T>(a[n][2 * row] - back.x, a[n][2 * row + 1] - back.y));
       }
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const uint32_t ones[4] = {kOnes<T>, kOnes<T>, kOnes<T>, kOnes<T>};
+      float sum[4] = {};                             // [j]: all weights of query 2 t + j
+      mma<T>(sum, ones, b[n][0][0], b[n][1][0]);
+      mma<T>(sum, ones, b[n][0][1], b[n][1][1]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (rest[n][j] > 0.875f) stick[n][j].add(sum[j] * (-1.0f / kScaleP<T>));
+        else stick[n][j] = LongSum{stick[n][j].sum * rest[n][j], 0.0f};
+      }
+    }
     const uint32_t values = stage + kHalf;
-    if (key0 + kTileKeys <= w.edge) {
+    if (!edge) {
       add_values<false>(values, b, 0, 0);
       return;
     }
@@ -328,7 +285,6 @@ template <typename T, int kD, int kN, bool kTma> struct TcEngine : TcShape<kD, k
       __syncwarp();
       add_values<true>(values, b, reach, reach + 1);
     }
-    if constexpr (kTma) ptx::fence_proxy_async_smem();      // the stage's next copies come behind these stores
   }
 
   __device__ __forceinline__ bool gone() const {
@@ -336,7 +292,7 @@ template <typename T, int kD, int kN, bool kTma> struct TcEngine : TcShape<kD, k
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) all = all && (!real[n][j] || left[n][j].sum < kStickGone);
+      for (int j = 0; j < 2; ++j) all = all && (!real[n][j] || stick[n][j].sum == 0.0f);
     return __all_sync(0xffffffffu, all);
   }
 
@@ -351,7 +307,7 @@ template <typename T, int kD, int kN, bool kTma> struct TcEngine : TcShape<kD, k
         for (int i = 0; i < kD / 16; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[i][n][j] = nan;
-        left[n][0].sum = left[n][1].sum = nan;
+        stick[n][0].sum = stick[n][1].sum = nan;
       }
     }
 #pragma unroll
@@ -370,42 +326,24 @@ template <typename T, int kD, int kN, bool kTma> struct TcEngine : TcShape<kD, k
               const int c = i * 16 + half * 8 + g;
               if (c < p.head_dim) out[c] = from_f32<T>(acc[i][n][half * 2 + j] * (1.0f / kScaleP<T>));
             }
-          if (g == 0) put_rem<T>(p, w, slot, r + j, left[n][j].sum);
+          if (g == 0) reinterpret_cast<T *>(p.rem)[rem_index(p, w.seq, w.head, w.row0 + r + j)] = from_f32<T>(stick[n][j].sum);
         }
       } else {
         float4 *const part = reinterpret_cast<float4 *>(p.part_o + (long long)slot * (kN * 8 * kD)) + n * (kD / 16) * 32 + lane;
 #pragma unroll
         for (int i = 0; i < kD / 16; ++i) part[i * 32] = make_float4(acc[i][n][0], acc[i][n][1], acc[i][n][2], acc[i][n][3]);
-        if (g == 0) *reinterpret_cast<float2 *>(p.part_l + (long long)slot * (kN * 8) + r) = make_float2(left[n][0].sum, left[n][1].sum);
+        if (g == 0) *reinterpret_cast<float2 *>(p.part_l + (long long)slot * (kN * 8) + r) = make_float2(stick[n][0].sum, stick[n][1].sum);
       }
     }
   }
 };
 
-template <typename T, int kD, int kN, bool kTma>
-__global__ void __launch_bounds__(TcShape<kD, kN>::kWarps * 32, 1)
-    decode_tc_kernel(const __grid_constant__ DecodeParams p, const __grid_constant__ Maps maps) {
-  using S = TcShape<kD, kN>;
-  using E = TcEngine<T, kD, kN, kTma>;
-  extern __shared__ __align__(1024) char ring[];
-  __shared__ ChunkShared<S::kWarps> shared;
-  if constexpr (kTma) {
-    __shared__ uint64_t bars[S::kWarps][S::kStages];
-    const uint32_t mine = smem_u32(bars[threadIdx.x >> 5]);
-    if ((threadIdx.x & 31) == 0) {
-      ptx::prefetch_tensormap(&maps.k);
-      ptx::prefetch_tensormap(&maps.v);
-      for (int i = 0; i < S::kStages; ++i) ptx::mbar_init(mine + 8 * i, 1);
-      ptx::fence_barrier_init();
-      ptx::fence_proxy_async_smem();
-    }
-    __syncwarp();
-    enter_kernel<true>();
-    decode_chunks<E>(p, ring, shared, typename E::Ring{&maps, mine});
-  } else {
-    enter_kernel<true>();
-    decode_chunks<E>(p, ring, shared, typename E::Ring());
-  }
+template <typename T, int kD, int kN>
+__global__ void __launch_bounds__(TcShape<kD, kN>::kWarps * 32, 1) decode_tc_kernel(const __grid_constant__ DecodeParams p) {
+  extern __shared__ __align__(128) char ring[];
+  __shared__ ChunkShared<TcShape<kD, kN>::kWarps> shared;
+  enter_kernel<true>();
+  decode_chunks<TcEngine<T, kD, kN>>(p, ring, shared);
 }
 
 // Joins the pieces of the items that were cut, newest first, 8 rows x 16 columns at a time as a warp's registers held them: a lane has two
@@ -438,13 +376,12 @@ __device__ __forceinline__ void load_eight(const float2 *const (&at)[8], float2 
 }
 // Adds a run of keys (x, l) behind what is summed up in (o, left).  (0 times what is no number stays out.)
 __device__ __forceinline__ void add_behind(float4 &o, float2 &left, const float4 &x, const float2 &l) {
-  const float a = exp2_all(left.x), b = exp2_all(left.y);
-  o.x += a != 0.0f ? a * x.x : 0.0f;
-  o.y += b != 0.0f ? b * x.y : 0.0f;
-  o.z += a != 0.0f ? a * x.z : 0.0f;
-  o.w += b != 0.0f ? b * x.w : 0.0f;
-  left.x += l.x;
-  left.y += l.y;
+  o.x += left.x != 0.0f ? left.x * x.x : 0.0f;
+  o.y += left.y != 0.0f ? left.y * x.y : 0.0f;
+  o.z += left.x != 0.0f ? left.x * x.z : 0.0f;
+  o.w += left.y != 0.0f ? left.y * x.w : 0.0f;
+  left.x = left.x != 0.0f ? left.x * l.x : 0.0f;
+  left.y = left.y != 0.0f ? left.y * l.y : 0.0f;
 }
 
 template <typename T, int kWarps, int kTogether>
@@ -465,7 +402,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_tc_join_kernel(const __gri
   const int slot_size = p.rows_per_block * p.part_cols;
   const float4 *const parts = reinterpret_cast<const float4 *>(p.part_o) + job * 32 + lane;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float2 left = make_float2(0.0f, 0.0f);
+  float2 left = make_float2(1.0f, 1.0f);       // of the stick
   if (real) {
     for (int k0 = begin; k0 < end; k0 += kJoinDeep) {
       const float4 *at[kJoinDeep];
@@ -493,7 +430,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_tc_join_kernel(const __gri
     __syncthreads();
     if (member != 0) return;
     o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    left = make_float2(0.0f, 0.0f);
+    left = make_float2(1.0f, 1.0f);
 #pragma unroll 8
     for (int m = 0; m < kTogether; ++m) add_behind(o, left, sums[warp + m][lane], lefts[warp + m][lane]);
   }
@@ -504,35 +441,22 @@ __global__ void __launch_bounds__(kWarps * 32) decode_tc_join_kernel(const __gri
     T *const out = reinterpret_cast<T *>(p.o.ptr) + row_offset(p, p.o, note.x, head, row0 + r + j);
     if (c < p.head_dim) out[c] = from_f32<T>((j ? o.y : o.x) * (1.0f / kScaleP<T>));
     if (c + 8 < p.head_dim) out[c + 8] = from_f32<T>((j ? o.w : o.z) * (1.0f / kScaleP<T>));
-    if (c == 0) reinterpret_cast<T *>(p.rem)[rem_index(p, note.x, head, row0 + r + j)] = from_f32<T>(exp2f(j ? left.y : left.x));
+    if (c == 0) reinterpret_cast<T *>(p.rem)[rem_index(p, note.x, head, row0 + r + j)] = from_f32<T>(j ? left.y : left.x);
   }
 }
 
-template <typename T, int kD, int kN, bool kTma> cudaError_t launch_one(const DecodeParams &p, const Maps &maps, cudaStream_t s) {
+template <typename T, int kD, int kN> cudaError_t launch_one(const DecodeParams &p, cudaStream_t s) {
   using S = TcShape<kD, kN>;
-  const auto kernel = decode_tc_kernel<T, kD, kN, kTma>;
+  const auto kernel = decode_tc_kernel<T, kD, kN>;
   const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3(p.chunks / S::kWarps), S::kWarps * 32, S::kBytes, s, p, maps);
+  return launch_kernel(kernel, dim3(p.chunks / S::kWarps), S::kWarps * 32, S::kBytes, s, p);
 }
-template <typename T, bool kTma> cudaError_t launch_shape(const DecodeParams &p, const Maps &maps, cudaStream_t s) {
+template <typename T> cudaError_t launch_shape(const DecodeParams &p, cudaStream_t s) {
   const int n = p.rows_per_block / 8;
-  if (p.head_dim <= 64)
-    return n == 1 ? launch_one<T, 64, 1, kTma>(p, maps, s) : n == 2 ? launch_one<T, 64, 2, kTma>(p, maps, s) : launch_one<T, 64, 4, kTma>(p, maps, s);
-  if (p.head_dim <= 128) return n == 1 ? launch_one<T, 128, 1, kTma>(p, maps, s) : launch_one<T, 128, 2, kTma>(p, maps, s);
-  return launch_one<T, 256, 1, kTma>(p, maps, s);
-}
-template <typename T> cudaError_t launch_type(const DecodeParams &p, const Maps &maps, cudaStream_t s) {
-  return p.box_rows != 0 ? launch_shape<T, true>(p, maps, s) : launch_shape<T, false>(p, maps, s);
-}
-
-// (head_dim, slots, heads, pages); the stride of an axis of one element is the caller's to leave as it likes.
-cudaError_t cache_map(CUtensorMap *map, const PagedRef &t, const DecodeParams &p, int dtype) {
-  const long long st = p.page_size > 1 ? t.st : (p.head_dim + 7) / 8 * 8, sh = p.kv_heads > 1 ? t.sh : st * p.page_size,
-                  sp = p.num_pages > 1 ? t.sp : sh * p.kv_heads;
-  const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.page_size, (cuuint64_t)p.kv_heads, (cuuint64_t)p.num_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sp * 2};
-  return encode_tile_map(map, t.ptr, dims, strides, p.box_rows, dtype);
+  if (p.head_dim <= 64) return n == 1 ? launch_one<T, 64, 1>(p, s) : n == 2 ? launch_one<T, 64, 2>(p, s) : launch_one<T, 64, 4>(p, s);
+  if (p.head_dim <= 128) return n == 1 ? launch_one<T, 128, 1>(p, s) : launch_one<T, 128, 2>(p, s);
+  return launch_one<T, 256, 1>(p, s);
 }
 
 }  // namespace
@@ -549,14 +473,8 @@ int decode_tc_warps(int rows, int head_dim) {
   return rows == 8 ? TcShape<64, 1>::kWarps : rows == 16 ? TcShape<64, 2>::kWarps : TcShape<64, 4>::kWarps;
 }
 
-cudaError_t launch_decode_tc(const DecodeParams &params, int dtype, cudaStream_t s) {
-  DecodeParams p = params;
-  p.box_rows = p.page_size % 16 == 0 ? 16 : p.page_size % 8 == 0 ? 8 : 0;
-  Maps maps;
-  memset(&maps, 0, sizeof(maps));
-  cudaError_t e = cudaSuccess;
-  if (p.box_rows != 0 && ((e = cache_map(&maps.k, p.k, p, dtype)) != cudaSuccess || (e = cache_map(&maps.v, p.v, p, dtype)) != cudaSuccess)) return e;
-  return dtype == SB_DTYPE_BF16 ? launch_type<__nv_bfloat16>(p, maps, s) : launch_type<__half>(p, maps, s);
+cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s) {
+  return dtype == SB_DTYPE_BF16 ? launch_shape<__nv_bfloat16>(p, s) : launch_shape<__half>(p, s);
 }
 
 // By the pieces that an item is cut into on the average: 1, 4 or 32 warps share a part.  (64 sequences x 16 heads, 1.7 pieces: 19 us

@@ -44,28 +44,6 @@ struct MapSlot {
 };
 constexpr int kMapSlots = 128;
 
-cudaError_t encode_tile_map(CUtensorMap *map, const void *ptr, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3], int box_rows,
-                            int dtype) {
-  EncodeTiledFn enc = encode_fn();
-  if (enc == nullptr) return cudaErrorNotSupported;
-  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  auto encode = [&] {
-    return enc(map, dtype == SB_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-               const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-  };
-  if (!encode()) {
-    // The driver's call wants a context.  The runtime's bind one to a thread as they go, but this may be the thread's first.
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaSetDevice(dev);
-    if (e != cudaSuccess) return e;
-    if (!encode()) return cudaErrorInvalidValue;
-  }
-  return cudaSuccess;
-}
-
 static cudaError_t encode_cached(CUtensorMap *map, const void *ptr, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3],
                                  int box_rows, int dtype) {
   static thread_local MapSlot table[kMapSlots];
@@ -83,8 +61,23 @@ static cudaError_t encode_cached(CUtensorMap *map, const void *ptr, const cuuint
     *map = slot.map;
     return cudaSuccess;
   }
-  const cudaError_t e = encode_tile_map(map, ptr, dims, strides, box_rows, dtype);
-  if (e != cudaSuccess) return e;
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return cudaErrorNotSupported;
+  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  auto encode = [&] {
+    return enc(map, dtype == SB_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+               const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (!encode()) {
+    // The driver's call wants a context.  The runtime's bind one to a thread as they go, but this may be the thread's first.
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return e;
+    if (!encode()) return cudaErrorInvalidValue;
+  }
   slot.key = key;
   slot.map = *map;
   slot.used = true;

@@ -218,8 +218,6 @@ __device__ __forceinline__ void mma_tmem_mnmajor(uint32_t d_tmem, uint32_t a_tme
 }
 
 // host: 4-D TMA map (head_dim, tokens, heads, batch), [64 x 128 x 1 x 1] box, 128-byte swizzle, zero fill
-cudaError_t encode_tile_map(CUtensorMap *map, const void *ptr, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3], int box_rows,
-                            int dtype);   // 64 columns x box_rows, swizzled by 128 bytes
 cudaError_t make_tile_map(CUtensorMap *map, const TensorRef &t, const KParams &p, int dtype, int box_rows = kBM);
 // host: 4-D TMA map of the stored A / dz tiles, (keys 128, pairs * 128 query rows, {A, dz}, heads), [64 x 64 x 1 x 1] box
 cudaError_t make_az_map(CUtensorMap *map, const KParams &p, int dtype, int box_rows = 64);
