@@ -144,15 +144,15 @@ __device__ __forceinline__ Cursor find_chunk(const DecodeParams &p, int &chunk, 
   chunk = warp * gridDim.x + blockIdx.x;
   Cursor c;
   c.rest = c.seq = c.item = c.u0 = c.n = c.keys = 0;
-  if (chunk > (total - 1) / size) return c;
+  if ((long long)chunk * size >= total) return c;
   const int unit = chunk * size;
   c.rest = min(size, total - unit);
-  int owner = 0;                               // the thread whose units this one is among
+  int group = 0;                               // the warp, then the thread, whose units this one is among
 #pragma unroll
-  for (int i = 0; i < kThreads; i += 32) {
-    const uint32_t vote = __ballot_sync(0xffffffffu, shared.before[i + lane] <= unit && shared.before[i + lane + 1] > unit);
-    if (vote != 0) owner = i + __ffs(vote) - 1;
-  }
+  for (int w = 1; w < kWarps; ++w)
+    if (shared.before[32 * w] <= unit) group = 32 * w;
+  const uint32_t vote = __ballot_sync(0xffffffffu, shared.before[group + lane] <= unit && shared.before[group + lane + 1] > unit);
+  const int owner = group + __ffs(vote) - 1;
   int first = shared.before[owner];
   for (c.seq = owner * each;; ++c.seq) {
     c.read_seq(p);
