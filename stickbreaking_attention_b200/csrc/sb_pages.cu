@@ -16,7 +16,7 @@ namespace {
 // ---- append -------------------------------------------------------------------------------------------------------------
 // Memory-bound: every new row read and written once.  A block looks up where its tokens go (sequence, page, slot), then its
 // threads copy 16 bytes at a time, all heads of a token, keys and values, kDeep of them in flight per thread.
-constexpr int kAppendThreads = 256, kMaxTokens = 64;
+constexpr int kAppendThreads = 256, kMaxTokens = 64, kAppendBlocks = 32;
 
 __device__ __forceinline__ long long append_end(const AppendParams &p, int i) {
   return p.cu64 ? reinterpret_cast<const long long *>(p.cu)[i] : (long long)reinterpret_cast<const int *>(p.cu)[i];
@@ -89,8 +89,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     dst[threadIdx.x] = to;
   }
   __syncthreads();
-  const int per_row = p.head_dim * p.esize / (int)sizeof(V);
-  const int per_token = 2 * p.kv_heads * per_row, work = count * per_token;
+  const int per_row = p.per_row, per_token = p.per_token, work = count * per_token;
   constexpr int kDeep = 4;
   for (int e0 = threadIdx.x; e0 < work; e0 += kDeep * kAppendThreads) {
     V x[kDeep];
@@ -100,7 +99,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
       const int e = e0 + i * kAppendThreads;
       to[i] = nullptr;
       if (e < work) {
-        const int t = e / per_token, in = e - t * per_token, row = in / per_row, c = in - row * per_row;
+        const int t = p.by_token.of(e), in = e - t * per_token, row = p.by_row.of(in), c = in - row * per_row;
         const bool val = row >= p.kv_heads;
         const int h = val ? row - p.kv_heads : row;
         if (dst[t] >= 0) {
@@ -262,45 +261,40 @@ __global__ void __launch_bounds__(kFreeThreads) free_kernel(const __grid_constan
   if (threadIdx.x == 0) p.seq_lens[b] = 0;
 }
 
-// Copies `bytes` from one place to another, a block's share of it.
-template <typename V> __device__ __forceinline__ void copy_share(char *to, const char *from, long long count, long long start, long long step) {
-  constexpr int kDeep = 4;
-  const V *s = reinterpret_cast<const V *>(from);
-  V *d = reinterpret_cast<V *>(to);
-  for (long long e0 = start; e0 < count; e0 += kDeep * step) {
-    V x[kDeep];
-#pragma unroll
-    for (int i = 0; i < kDeep; ++i)
-      if (e0 + i * step < count) x[i] = s[e0 + i * step];
-#pragma unroll
-    for (int i = 0; i < kDeep; ++i)
-      if (e0 + i * step < count) d[e0 + i * step] = x[i];
-  }
-}
-
-// The first `rows` slots of page `from` to page `to`: all heads of one layer's keys or values, by the block.
+// The first `rows` slots of page `from` to page `to`, the heads of part `part`, one layer's keys or values, by the block.
+constexpr int kCopyThreads = 256;
 template <typename V>
-__device__ __forceinline__ void copy_page(const PagesParams &p, const CacheRef &c, int layer, int from, int to, int rows) {
-  const char *src = c.ptr + layer * c.sl + from * c.sp;
-  char *dst = c.ptr + layer * c.sl + to * c.sp;
-  const int per_row = p.row_bytes / (int)sizeof(V);
-  const bool dense = c.st == p.row_bytes;
-  if (dense && rows == p.page_size && c.sh == (long long)p.row_bytes * p.page_size) {
-    copy_share<V>(dst, src, (long long)p.heads * rows * per_row, threadIdx.x, blockDim.x);
-    return;
-  }
+__device__ __forceinline__ void copy_page(const PagesParams &p, const CacheRef &c, int layer, int from, int to, int rows, int part) {
+  const int h0 = part * p.part_heads, heads = min(p.part_heads, p.heads - h0);
+  const char *src = c.ptr + layer * c.sl + from * c.sp + h0 * c.sh;
+  char *dst = c.ptr + layer * c.sl + to * c.sp + h0 * c.sh;
+  const bool dense = c.st == p.row_bytes;                   // a head's rows lie one behind the other
+  const bool whole = dense && rows == p.page_size && c.sh == (long long)p.row_bytes * p.page_size;      // and so do its heads
+  const int per_head = rows * p.per_row, work = heads * per_head;
   constexpr int kDeep = 4;
-  const int per_head = rows * per_row, work = p.heads * per_head;
-  for (int e0 = threadIdx.x; e0 < work; e0 += kDeep * (int)blockDim.x) {
+  // a division for the head, where its copies are not one run with the next one's: by the block's own number of rows
+  const float per = 1.0f / (float)per_head;
+  for (int e0 = threadIdx.x; e0 < work; e0 += kDeep * kCopyThreads) {
     V x[kDeep];
     long long at[kDeep];
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
-      const int e = e0 + i * (int)blockDim.x;
+      const int e = e0 + i * kCopyThreads;
       at[i] = -1;
       if (e < work) {
-        const int h = e / per_head, in = e - h * per_head, r = in / per_row, col = in - r * per_row;
-        at[i] = h * c.sh + r * c.st + col * (int)sizeof(V);
+        if (whole) {
+          at[i] = (long long)e * (int)sizeof(V);
+        } else {
+          int h = min((int)((float)e * per), heads - 1), in = e - h * per_head;      // off by one at most
+          if (in < 0) { --h; in += per_head; }
+          if (in >= per_head) { ++h; in -= per_head; }
+          if (dense) {
+            at[i] = h * c.sh + in * (int)sizeof(V);
+          } else {
+            const int r = p.by_row.of(in);
+            at[i] = h * c.sh + r * c.st + (in - r * p.per_row) * (int)sizeof(V);
+          }
+        }
         x[i] = *reinterpret_cast<const V *>(src + at[i]);
       }
     }
@@ -368,8 +362,7 @@ __global__ void __launch_bounds__(kBookThreads) fork_plan_kernel(const __grid_co
   if (threadIdx.x == 0) p.work[0] = 1;
 }
 
-// Blocks (pair, part): the parts of a pair are its layers' keys and values, and first its row of the table.
-constexpr int kCopyThreads = 256;
+// Blocks (part, pair): the parts of a pair are shares of its layers' keys and values, and first its row of the table.
 template <typename V>
 __global__ void __launch_bounds__(kCopyThreads) fork_kernel(const __grid_constant__ PagesParams p) {
   enter_kernel<true>();
@@ -395,8 +388,8 @@ __global__ void __launch_bounds__(kCopyThreads) fork_kernel(const __grid_constan
     report(p.status, SB_DEV_BAD_PAGE, p.a[pair]);
     return;
   }
-  const int layer = (part - 1) >> 1;
-  copy_page<V>(p, (part - 1) & 1 ? p.v : p.k, layer, old, fresh, rest);
+  const int job = p.by_parts.of(part - 1);
+  copy_page<V>(p, job & 1 ? p.v : p.k, job >> 1, old, fresh, rest, part - 1 - job * p.parts);
 }
 
 __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid_constant__ PagesParams p) {
@@ -443,17 +436,18 @@ __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid
   }
 }
 
-// Blocks below copy_blocks copy the moved pages, a (page, layer, keys or values) at a time; the others rewrite the tables.
+// Blocks below copy_blocks copy the moved pages, a share of a (page, layer, keys or values) at a time; the others rewrite the tables.
 template <typename V>
 __global__ void __launch_bounds__(kCopyThreads) compact_kernel(const __grid_constant__ PagesParams p, int copy_blocks) {
   enter_kernel<true>();
   const int moved = p.work[1], live = p.work[2];
   const int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;
   if ((int)blockIdx.x < copy_blocks) {
-    const long long jobs = (long long)moved * p.layers * 2;
+    const int per_pair = p.layers * 2 * p.parts;
+    const long long jobs = (long long)moved * per_pair;
     for (long long j = blockIdx.x; j < jobs; j += copy_blocks) {
-      const int r = (int)(j / (2 * p.layers)), part = (int)(j - (long long)r * 2 * p.layers);
-      copy_page<V>(p, part & 1 ? p.v : p.k, part >> 1, pairs[2 * r + 1], pairs[2 * r], p.page_size);
+      const int r = (int)(j / per_pair), in = (int)(j - (long long)r * per_pair), job = p.by_parts.of(in);
+      copy_page<V>(p, job & 1 ? p.v : p.k, job >> 1, pairs[2 * r + 1], pairs[2 * r], p.page_size, in - job * p.parts);
     }
     return;
   }
@@ -477,8 +471,17 @@ cudaError_t launch_append(const AppendParams &p, cudaStream_t s) {
   int sms = 0;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
-  q.per_block = (int)std::min<long long>(kMaxTokens, std::max<long long>(1, all / (8 * sms)));
+  // A block's lookups are three trips to memory before its first copy: blocks enough that others' copies are under way meanwhile.
+  // (34006 tokens x 8 heads x 128, bf16: 51, 49, 47, 55 us with 8, 16, 32, 64 blocks per SM.)
+  q.per_block = (int)std::min<long long>(kMaxTokens, std::max<long long>(1, all / (kAppendBlocks * sms)));
   const dim3 grid((unsigned)((all + q.per_block - 1) / q.per_block));
+  auto go = [&](auto kernel, int unit) {
+    q.per_row = p.head_dim * p.esize / unit;
+    q.per_token = 2 * p.kv_heads * q.per_row;
+    q.by_row = FastDiv::by(q.per_row);
+    q.by_token = FastDiv::by(q.per_token);
+    return launch_kernel(kernel, grid, kAppendThreads, 0, s, q);
+  };
   auto aligned = [&](const char *ptr, std::initializer_list<long long> strides) {
     if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0) return false;
     for (long long x : strides)
@@ -487,20 +490,34 @@ cudaError_t launch_append(const AppendParams &p, cudaStream_t s) {
   };
   if (p.head_dim * p.esize % 16 == 0 && aligned(p.k.ptr, {p.k.sb, p.k.sh, p.k.st}) && aligned(p.v.ptr, {p.v.sb, p.v.sh, p.v.st}) &&
       aligned(p.kc.ptr, {p.kc.sp, p.kc.sh, p.kc.st}) && aligned(p.vc.ptr, {p.vc.sp, p.vc.sh, p.vc.st}))
-    return launch_kernel(append_kernel<uint4>, grid, kAppendThreads, 0, s, q);
-  if (p.esize == 4) return launch_kernel(append_kernel<uint32_t>, grid, kAppendThreads, 0, s, q);
-  return launch_kernel(append_kernel<unsigned short>, grid, kAppendThreads, 0, s, q);
+    return go(append_kernel<uint4>, 16);
+  if (p.esize == 4) return go(append_kernel<uint32_t>, 4);
+  return go(append_kernel<unsigned short>, 2);
 }
 
 cudaError_t launch_extend(const PagesParams &p, cudaStream_t s) { return launch_kernel(extend_kernel, dim3(1), kBookThreads, 0, s, p); }
 
 cudaError_t launch_free(const PagesParams &p, cudaStream_t s) { return launch_kernel(free_kernel, dim3(p.n), kFreeThreads, 0, s, p); }
 
-cudaError_t launch_fork(const PagesParams &p, cudaStream_t s, int *launches) {
-  cudaError_t e = launch_kernel(fork_plan_kernel, dim3(1), kBookThreads, 0, s, p);
+// A page's heads are shared out so that there are `blocks` pieces of work, or each is one head's.
+static void set_parts(PagesParams &p, long long jobs, long long blocks) {
+  const long long parts = std::min<long long>(p.heads, std::max<long long>(1, (blocks + jobs - 1) / jobs));
+  p.part_heads = (int)((p.heads + parts - 1) / parts);
+  p.parts = (p.heads + p.part_heads - 1) / p.part_heads;
+  p.per_row = p.row_bytes / p.vec;
+  p.by_row = FastDiv::by(p.per_row);
+  p.by_parts = FastDiv::by(p.parts);
+}
+
+cudaError_t launch_fork(const PagesParams &params, cudaStream_t s, int *launches) {
+  PagesParams p = params;
+  int sms = 0;
+  cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
+  if ((e = launch_kernel(fork_plan_kernel, dim3(1), kBookThreads, 0, s, p)) != cudaSuccess) return e;
   *launches += 2;
-  const dim3 grid(1 + 2 * p.layers, p.n);
+  set_parts(p, 2LL * p.layers * p.n, 16LL * sms);
+  const dim3 grid(1 + 2 * p.layers * p.parts, p.n);
   switch (p.vec) {
     case 16: return launch_kernel(fork_kernel<uint4>, grid, kCopyThreads, 0, s, p);
     case 4: return launch_kernel(fork_kernel<uint32_t>, grid, kCopyThreads, 0, s, p);
@@ -508,12 +525,14 @@ cudaError_t launch_fork(const PagesParams &p, cudaStream_t s, int *launches) {
   }
 }
 
-cudaError_t launch_compact(const PagesParams &p, cudaStream_t s, int *launches) {
+cudaError_t launch_compact(const PagesParams &params, cudaStream_t s, int *launches) {
+  PagesParams p = params;
   int sms = 0;
   cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
   if ((e = launch_kernel(compact_plan_kernel, dim3(1), kBookThreads, 0, s, p)) != cudaSuccess) return e;
   *launches += 2;
+  set_parts(p, 1, p.heads);      // how many pages will move only the device knows: a head at a time
   const int copy_blocks = 8 * sms, table_blocks = std::min(p.max_seqs, sms);
   const dim3 grid(copy_blocks + table_blocks);
   switch (p.vec) {

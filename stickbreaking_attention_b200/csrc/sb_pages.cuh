@@ -11,6 +11,20 @@ struct CacheRef {
   long long sl, sp, sh, st;
 };
 
+// x / d for 0 <= x < 2^31 by a multiplication: with 2^l >= d > 2^(l - 1), the quotient is exactly x * ceil(2^(31 + l) / d) >> 31 + l.
+struct FastDiv {
+  unsigned mul;
+  int post, one;
+  __host__ static FastDiv by(int d) {
+    int l = 0;
+    while ((1LL << l) < d) ++l;
+    return FastDiv{(unsigned)(((1ULL << (31 + l)) + d - 1) / d), l - 1, d == 1};
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int of(int x) const { return one ? x : (int)(__umulhi((unsigned)x, mul) >> post); }
+#endif
+};
+
 struct AppendParams {
   TensorRef k, v;                  // (batch, heads, tokens, head_dim); packed: batch 1
   CacheRef kc, vc;                 // strides in elements
@@ -22,6 +36,8 @@ struct AppendParams {
   int num_seq, kv_heads, head_dim, page_size, num_pages, max_pages, esize;
   long long tokens;                // of a sequence; packed: of all
   int per_block;                   // tokens of a block
+  int per_row, per_token;          // copies of a row; of a token's rows, keys and values
+  FastDiv by_row, by_token;
   int *status;
 };
 
@@ -35,6 +51,8 @@ struct PagesParams {
   int n, count;                    // entries of a and b; extend without counts: new tokens of every sequence that has some
   CacheRef k, v;                   // fork, compact: strides in bytes
   int layers, heads, row_bytes, vec;
+  int per_row, parts, part_heads;  // copies of a row; a page's heads are copied by `parts` blocks, part_heads each
+  FastDiv by_row, by_parts;
   int *work;                       // see work_ints
   int *status;
 };
