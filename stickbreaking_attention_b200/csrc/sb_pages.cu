@@ -118,8 +118,16 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 
 // ---- the keeping of the pages ----------------------------------------------------------------------------------------------
 // One block decides what happens (which pages go where), many carry it out.  The deciding block reads the counts of all pages,
-// 16 per thread at a time.
-constexpr int kBookThreads = 1024, kPer = 16;
+// 16 per thread at a time.  What it takes for a small pool is a chain of trips to memory and barriers, so its lists are in shared
+// memory where they are short, and it has 256 threads where those do (4 sequences, 160 pages: 7.6 us with 1024 and lists in the workspace).
+constexpr int kBookThreads = 1024, kFewThreads = 256, kPer = 16, kShort = 2048;
+struct Book {
+  int scan[33];
+  int list[kShort], other[kShort];
+};
+inline int book_threads(const PagesParams &p) {
+  return p.num_pages <= kFewThreads * kPer && p.max_seqs <= 2 * kFewThreads && p.n <= 2 * kFewThreads ? kFewThreads : kBookThreads;
+}
 
 // Exclusive prefix sum over the block's threads; total in `all`.  shared: 33 ints.  Contains barriers.
 __device__ __forceinline__ int block_scan(int x, int *shared, int &all) {
@@ -134,7 +142,7 @@ __device__ __forceinline__ int block_scan(int x, int *shared, int &all) {
   if (lane == 31) shared[warp] = sum;
   __syncthreads();
   if (warp == 0) {
-    const int own = shared[lane];
+    const int own = lane < (int)(blockDim.x >> 5) ? shared[lane] : 0;
     int s = own;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -166,7 +174,7 @@ __device__ __forceinline__ void read_refs(const PagesParams &p, int first, int (
 // The `want` lowest free pages, into list; false if there are fewer.
 __device__ __forceinline__ bool list_free(const PagesParams &p, int want, int *list, int *shared) {
   int found = 0;
-  for (int base = 0; base < p.num_pages && found < want; base += kBookThreads * kPer) {
+  for (int base = 0; base < p.num_pages && found < want; base += (int)blockDim.x * kPer) {
     const int first = base + threadIdx.x * kPer;
     int x[kPer], mine = 0, all;
     read_refs(p, first, x);
@@ -194,12 +202,13 @@ __device__ __forceinline__ int pages_for(const PagesParams &p, int len) { return
 __device__ __forceinline__ int extra(const PagesParams &p, int b, int len) { return p.a != nullptr ? p.a[b] : len > 0 ? p.count : 0; }
 
 __global__ void __launch_bounds__(kBookThreads) extend_kernel(const __grid_constant__ PagesParams p) {
-  __shared__ int shared[33];
+  __shared__ Book book;
+  int *const shared = book.scan;
   enter_kernel<true>();
-  int *list = p.work + kPagesHeader, *prefix = list + p.num_pages;
+  int *list = p.work + kPagesHeader, *const prefix = p.max_seqs <= kShort ? book.other : list + p.num_pages;
   int want = 0;
   bool bad = false;
-  for (int base = 0; base < p.max_seqs; base += kBookThreads) {
+  for (int base = 0; base < p.max_seqs; base += blockDim.x) {
     const int b = base + threadIdx.x;
     int need = 0;
     if (b < p.max_seqs) {
@@ -218,11 +227,12 @@ __global__ void __launch_bounds__(kBookThreads) extend_kernel(const __grid_const
     want = min(want + all, p.num_pages + 1);
   }
   if (__syncthreads_or(bad)) return;
+  if (want <= kShort) list = book.list;
   if (want > 0 && !list_free(p, want, list, shared)) {
     if (threadIdx.x == 0) report(p.status, SB_DEV_OUT_OF_PAGES, want);
     return;
   }
-  for (int r = threadIdx.x; r < want; r += kBookThreads) {
+  for (int r = threadIdx.x; r < want; r += blockDim.x) {
     int lo = 0, hi = p.max_seqs;              // the last sequence whose pages begin at or before r
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
@@ -234,7 +244,7 @@ __global__ void __launch_bounds__(kBookThreads) extend_kernel(const __grid_const
     p.refs[page] = 1;
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < p.max_seqs; b += kBookThreads) {
+  for (int b = threadIdx.x; b < p.max_seqs; b += blockDim.x) {
     const int len = p.seq_lens[b], more = extra(p, b, len);
     if (more > 0) p.seq_lens[b] = len + more;
   }
@@ -309,14 +319,15 @@ __device__ __forceinline__ void copy_page(const PagesParams &p, const CacheRef &
 __device__ __forceinline__ int *fork_plan(const PagesParams &p) { return p.work + kPagesHeader + 2 * p.num_pages + p.max_seqs; }
 
 __global__ void __launch_bounds__(kBookThreads) fork_plan_kernel(const __grid_constant__ PagesParams p) {
-  __shared__ int shared[33];
+  __shared__ Book book;
+  int *const shared = book.scan;
   enter_kernel<true>();
-  int *list = p.work + kPagesHeader, *mark = list + 2 * p.num_pages, *plan = fork_plan(p);
+  int *list = p.work + kPagesHeader, *const mark = p.max_seqs <= kShort ? book.other : list + 2 * p.num_pages, *const plan = fork_plan(p);
   if (threadIdx.x == 0) p.work[0] = 0;
-  for (int i = threadIdx.x; i < p.max_seqs; i += kBookThreads) mark[i] = 0;
+  for (int i = threadIdx.x; i < p.max_seqs; i += blockDim.x) mark[i] = 0;
   __syncthreads();
   bool bad = false;
-  for (int i = threadIdx.x; i < p.n; i += kBookThreads) {
+  for (int i = threadIdx.x; i < p.n; i += blockDim.x) {
     const int s = p.a[i], d = p.b[i];
     int wrong = -1;
     if ((unsigned)s >= (unsigned)p.max_seqs) wrong = s;
@@ -327,14 +338,14 @@ __global__ void __launch_bounds__(kBookThreads) fork_plan_kernel(const __grid_co
     report(p.status, SB_DEV_BAD_SEQUENCE, wrong);
   }
   if (__syncthreads_or(bad)) return;
-  for (int i = threadIdx.x; i < p.n; i += kBookThreads)
+  for (int i = threadIdx.x; i < p.n; i += blockDim.x)
     if (mark[p.a[i]] != 0) {                  // a sequence cannot be forked and be a fork in one call
       bad = true;
       report(p.status, SB_DEV_BAD_SEQUENCE, p.a[i]);
     }
   if (__syncthreads_or(bad)) return;
   int want = 0;
-  for (int base = 0; base < p.n; base += kBookThreads) {
+  for (int base = 0; base < p.n; base += blockDim.x) {
     const int i = base + threadIdx.x;
     int len = 0;
     if (i < p.n) len = p.seq_lens[p.a[i]];
@@ -347,11 +358,12 @@ __global__ void __launch_bounds__(kBookThreads) fork_plan_kernel(const __grid_co
     }
     want += all;
   }
+  if (want <= kShort) list = book.list;
   if (want > p.num_pages || !list_free(p, want, list, shared)) {
     if (threadIdx.x == 0) report(p.status, SB_DEV_OUT_OF_PAGES, want);
     return;
   }
-  for (int i = threadIdx.x; i < p.n; i += kBookThreads) {
+  for (int i = threadIdx.x; i < p.n; i += blockDim.x) {
     const int rank = plan[2 * i + 1];
     if (rank >= 0) {
       plan[2 * i + 1] = list[rank];
@@ -397,7 +409,7 @@ __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid
   enter_kernel<true>();
   int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;    // (hole, page) pairs, no more than half the pages; new place of each
   int live = 0, mine = 0;
-  for (int base = 0; base < p.num_pages; base += kBookThreads * kPer) {
+  for (int base = 0; base < p.num_pages; base += (int)blockDim.x * kPer) {
     int x[kPer];
     read_refs(p, base + threadIdx.x * kPer, x);
 #pragma unroll
@@ -405,7 +417,7 @@ __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid
   }
   block_scan(mine, shared, live);
   int holes = 0, moved = 0;
-  for (int base = 0; base < p.num_pages; base += kBookThreads * kPer) {
+  for (int base = 0; base < p.num_pages; base += (int)blockDim.x * kPer) {
     const int first = base + threadIdx.x * kPer;
     int x[kPer], h = 0, m = 0, all_h, all_m;
     read_refs(p, first, x);
@@ -424,7 +436,7 @@ __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid
     moved += all_m;
   }
   __syncthreads();
-  for (int r = threadIdx.x; r < moved; r += kBookThreads) {
+  for (int r = threadIdx.x; r < moved; r += blockDim.x) {
     const int to = pairs[2 * r], from = pairs[2 * r + 1];
     place[from] = to;
     p.refs[to] = p.refs[from];
@@ -495,7 +507,7 @@ cudaError_t launch_append(const AppendParams &p, cudaStream_t s) {
   return go(append_kernel<unsigned short>, 2);
 }
 
-cudaError_t launch_extend(const PagesParams &p, cudaStream_t s) { return launch_kernel(extend_kernel, dim3(1), kBookThreads, 0, s, p); }
+cudaError_t launch_extend(const PagesParams &p, cudaStream_t s) { return launch_kernel(extend_kernel, dim3(1), book_threads(p), 0, s, p); }
 
 cudaError_t launch_free(const PagesParams &p, cudaStream_t s) { return launch_kernel(free_kernel, dim3(p.n), kFreeThreads, 0, s, p); }
 
@@ -514,7 +526,7 @@ cudaError_t launch_fork(const PagesParams &params, cudaStream_t s, int *launches
   int sms = 0;
   cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
-  if ((e = launch_kernel(fork_plan_kernel, dim3(1), kBookThreads, 0, s, p)) != cudaSuccess) return e;
+  if ((e = launch_kernel(fork_plan_kernel, dim3(1), book_threads(p), 0, s, p)) != cudaSuccess) return e;
   *launches += 2;
   set_parts(p, 2LL * p.layers * p.n, 16LL * sms);
   const dim3 grid(1 + 2 * p.layers * p.parts, p.n);
@@ -530,7 +542,7 @@ cudaError_t launch_compact(const PagesParams &params, cudaStream_t s, int *launc
   int sms = 0;
   cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
-  if ((e = launch_kernel(compact_plan_kernel, dim3(1), kBookThreads, 0, s, p)) != cudaSuccess) return e;
+  if ((e = launch_kernel(compact_plan_kernel, dim3(1), book_threads(p), 0, s, p)) != cudaSuccess) return e;
   *launches += 2;
   set_parts(p, 1, p.heads);      // how many pages will move only the device knows: a head at a time
   const int copy_blocks = 8 * sms, table_blocks = std::min(p.max_seqs, sms);

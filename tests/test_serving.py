@@ -534,7 +534,7 @@ def test_pages_refusals_on_the_device(cuda_device):
 def test_fork_and_compact_copy_all_layers(cuda_device, dtype, d, layout):
     """Copied rows, all layers and heads; every other row of the pool as it was."""
     import stickbreaking_attention_b200 as sb
-    layers, pages, kv, page = (1 if layout == "one_layer" else 3), 30, 2, 16
+    layers, pages, kv, page = (1 if layout == "one_layer" else 3), 30, 5, 16
     gen = torch.Generator().manual_seed(30)
     ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda_device)
 
