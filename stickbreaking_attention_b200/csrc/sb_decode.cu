@@ -335,17 +335,19 @@ cudaError_t launch_decode_simt(const DecodeParams &p, int dtype, cudaStream_t s)
 }
 
 // The columns behind head_dim that a part reads (up to 127) lie in the next row, or behind the last one in the padding that the
-// workspace has there.  By the pieces that an item is cut into on the average, 1, 4 or 32 warps share a part.
+// workspace has there.  By the pieces that an item is cut into on the average, 1, 4 or 32 warps share a part, 8
+// where 32 would not all find room at once.
 cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s) {
   const long long items = (long long)p.batch * p.items_per_seq;
   const int notes = (int)(p.by_item ? items : p.chunks);
   const int jobs = p.rows_per_block * ((p.head_dim + kJoinCols - 1) / kJoinCols);
-  const int together = p.chunks < 4 * items ? 1 : p.chunks < 16 * items ? 4 : 32;
+  const int together = p.chunks < 4 * items ? 1 : p.chunks < 16 * items ? 4 : items * jobs > 2 * p.chunks / 12 ? 8 : 32;
   auto go = [&](auto kernel, int warps, int per_block) {
     return launch_kernel(kernel, dim3(notes, (jobs + per_block - 1) / per_block), warps * 32, 0, s, p);
   };
 #define SB_JOIN(T)                                               \
   together == 32  ? go(decode_join_kernel<T, 32, 32>, 32, 1)     \
+  : together == 8 ? go(decode_join_kernel<T, 8, 8>, 8, 1)        \
   : together == 4 ? go(decode_join_kernel<T, 4, 4>, 4, 1)        \
                   : go(decode_join_kernel<T, 4, 1>, 4, 4)
   switch (dtype) {

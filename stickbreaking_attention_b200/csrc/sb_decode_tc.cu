@@ -477,17 +477,18 @@ cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s) {
   return dtype == SB_DTYPE_BF16 ? launch_shape<__nv_bfloat16>(p, s) : launch_shape<__half>(p, s);
 }
 
-// By the pieces that an item is cut into on the average: 1, 4 or 32 warps share a part.  (64 sequences x 16 heads, 1.7 pieces: 19 us
+// By the pieces that an item is cut into on the average: 1, 4 or 32 warps share a part, 8 where 32 would not all find room at once.  (64 sequences x 16 heads, 1.7 pieces: 19 us
 // after the main kernel with 4 warps to a part, 32768 of them, and 6 with one.)
 cudaError_t launch_decode_tc_join(const DecodeParams &p, int dtype, cudaStream_t s) {
   const long long items = (long long)p.batch * p.items_per_seq;
   const int notes = (int)(p.by_item ? items : p.chunks), jobs = p.rows_per_block / 8 * (p.part_cols / 16);
-  const int together = p.chunks < 4 * items ? 1 : p.chunks < 16 * items ? 4 : 32;
+  const int together = p.chunks < 4 * items ? 1 : p.chunks < 16 * items ? 4 : items * jobs > 2 * p.chunks / 12 ? 8 : 32;
   auto go = [&](auto kernel, int warps, int per_block) {
     return launch_kernel(kernel, dim3(notes, (jobs + per_block - 1) / per_block), warps * 32, 0, s, p);
   };
 #define SB_JOIN(T)                                                  \
   together == 32  ? go(decode_tc_join_kernel<T, 32, 32>, 32, 1)     \
+  : together == 8 ? go(decode_tc_join_kernel<T, 8, 8>, 8, 1)        \
   : together == 4 ? go(decode_tc_join_kernel<T, 4, 4>, 4, 1)        \
                   : go(decode_tc_join_kernel<T, 4, 1>, 4, 4)
   return dtype == SB_DTYPE_BF16 ? SB_JOIN(__nv_bfloat16) : SB_JOIN(__half);
