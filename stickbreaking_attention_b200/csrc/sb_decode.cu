@@ -12,12 +12,14 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool ta
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
 }
 
-// kCols: columns a lane holds (32 kCols >= head_dim).
-template <int kCols> struct SimtShape {
+// kCols: columns a lane holds (32 kCols >= head_dim); kRows: query rows.  As many warps as registers and shared memory allow: a
+// tile is a long chain (16 dots, a scan, 16 sums), other warps' tiles fill it, and their copies are in flight as well.
+// (fp32, 8 heads x 128 columns, 20 sequences of 157 to 8150 tokens: 122, 92, 73 us with 4, 6, 12 warps of 3, 2, 1 stages.)
+template <int kCols, int kRows> struct SimtShape {
   static constexpr int kWidth = 32 * kCols;                              // floats of a row in shared memory
-  static constexpr int kWarps = kCols <= 2 ? 8 : kCols <= 4 ? 4 : 2;
-  static constexpr int kStages = 3;
+  static constexpr int kWarps = kCols <= 2 ? 12 : kCols <= 4 ? (kRows <= 4 ? 12 : 8) : 6;
   static constexpr int kStage = 2 * kTileKeys * kWidth * 4;              // 16 keys, 16 values
+  static constexpr int kStages = 192 * 1024 / (kWarps * kStage);
   static constexpr int kBytes = kWarps * kStages * kStage;               // 192 KiB
 };
 
@@ -41,8 +43,8 @@ template <int kCols> __device__ __forceinline__ int col_of(int lane, int i) {
 // The CUDA-core engine.  kRows: query rows (1, 2, 4, 8); kVec: bytes of a copy (fp32: 16 or 4; 16-bit types: 0, converted on the
 // way).  Lane l holds the scores of row 2 pair + (l & 1) at key l >> 1 of the tile: 16 keys and two rows fill a warp, and the scan
 // over keys takes four shuffles.  `left`: natural log of the stick that remains.
-template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtShape<kCols> {
-  using S = SimtShape<kCols>;
+template <typename T, int kCols, int kRows, int kVec> struct SimtEngine : SimtShape<kCols, kRows> {
+  using S = SimtShape<kCols, kRows>;
   using S::kWidth;
   static constexpr int kPairs = (kRows + 1) / 2;
   float q[kRows][kCols], acc[kRows][kCols];
@@ -321,7 +323,11 @@ template <typename T, int kVec> cudaError_t launch_cols(const DecodeParams &p, c
 
 // (More rows of a head_dim over 128 than four do not fit into a thread's registers.)
 int decode_simt_rows(int rows, int head_dim) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 || head_dim > 128 ? 4 : 8; }
-int decode_simt_warps(int head_dim) { return head_dim <= 64 ? SimtShape<2>::kWarps : head_dim <= 128 ? SimtShape<4>::kWarps : SimtShape<8>::kWarps; }
+int decode_simt_warps(int rows, int head_dim) {
+  if (head_dim <= 64) return SimtShape<2, 1>::kWarps;
+  if (head_dim <= 128) return rows <= 4 ? SimtShape<4, 4>::kWarps : SimtShape<4, 8>::kWarps;
+  return SimtShape<8, 1>::kWarps;
+}
 
 cudaError_t launch_decode_simt(const DecodeParams &p, int dtype, cudaStream_t s) {
   auto aligned = [](const PagedRef &t) {
@@ -335,13 +341,13 @@ cudaError_t launch_decode_simt(const DecodeParams &p, int dtype, cudaStream_t s)
 }
 
 // The columns behind head_dim that a part reads (up to 127) lie in the next row, or behind the last one in the padding that the
-// workspace has there.  By the pieces that an item is cut into on the average, 1, 4 or 32 warps share a part, 8
-// where 32 would not all find room at once.
+// workspace has there.  By the pieces that an item is cut into on the average, 1, 4, 8 or 32 warps
+// share a part.
 cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s) {
   const long long items = (long long)p.batch * p.items_per_seq;
   const int notes = (int)(p.by_item ? items : p.chunks);
   const int jobs = p.rows_per_block * ((p.head_dim + kJoinCols - 1) / kJoinCols);
-  const int together = p.chunks < 4 * items ? 1 : p.chunks < 16 * items ? 4 : items * jobs > 2 * p.chunks / 12 ? 8 : 32;
+  const int together = p.chunks < 4 * items ? 1 : p.chunks < 16 * items ? 4 : p.chunks < 256 * items ? 8 : 32;
   auto go = [&](auto kernel, int warps, int per_block) {
     return launch_kernel(kernel, dim3(notes, (jobs + per_block - 1) / per_block), warps * 32, 0, s, p);
   };

@@ -375,6 +375,6 @@ int decode_tc_rows(int rows, int head_dim);     // query rows per item
 int decode_simt_rows(int rows, int head_dim);
 int decode_tc_cols(int head_dim);               // columns of a piece in the workspace
 int decode_tc_warps(int rows, int head_dim);    // warps per block for so many rows per item; one block per SM
-int decode_simt_warps(int head_dim);
+int decode_simt_warps(int rows, int head_dim);
 
 }  // namespace sb

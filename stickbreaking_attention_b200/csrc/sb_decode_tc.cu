@@ -34,7 +34,9 @@ using ptx::rcp;
 using ptx::smem_u32;
 
 // kD: head_dim rounded up to 64, 128, 256; kN: blocks of 8 query rows.  As many warps as their registers allow: a tile is a
-// chain of some 800 cycles (scores, scan over keys, weights, values), and other warps' tiles are what fills them.
+// chain of some 700 cycles (scores, scan over keys, weights, values), and other warps' tiles are what fills them.  (128 columns, 8
+// rows: 64 sequences x 16 heads x 512..4096 tokens 161, 155, 150 us with 8, 12, 16 warps, 48 ragged sequences of shared key heads,
+// half of them local, 120, 89, 93; 16 warps spill.)
 template <int kD, int kN> struct TcShape {
   static constexpr int kChunks = kD / 8;                            // 16-byte chunks of a row
   static constexpr int kHalf = kTileKeys * kD * 2;                  // bytes of a stage's keys (or values)
@@ -477,12 +479,12 @@ cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s) {
   return dtype == SB_DTYPE_BF16 ? launch_shape<__nv_bfloat16>(p, s) : launch_shape<__half>(p, s);
 }
 
-// By the pieces that an item is cut into on the average: 1, 4 or 32 warps share a part, 8 where 32 would not all find room at once.  (64 sequences x 16 heads, 1.7 pieces: 19 us
+// By the pieces that an item is cut into on the average: 1, 4, 8 or 32 warps share a part.  (64 sequences x 16 heads, 1.7 pieces: 19 us
 // after the main kernel with 4 warps to a part, 32768 of them, and 6 with one.)
 cudaError_t launch_decode_tc_join(const DecodeParams &p, int dtype, cudaStream_t s) {
   const long long items = (long long)p.batch * p.items_per_seq;
   const int notes = (int)(p.by_item ? items : p.chunks), jobs = p.rows_per_block / 8 * (p.part_cols / 16);
-  const int together = p.chunks < 4 * items ? 1 : p.chunks < 16 * items ? 4 : items * jobs > 2 * p.chunks / 12 ? 8 : 32;
+  const int together = p.chunks < 4 * items ? 1 : p.chunks < 16 * items ? 4 : p.chunks < 256 * items ? 8 : 32;
   auto go = [&](auto kernel, int warps, int per_block) {
     return launch_kernel(kernel, dim3(notes, (jobs + per_block - 1) / per_block), warps * 32, 0, s, p);
   };

@@ -70,7 +70,7 @@ int plan_decode(const SbDecodeParams *p, DecodePlan &pl) {
   int sms = 0;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return fail(SB_ERR_CUDA, "SM count: %s", cudaGetErrorString(e));
-  pl.chunks = sms * (tc ? decode_tc_warps(pl.rows_per_block, p->head_dim) : decode_simt_warps(p->head_dim));
+  pl.chunks = sms * (tc ? decode_tc_warps(pl.rows_per_block, p->head_dim) : decode_simt_warps(pl.rows_per_block, p->head_dim));
   const long long items = (long long)p->batch * p->kv_heads * pl.row_blocks;
   pl.by_item = items < pl.chunks;
   pl.part_cols = tc ? decode_tc_cols(p->head_dim) : p->head_dim;
