@@ -119,7 +119,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // ---- the keeping of the pages ----------------------------------------------------------------------------------------------
 // One block decides what happens (which pages go where), many carry it out.  The deciding block reads the counts of all pages,
 // 16 per thread at a time.  What it takes for a small pool is a chain of trips to memory and barriers, so its lists are in shared
-// memory where they are short, and it has 256 threads where those do (4 sequences, 160 pages: 7.6 us with 1024 and lists in the workspace).
+// memory where they are short, and it has 256 threads where those do (a fork of 4 sequences in 160 pages: 4.0 us, 7.6 with
+// 1024 and lists in the workspace).
 constexpr int kBookThreads = 1024, kFewThreads = 256, kPer = 16, kShort = 2048;
 struct Book {
   int scan[33];

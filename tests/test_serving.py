@@ -290,6 +290,64 @@ def test_decode_pools_beyond_32_bit_offsets(cuda_device):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_decode_as_many_new_tokens_as_keys(cuda_device, dtype):
+    """Up to 1024 new tokens, in many blocks of rows, some in front of their sequences."""
+    import stickbreaking_attention_b200 as sb
+    lens, d, page = [1024, 150, 0, 1030], 8, 16
+    q, cache = make(16, lens, 2, 1, d, page, dtype, new=1024, shift=0.5)
+    got = run_decode(sb, cuda_device, q, cache)
+    gen = torch.Generator().manual_seed(17)
+    some = sorted({0, 1, 5, 15, 16, 17, 873, 874, 875, 1022, 1023, *torch.randint(0, 1024, (12,), generator=gen).tolist()})
+    for t in some:                                       # token t is the last of a batch that ends with it
+        ends = (cache[3] - 1023 + t).clamp(min=0).int()
+        want = R.decode(q[:, :, t:t + 1], *cache[:3], ends)
+        R.check_decode((got[0][:, :, t:t + 1], got[1][:, :, t:t + 1]), want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_decode_tables_of_enormous_capacity(cuda_device, dtype):
+    """1024 sequences with room for 39 million tokens each: more tiles than 31 bits count, if all of them were in use."""
+    import stickbreaking_attention_b200 as sb
+    gen = torch.Generator().manual_seed(18)
+    batch, page, d = 1024, 65536, 8
+    k, v = (torch.randn(2, 1, page, d, generator=gen).to(dtype) for _ in range(2))
+    table = torch.full((batch, 600), -1, dtype=torch.int32)
+    table[:, 0] = torch.arange(batch) % 2                # pages may be shared by any number of readers
+    lens = torch.randint(0, 200, (batch,), generator=gen, dtype=torch.int32)
+    lens[7], lens[500] = 4000, 65536
+    q = torch.randn(batch, 1, 1, d, generator=gen).to(dtype)
+    R.check_decode(run_decode(sb, cuda_device, q, (k, v, table, lens)), R.decode(q, k, v, table, lens))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_two_captured_graphs_at_once(cuda_device, dtype):
+    """Two graphs with an attention each, replayed on two streams at the same time: neither uses the other's scratch."""
+    import stickbreaking_attention_b200 as sb
+    sets = []
+    with torch.no_grad():
+        for seed, lens in ((19, [9000, 40]), (20, [300, 7000, 1])):
+            q, cache = make(seed, lens, 8, 2, 64, 16, dtype, shift=0.8)
+            args = [t.to(cuda_device) for t in (q, *cache)]
+            want = sb.sb_attn_decode(*args)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = [sb.sb_attn_decode(*args) for _ in range(5)]
+            sets.append((graph, out, want, torch.cuda.Stream(), args))     # (the graph reads the inputs where they are)
+        for _ in range(4):
+            for graph, _, _, stream, _ in sets:
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+    for _, out, want, _, _ in sets:
+        for o, rem in out:
+            assert torch.equal(o, want[0]) and torch.equal(rem, want[1])
+
+
+@gpu
 @pytest.mark.parametrize("dtype,d", [(FP32, 64), (BF16, 128), (FP16, 64), (BF16, 50)])
 def test_decode_gives_the_rows_of_the_whole_attention(cuda_device, dtype, d):
     import stickbreaking_attention_b200 as sb
@@ -389,6 +447,32 @@ def test_append_large_pool_of_tokens_and_views(cuda_device):
         sb.kv_append(dev(k), dev(v), ck, cv, dev(table), dev(lengths), dev(ends), zero_start=False)
         sb.check_status(cuda_device)
         assert same(ck.contiguous(), want[0]) and same(cv.contiguous(), want[1])
+
+
+@gpu
+def test_append_many_small_tokens(cuda_device):
+    """400000 tokens of one head and 8 columns: blocks of 64 tokens."""
+    import stickbreaking_attention_b200 as sb
+    page, lens = 64, [150000, 1, 249999]
+    gen = torch.Generator().manual_seed(24)
+    pages = sum(-(-n // page) for n in lens)
+    order = torch.randperm(pages, generator=gen).int()
+    table = torch.full((3, 4000), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(lens):
+        count = -(-n // page)
+        table[b, :count] = order[at:at + count]
+        at += count
+    k, v = (torch.randn(1, sum(lens), 8, generator=gen).to(BF16).to(cuda_device) for _ in range(2))
+    kp, vp = (torch.zeros(pages, 1, page, 8, dtype=BF16, device=cuda_device) for _ in range(2))
+    cu = torch.tensor([0] + lens).cumsum(0).to(cuda_device)
+    sb.kv_append(k, v, kp, vp, table.to(cuda_device), torch.tensor(lens, dtype=torch.int32, device=cuda_device), cu)
+    sb.check_status(cuda_device)
+    for b, n in enumerate(lens):
+        rows = table[b, : -(-n // page)].long().to(cuda_device)
+        for pool, new in ((kp, k), (vp, v)):
+            assert torch.equal(pool[rows, 0].flatten(0, 1)[:n], new[0, int(cu[b]):int(cu[b + 1])])
+            assert bool((pool[rows, 0].flatten(0, 1)[n:] == 0).all())
 
 
 @gpu
@@ -499,6 +583,39 @@ def test_pages_random_programs(cuda_device, page, max_seqs, num_pages, seed):
                     got = k[layer].transpose(1, 2).flatten(0, 1)[at]
                     assert bool((got == (want + 0.5 * layer)[:, None, None]).all())
                     assert bool((v[layer].transpose(1, 2).flatten(0, 1)[at] == -(want + 0.5 * layer)[:, None, None]).all())
+
+
+@gpu
+def test_pages_of_many_sequences(cuda_device):
+    """Books too long for shared memory: 6000 sequences, 2600 forks in one call, a sequence of 5000 pages."""
+    import stickbreaking_attention_b200 as sb
+    page, max_seqs, num_pages, max_pages = 4, 6000, 20000, 5200
+    cache = sb.PagedKVCache(1, num_pages, 1, page, 8, max_seqs, max_pages * page, dtype=BF16, device=cuda_device)
+    books = R.Books(max_seqs, max_pages, num_pages, page)
+    rng = random.Random(31)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)
+    counts = [rng.randint(0, 9) if s < 2600 else 0 for s in range(max_seqs)]
+    counts[17] = 20000
+    src = list(range(2600))
+    rng.shuffle(src)
+    dst = list(range(3000, 5600))
+    gone = [rng.randrange(max_seqs) for _ in range(3000)]
+
+    def step(ok, call):
+        assert ok
+        call()
+        sb.check_status(cuda_device)
+        books_equal(cache, books)
+
+    step(books.extend(torch.tensor(counts)), lambda: cache.extend(ints(counts)))
+    for s in range(max_seqs):
+        for pos in range(books.lens[s]):
+            books.write(s, pos, 0)
+    step(books.fork(src, dst), lambda: cache.fork(ints(src), ints(dst)))
+    step(books.free(gone), lambda: cache.free(ints(gone)))
+    books.compact()
+    step(True, cache.compact)
+    step(books.extend(3), lambda: cache.extend(3))
 
 
 @gpu
