@@ -19,9 +19,11 @@
 // difference loses nothing over thousands of keys that take 1e-5 each, whose 1 - beta are rounded in their last bits; the
 // product loses nothing where little is left.  The tile's weights are added up by one more product, with ones for values.
 //
-// P enters the second product as the sum of two 16-bit numbers (16 or 22 bits): rounded once it would double the error that the
-// output's own rounding makes, and the second product of the pair is free.  In fp16 it is scaled by 2^15, since a weight of 1e-5
-// has few bits left there.  Scores, weights and the output's accumulators are 32-bit, the stick 32-bit with what its sums lost.
+// P enters the second product as the sum of 16-bit numbers: three in bf16 (24 bits, as many as the weights have) and two in fp16
+// (22 bits).  With two in bf16, 16 bits, the share of output values that are not the nearest of their type to the exact one is
+// 1.9e-3 for 5.2e-4 with three (48 ragged sequences of shared key heads) and 2.6e-3 for 1.7e-3 (64 x 16 heads of their own); the
+// third costs 92.4 us for 89.7, and 153.5 for 152.8.  In fp16 weights are scaled by 2^15 and so held in steps of 2^-39: each is
+// off by up to 2^-40.  Scores, weights and the output's accumulators are 32-bit, the stick 32-bit with what its sums lost.
 #include "sb_decode.cuh"
 #include "sb_ptx.cuh"
 
@@ -84,6 +86,8 @@ template <typename T> constexpr float kScaleP = 1.0f;
 template <> constexpr float kScaleP<__half> = 32768.0f;
 template <typename T> constexpr uint32_t kOnes = 0x3f803f80;      // two times 1.0
 template <> constexpr uint32_t kOnes<__half> = 0x3c003c00;
+template <typename T> constexpr int kParts = 3;                    // 16-bit numbers that make up a weight
+template <> constexpr int kParts<__half> = 2;
 
 // Where chunk c of row r of a stage's keys or values lies: blocks of 64 columns, rows of 128 bytes, swizzled.
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
@@ -168,9 +172,9 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
     }
   }
 
-  // O^T += V^T P^T, P as two 16-bit numbers; `b`: [row block][rows m, m + 8][high, low].  kSome: only for the queries whose
+  // O^T += V^T P^T; `b`: the weights, [row block][rows m, m + 8][part, the largest first].  kSome: only for the queries whose
   // limits are in [low, high).
-  template <bool kSome> __device__ __forceinline__ void add_values(uint32_t values, const uint32_t (&b)[kN][2][2], int low, int high) {
+  template <bool kSome> __device__ __forceinline__ void add_values(uint32_t values, const uint32_t (&b)[kN][2][kParts<T>], int low, int high) {
     const int lane = threadIdx.x & 31;
     const int r = key_of(lane & 7, lane >> 4), c = (lane >> 3) & 1;
 #pragma unroll
@@ -182,8 +186,8 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
         float o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] = acc[i][n][j];
-        mma<T>(o, a, b[n][0][0], b[n][1][0]);
-        mma<T>(o, a, b[n][0][1], b[n][1][1]);
+#pragma unroll
+        for (int part = 0; part < kParts<T>; ++part) mma<T>(o, a, b[n][0][part], b[n][1][part]);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (!kSome || (limit[n][j & 1] >= low && limit[n][j & 1] < high)) acc[i][n][j] = o[j];
@@ -245,23 +249,26 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
         a[n][2 + j] = beta[1] * (g < 4 ? whole : whole * kept[0]);
       }
     }
-    // the two 16-bit parts of the weights, moved from (key, query) to (query, key)
-    uint32_t b[kN][2][2];
+    // the 16-bit parts of the weights, moved from (key, query) to (query, key)
+    uint32_t b[kN][2][kParts<T>];
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int row = 0; row < 2; ++row) {
-        const uint32_t hi = pack<T>(a[n][2 * row], a[n][2 * row + 1]);
-        const float2 back = unpack<T>(hi);
-        b[n][row][0] = transpose8x8(hi);
-        b[n][row][1] = transpose8x8(pack<T>(a[n][2 * row] - back.x, a[n][2 * row + 1] - back.y));
-      }
+      for (int row = 0; row < 2; ++row)
+#pragma unroll
+        for (int part = 0; part < kParts<T>; ++part) {
+          const uint32_t rounded = pack<T>(a[n][2 * row], a[n][2 * row + 1]);
+          const float2 back = unpack<T>(rounded);
+          a[n][2 * row] -= back.x;               // what is left for the parts behind this one, exactly
+          a[n][2 * row + 1] -= back.y;
+          b[n][row][part] = transpose8x8(rounded);
+        }
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       const uint32_t ones[4] = {kOnes<T>, kOnes<T>, kOnes<T>, kOnes<T>};
       float sum[4] = {};                             // [j]: all weights of query 2 t + j
-      mma<T>(sum, ones, b[n][0][0], b[n][1][0]);
-      mma<T>(sum, ones, b[n][0][1], b[n][1][1]);
+#pragma unroll
+      for (int part = 0; part < kParts<T>; ++part) mma<T>(sum, ones, b[n][0][part], b[n][1][part]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (rest[n][j] > 0.875f) stick[n][j].add(sum[j] * (-1.0f / kScaleP<T>));

@@ -1,0 +1,43 @@
+"""The serving operators where they are easily wrong: bits of the weights."""
+import pytest
+import torch
+
+import serving_reference as R
+
+gpu = pytest.mark.gpu
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_decode_weights_keep_their_bits(cuda_device, dtype):
+    """Values that cancel: what is left of o shows the errors of the weights themselves, not the rounding of the output.
+
+    Bound, relative to sum a|v|.  Scores of up to 0.1 (8 columns): dz = 10 * 2^-24 * 0.1, three times at most in a weight.  beta and
+    1 - beta: the exponential 2^-22 (halved by 1 / (1 + e)), three roundings of 2^-24, the reciprocal 2^-23: 2^-21.4; a weight has
+    up to three of them and three products: 1.3e-6.  The sums in 32 bits, perhaps truncated: 3 * 2^-23.  Together below 2^-19.
+    Weights in 16 bits would be off by up to 2^-18, a quarter of these rows by more than the bound."""
+    import stickbreaking_attention_b200 as sb
+    gen = torch.Generator().manual_seed(60)
+    seqs, heads, d = 64, 8, 8
+    q, k = (0.1 * (2 * torch.rand(shape, generator=gen) - 1) for shape in ((seqs, heads, 1, d), (seqs, heads, 3, d)))
+    q, k = (10 * q).to(dtype), k.to(dtype)                            # |<q, k>| <= 8 * 0.1, times 1/8
+    z = (k.double() @ q.double().transpose(2, 3)).squeeze(3) / 8      # (seqs, heads, 3)
+    beta = torch.sigmoid(z)
+    a = beta * torch.stack(((1 - beta[..., 1]) * (1 - beta[..., 2]), 1 - beta[..., 2], torch.ones_like(beta[..., 2])), -1)
+    v = torch.zeros(seqs, heads, 3, d, dtype=torch.float64)
+    v[..., 2, :] = (1 + torch.rand(seqs, heads, d, generator=gen)).to(dtype).double()
+    for j in (1, 0):                                                  # each takes away what the newer ones sum up to
+        v[..., j, :] = (-(a[..., None] * v).sum(2) / a[..., j, None]).to(dtype).double()
+    want = (a[..., None] * v).sum(2)
+    bound = (2.0 ** -19 + 3 * 10 * 2.0 ** -24 * 0.1) * (a[..., None] * v.abs()).sum(2) + R.EPS[dtype] / 2 * want.abs() + R.SMALLEST[dtype]
+    pages = [torch.nn.functional.pad(t.to(dtype), (0, 0, 0, 13)).to(cuda_device) for t in (k, v)]
+    table = torch.arange(seqs, dtype=torch.int32, device=cuda_device)[:, None]
+    lens = torch.full((seqs,), 3, dtype=torch.int32, device=cuda_device)
+    with torch.no_grad():
+        o, _ = sb.sb_attn_decode(q.to(cuda_device), *pages, table, lens, inv_temp=0.125, attend_current=True)
+    sb.check_status(cuda_device)
+    off = (o[:, :, 0].cpu().double() - want).abs() / bound
+    assert float(off.max()) <= 1.0, f"{float(off.max()):.3g} times what rounding explains"
