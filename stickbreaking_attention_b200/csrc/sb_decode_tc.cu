@@ -17,7 +17,11 @@
 //   weight = stick * (product of 1 - beta over the tile's later keys) * beta,
 // and the stick behind the tile is what was there less the tile's weights, where more than 7/8 of it are left, else the product.  The
 // difference loses nothing over thousands of keys that take 1e-5 each, whose 1 - beta are rounded in their last bits; the
-// product loses nothing where little is left.  The tile's weights are added up by one more product, with ones for values.
+// product loses nothing where little is left.  The tile's weights are added up by one more product, with ones for values, as
+// 16-bit numbers, whose steps have an end: a stick below 2^-16 in fp16, 2^-100 in bf16, is the product always, or it would stand still
+// where a tile's weights are 0 in 16 bits.  (The last bits of 1 - beta, 2^-21 of the stick per tile, are then as much as the steps of
+// 2^-39 of 16 weights, and of a share of 2^-16 of the whole.)  Below 2^-100 it is rounded down, so that it comes to 0
+// instead of standing still at fp32's smallest numbers.
 //
 // P enters the second product as the sum of 16-bit numbers: three in bf16 (24 bits, as many as the weights have) and two in fp16
 // (22 bits).  With two in bf16, 16 bits, the share of output values that are not the nearest of their type to the exact one is
@@ -86,6 +90,8 @@ template <typename T> constexpr float kScaleP = 1.0f;
 template <> constexpr float kScaleP<__half> = 32768.0f;
 template <typename T> constexpr uint32_t kOnes = 0x3f803f80;      // two times 1.0
 template <> constexpr uint32_t kOnes<__half> = 0x3c003c00;
+template <typename T> constexpr float kSmallStick = 0x1p-100f;     // from here on the difference is not taken
+template <> constexpr float kSmallStick<__half> = 0x1p-16f;
 template <typename T> constexpr int kParts = 3;                    // 16-bit numbers that make up a weight
 template <> constexpr int kParts<__half> = 2;
 
@@ -271,8 +277,9 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
       for (int part = 0; part < kParts<T>; ++part) mma<T>(sum, ones, b[n][0][part], b[n][1][part]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (rest[n][j] > 0.875f) stick[n][j].add(sum[j] * (-1.0f / kScaleP<T>));
-        else stick[n][j] = LongSum{stick[n][j].sum * rest[n][j], 0.0f};
+        const float whole = stick[n][j].sum;
+        if (rest[n][j] > 0.875f && whole > kSmallStick<T>) stick[n][j].add(sum[j] * (-1.0f / kScaleP<T>));
+        else stick[n][j] = LongSum{whole > 0x1p-100f ? whole * rest[n][j] : __fmul_rz(whole, rest[n][j]), 0.0f};
       }
     }
     const uint32_t values = stage + kHalf;

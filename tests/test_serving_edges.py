@@ -1,4 +1,6 @@
-"""The serving operators where they are easily wrong: bits of the weights."""
+"""The serving operators where they are easily wrong: bits of the weights, sticks that wear down slowly."""
+import math
+
 import pytest
 import torch
 
@@ -41,3 +43,35 @@ def test_decode_weights_keep_their_bits(cuda_device, dtype):
     sb.check_status(cuda_device)
     off = (o[:, :, 0].cpu().double() - want).abs() / bound
     assert float(off.max()) <= 1.0, f"{float(off.max()):.3g} times what rounding explains"
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("bits", [30, 60, 155])
+def test_decode_sticks_that_wear_down_slowly(cuda_device, dtype, bits):
+    """Thousands of keys that take 1/192 of the stick each, and behind them one that would take all of the rest: its weight is what
+    is left of the stick, and it has the only value that is not 0.  2000 sequences with the same pages, so that few are cut.
+
+    Bound: the reference's, and of the weight itself 2^-145 (a stick of few bits, 2^-149 to 2^-126, loses up to one of its steps of
+    2^-149 per tile, of which 12 are left at a time), in fp16 2^-40 (weights are held in steps of 2^-39)."""
+    import stickbreaking_attention_b200 as sb
+    seqs, d, page, z = 2000, 8, 64, -5.25
+    newer = math.ceil(bits * math.log(2) / math.log1p(math.exp(z)))
+    n = newer + 1
+    pages = -(-n // page)
+    k, v = (torch.zeros(pages, 1, page, d, dtype=dtype) for _ in range(2))
+    k[..., 0] = z
+    k[0, 0, 0, 0] = 30.0
+    large = 60000.0 if dtype == FP16 else 1e38
+    v[0, 0, 0] = large
+    q = torch.zeros(1, 1, 1, d, dtype=dtype)
+    q[..., 0] = 1.0
+    table, lens = torch.arange(pages, dtype=torch.int32)[None], torch.tensor([n], dtype=torch.int32)
+    o, rem, o_err, rem_err = R.decode(q, k, v, table, lens, scale=1.0, attend_current=True)
+    o_err = o_err + (2.0 ** -40 if dtype == FP16 else 2.0 ** -145) * large
+    dev = lambda t: t.to(cuda_device)
+    with torch.no_grad():
+        got = sb.sb_attn_decode(dev(q).expand(seqs, 1, 1, d), dev(k), dev(v), dev(table).expand(seqs, pages).contiguous(),
+                                dev(lens).expand(seqs).contiguous(), inv_temp=1.0, attend_current=True)
+    sb.check_status(cuda_device)
+    R.check_decode(got, tuple(t.expand(seqs, *t.shape[1:]) for t in (o, rem, o_err, rem_err)))
