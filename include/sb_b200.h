@@ -54,8 +54,8 @@ enum SbDeviceStatus {
   SB_DEV_WAIT_TIMEOUT = 2,   /* a bounded on-chip wait gave up; status[1] = which barrier      */
   SB_DEV_BAD_PAGE = 3,       /* a page table names a page that the pool does not have, for a token that its
                                 sequence holds; status[1] = sequence.  The page is not touched        */
-  SB_DEV_BAD_SEQ_LEN = 4,    /* a sequence's length, or the length it would grow to, is negative or beyond its row of
-                                the page table; status[1] = sequence                                  */
+  SB_DEV_BAD_SEQ_LEN = 4,    /* a sequence's length, or the length it would grow to, is negative, beyond its row of
+                                the page table or beyond 2^31 - 16; status[1] = sequence              */
   SB_DEV_OUT_OF_PAGES = 5,   /* fewer free pages than the call needs; status[1] = how many it needs.  Nothing was changed */
   SB_DEV_BAD_SEQUENCE = 6    /* an index of sb_kv_fork or sb_kv_free is no sequence, or one that the call cannot take;
                                 status[1] = the index.  Nothing was changed                           */
@@ -232,7 +232,8 @@ SB_EXPORT size_t sb_set_backward_scratch_budget(size_t bytes);
  * The cache.  Keys and values live in pools of pages; a page holds `page_size` consecutive tokens of one sequence, for all
  * key heads: (layers, pages, kv_heads, page_size, head_dim) with a unit stride on head_dim and any positive strides on the
  * other axes (so (pages, page_size, kv_heads, head_dim) is a matter of strides).  `page_table` row b lists the pages of
- * sequence b in the order of its tokens, `seq_lens[b]` is its length.  Entries behind the last page in use are not read.
+ * sequence b in the order of its tokens, `seq_lens[b]` is its length, 2^31 - 16 at most.  Entries behind the last page in use are
+ * not read.
  * Lengths and tables stay on the device; no call looks at them on the host.  The reference has no cache: its operators
  * attend over whole sequences (sb_varlen/__init__.py:24-82).                                                           */
 typedef struct SbCache {

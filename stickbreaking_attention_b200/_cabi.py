@@ -25,7 +25,8 @@ SB_DEV_MESSAGES = {
        "or without its leading zero); offending sequence index: {0}",
     2: "a bounded on-chip wait timed out in barrier {0}",
     3: "a page table names a page that the cache does not have; sequence: {0}",
-    4: "a sequence's length, or the length it would grow to, is negative or beyond its row of the page table; sequence: {0}",
+    4: "a sequence's length, or the length it would grow to, is negative, beyond its row of the page table or beyond 2^31 - 16; "
+       "sequence: {0}",
     5: "the cache has too few free pages: {0} needed; nothing was changed",
     6: "listed sequence {0} is none, or one that the call cannot take; nothing was changed",
 }

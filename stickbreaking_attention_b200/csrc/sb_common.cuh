@@ -359,6 +359,13 @@ inline cudaError_t launch_kernel(void (*kernel)(Params...), dim3 grid, int threa
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// A length that a cached sequence can have: as many tokens as its row of the page table has room for, and so few that the tile
+// behind the last key is still counted in 31 bits.
+constexpr int kMostTokens = 0x7ffffff0;
+__device__ __forceinline__ bool cached_length_ok(long long len, int max_pages, int page_size) {
+  return len >= 0 && len <= kMostTokens && len <= (long long)max_pages * page_size;
+}
+
 // Of every C entry point: the thread's error text and launch count start over (the count's address); an error's code and text;
 // whether the current device can run the kernels.
 int *begin_call();

@@ -55,7 +55,7 @@ struct DecodeParams {
 // What a sequence's length says: its keys that some query attends to, or -1 for a length that cannot be.
 __device__ __forceinline__ int seq_keys(const DecodeParams &p, int b) {
   const int len = p.seq_lens[b];
-  if (len < 0 || len > (long long)p.max_pages * p.page_size) return -1;
+  if (!cached_length_ok(len, p.max_pages, p.page_size)) return -1;
   return max(len - (p.attend_current ? 0 : 1), 0);
 }
 __device__ __forceinline__ int units_of(const DecodeParams &p, int keys) {

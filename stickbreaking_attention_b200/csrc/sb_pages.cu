@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     if (back > 0) {
       const int len = p.seq_lens[seq];
       const long long pos = len - back;
-      if (len < 0 || len > (long long)p.max_pages * p.page_size) report(p.status, SB_DEV_BAD_SEQ_LEN, (int)seq);
+      if (!cached_length_ok(len, p.max_pages, p.page_size)) report(p.status, SB_DEV_BAD_SEQ_LEN, (int)seq);
       else if (pos >= 0) {
         const int index = (int)(pos / p.page_size), page = p.page_table[seq * p.table_stride + index];
         if ((unsigned)page >= (unsigned)p.num_pages) report(p.status, SB_DEV_BAD_PAGE, (int)seq);
@@ -194,9 +194,7 @@ __device__ __forceinline__ bool list_free(const PagesParams &p, int want, int *l
   return found >= want;
 }
 
-__device__ __forceinline__ bool length_ok(const PagesParams &p, long long len) {
-  return len >= 0 && len <= (long long)p.max_pages * p.page_size;
-}
+__device__ __forceinline__ bool length_ok(const PagesParams &p, long long len) { return cached_length_ok(len, p.max_pages, p.page_size); }
 __device__ __forceinline__ int pages_for(const PagesParams &p, int len) { return (int)(((long long)len + p.page_size - 1) / p.page_size); }
 
 // New tokens of sequence b.

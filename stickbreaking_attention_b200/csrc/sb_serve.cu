@@ -1,4 +1,5 @@
 // C entry points of the serving operators: argument checks, workspace layout, kernel selection.
+#include <algorithm>
 #include <cstring>
 
 #include "sb_decode.cuh"
@@ -75,8 +76,9 @@ int plan_decode(const SbDecodeParams *p, DecodePlan &pl) {
   pl.by_item = items < pl.chunks;
   pl.part_cols = tc ? decode_tc_cols(p->head_dim) : p->head_dim;
   if (items > (1LL << 30)) return fail(SB_ERR_ARGUMENT, "batch * kv_heads too large");
+  const long long longest = std::min<long long>((long long)p->max_pages * p->page_size, kMostTokens);
   pl.unit_shift = 4;                         // the units of all items have to be counted in 31 bits
-  while (items * (((long long)p->max_pages * p->page_size >> pl.unit_shift) + 1) > 0x7fffffffLL) ++pl.unit_shift;
+  while (items * ((longest >> pl.unit_shift) + 1) > 0x7fffffffLL) ++pl.unit_shift;
   const size_t slots = 2 * (size_t)pl.chunks * pl.rows_per_block, notes = (size_t)(pl.by_item ? items : pl.chunks) * sizeof(int4);
   pl.part_o = (notes + 255) / 256 * 256;
   pl.part_l = pl.part_o + (slots * pl.part_cols + 128) * sizeof(float);      // (padded: see launch_decode_join)

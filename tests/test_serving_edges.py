@@ -1,4 +1,4 @@
-"""The serving operators where they are easily wrong: bits of the weights, sticks that wear down slowly."""
+"""The serving operators where they are easily wrong: bits of the weights, sticks that wear down slowly, lengths of 31 bits."""
 import math
 
 import pytest
@@ -75,3 +75,76 @@ def test_decode_sticks_that_wear_down_slowly(cuda_device, dtype, bits):
                                 dev(lens).expand(seqs).contiguous(), inv_temp=1.0, attend_current=True)
     sb.check_status(cuda_device)
     R.check_decode(got, tuple(t.expand(seqs, *t.shape[1:]) for t in (o, rem, o_err, rem_err)))
+
+
+def ints(*x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ---- lengths of 31 bits ----------------------------------------------------------------------------------------------------
+
+LONGEST = 2 ** 31 - 16
+
+
+@gpu
+def test_extend_refuses_lengths_that_31_bits_do_not_hold(cuda_device):
+    """Rows with room for more than 2^31 tokens: a sequence grows up to 2^31 - 16 and no further, and a refused call changes nothing."""
+    import stickbreaking_attention_b200 as sb
+    page, columns = 65536, 32770
+    table = torch.full((3, columns), -1, dtype=torch.int32, device=cuda_device)
+    lens, refs = ints(10, 5, 0), torch.zeros(32768 + 4, dtype=torch.int32, device=cuda_device)
+    table[0, 0], table[1, 0], refs[0], refs[1] = 0, 1, 1, 1
+
+    def extend(counts, what=None):
+        before = [t.clone() for t in (table, lens, refs)]
+        sb.kv_extend(table, lens, refs, counts, page)
+        if what is None:
+            return sb.check_status(cuda_device)
+        with pytest.raises(sb._cabi.SbError, match=what):
+            sb.check_status(cuda_device)
+        for t, old in zip((table, lens, refs), before):
+            assert torch.equal(t, old)
+
+    for more in (2 ** 31 - 1, 2 ** 31 - 10, 2 ** 31 - 11, LONGEST - 9):
+        extend(ints(more, 2 * page, 1), "length")
+    extend(2 ** 31 - 1, "length")
+    extend(ints(LONGEST - 10, 3, 1))
+    assert lens.tolist() == [LONGEST, 8, 1] and int(refs.sum()) == 32768 + 2
+    assert table[0, :3].tolist() == [0, 2, 3] and table[0, 32767:].tolist() == [32768, -1, -1]
+    assert table[1, :2].tolist() == [1, -1] and table[2, :2].tolist() == [32769, -1]
+    extend(1, "length")
+    extend(ints(0, 1, 1))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("attend_current", [False, True])
+def test_decode_of_the_longest_sequences(cuda_device, dtype, attend_current):
+    """2^31 - 16 tokens, nearly all of them in one page that the row names 32766 times; longer ones are refused."""
+    import stickbreaking_attention_b200 as sb
+    gen = torch.Generator().manual_seed(61)
+    page, d, columns, new = 65536, 8, 32770, 2
+    k, v = (torch.randn(3, 1, page, d, generator=gen).to(dtype) for _ in range(2))
+    q = torch.randn(4, 2, new, d, generator=gen).to(dtype)
+    table = torch.zeros(4, columns, dtype=torch.int32)
+    table[:, 32766], table[:, 32767] = 1, 2
+    lens = torch.tensor([LONGEST, LONGEST + 1, 2 ** 31 - 1, 100], dtype=torch.int32)
+    dev = lambda t: t.to(cuda_device)
+    kp, vp, tab, lengths = dev(k), dev(v), dev(table), dev(lens)
+    newest = torch.randn(4, 1, 1, d, generator=gen).to(dtype)
+    with torch.no_grad():
+        for refused in (sb.kv_append, None):
+            if refused:
+                refused(dev(newest[:1]), dev(newest[:1]), kp, vp, tab[:1], lengths[:1])       # of the longest, the last slot but 15
+                sb.check_status(cuda_device)
+                refused(dev(newest[1:3]), dev(newest[1:3]), kp, vp, tab[1:3], lengths[1:3])
+            else:
+                o, rem = sb.sb_attn_decode(dev(q), kp, vp, tab, lengths, attend_current=attend_current)
+            with pytest.raises(sb._cabi.SbError, match="length"):
+                sb.check_status(cuda_device)
+    k[2, 0, page - 17], v[2, 0, page - 17] = newest[0, 0, 0], newest[0, 0, 0]
+    assert torch.equal(kp.cpu(), k) and torch.equal(vp.cpu(), v)
+    assert bool(o[1:3].isnan().all()) and bool(rem[1:3].isnan().all())
+    short = torch.tensor([[1, 2], [0, -1]], dtype=torch.int32)              # older keys have no weight left
+    want = R.decode(q[[0, 3]], k, v, short, torch.tensor([LONGEST - 32766 * page, 100], dtype=torch.int32), attend_current=attend_current)
+    R.check_decode((o[[0, 3]], rem[[0, 3]]), want)
