@@ -52,13 +52,15 @@ enum SbDeviceStatus {
                                 is filled with NaN (where the reference raises on the host,
                                 sb_varlen/__init__.py:72-74)                                   */
   SB_DEV_WAIT_TIMEOUT = 2,   /* a bounded on-chip wait gave up; status[1] = which barrier      */
-  SB_DEV_BAD_PAGE = 3,       /* a page table names a page that the pool does not have, for a token that its
-                                sequence holds; status[1] = sequence.  The page is not touched        */
+  SB_DEV_BAD_PAGE = 3,       /* a page table names a page that the pool does not have (for the keeping operators: or that is
+                                counted as free), for a token that its sequence holds; status[1] = sequence.  The page
+                                is not touched                                                        */
   SB_DEV_BAD_SEQ_LEN = 4,    /* a sequence's length, or the length it would grow to, is negative, beyond its row of
                                 the page table or beyond 2^31 - 16; status[1] = sequence              */
   SB_DEV_OUT_OF_PAGES = 5,   /* fewer free pages than the call needs; status[1] = how many it needs.  Nothing was changed */
-  SB_DEV_BAD_SEQUENCE = 6    /* an index of sb_kv_fork or sb_kv_free is no sequence, or one that the call cannot take;
+  SB_DEV_BAD_SEQUENCE = 6,   /* an index of sb_kv_fork or sb_kv_free is no sequence, or one that the call cannot take;
                                 status[1] = the index.  Nothing was changed                           */
+  SB_DEV_BAD_COUNT = 7       /* sb_kv_compact: a page's count is negative; status[1] = the page.  Nothing was changed */
 };
 
 enum SbKernelPath {
@@ -343,7 +345,8 @@ SB_EXPORT int sb_kv_fork(const SbPagesParams *p, void *stream);
 /* The listed sequences give their pages back and are empty; one that is empty, or listed twice, is no error. */
 SB_EXPORT int sb_kv_free(const SbPagesParams *p, void *stream);
 /* Moves the pages in use to the front of the pool: with N of them, the r-th one at or behind N goes to the r-th free one before
- * N, all layers, and the tables follow.  Pages that have become free keep what they held. */
+ * N, all layers, and the tables follow.  Pages that have become free keep what they held.  A table entry that names no page, or a
+ * free one, is left as it is (SB_DEV_BAD_PAGE, where any page moves). */
 SB_EXPORT int sb_kv_compact(const SbPagesParams *p, void *stream);
 
 /* Which kernels sb_fwd / sb_bwd run for these parameters (an SbKernelPath), or -1 if invalid. */

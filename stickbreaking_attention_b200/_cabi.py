@@ -24,11 +24,12 @@ SB_DEV_MESSAGES = {
     1: "cu_seqlens is invalid (not non-decreasing, beyond the token count, longer than max_seqlens, "
        "or without its leading zero); offending sequence index: {0}",
     2: "a bounded on-chip wait timed out in barrier {0}",
-    3: "a page table names a page that the cache does not have; sequence: {0}",
+    3: "a page table names a page that the cache does not have, or that is counted as free; sequence: {0}",
     4: "a sequence's length, or the length it would grow to, is negative, beyond its row of the page table or beyond 2^31 - 16; "
        "sequence: {0}",
     5: "the cache has too few free pages: {0} needed; nothing was changed",
     6: "listed sequence {0} is none, or one that the call cannot take; nothing was changed",
+    7: "the count of sequences that hold a page is negative; page: {0}; nothing was changed",
 }
 EXPORTS = ("sb_workspace_bytes", "sb_fwd", "sb_bwd", "sb_fwd_static_scratch", "sb_set_backward_scratch_budget",
            "sb_kernel_path", "sb_last_launch_count", "sb_last_error", "sb_abi_version", "sb_attn_decode_workspace_bytes",

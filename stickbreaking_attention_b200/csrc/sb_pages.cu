@@ -313,7 +313,7 @@ __device__ __forceinline__ void copy_page(const PagesParams &p, const CacheRef &
   }
 }
 
-// header of `work`: [0] whether there is something to carry out, [1] pages to move, [2] live pages
+// header of `work`: [0] fork: whether there is something to carry out, [1] compact: pages to move
 // fork: behind the lists, for each pair the source's length and the page that its copied rows get (or -1)
 __device__ __forceinline__ int *fork_plan(const PagesParams &p) { return p.work + kPagesHeader + 2 * p.num_pages + p.max_seqs; }
 
@@ -406,13 +406,25 @@ __global__ void __launch_bounds__(kCopyThreads) fork_kernel(const __grid_constan
 __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid_constant__ PagesParams p) {
   __shared__ int shared[33];
   enter_kernel<true>();
-  int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;    // (hole, page) pairs, no more than half the pages; new place of each
+  int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;    // (hole, page) pairs, no more than half the pages; new place of each, -1 of a free one
   int live = 0, mine = 0;
+  bool bad = false;
   for (int base = 0; base < p.num_pages; base += (int)blockDim.x * kPer) {
+    const int first = base + threadIdx.x * kPer;
     int x[kPer];
-    read_refs(p, base + threadIdx.x * kPer, x);
+    read_refs(p, first, x);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) mine += x[i] > 0;
+    for (int i = 0; i < kPer; ++i) {
+      mine += x[i] > 0;
+      if (x[i] < 0 && first + i < p.num_pages) {      // a page neither free nor in use: there would be fewer holes than pages to move
+        bad = true;
+        report(p.status, SB_DEV_BAD_COUNT, first + i);
+      }
+    }
+  }
+  if (__syncthreads_or(bad)) {
+    if (threadIdx.x == 0) p.work[1] = 0;
+    return;
   }
   block_scan(mine, shared, live);
   int holes = 0, moved = 0;
@@ -430,6 +442,7 @@ __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid
     for (int i = 0; i < kPer; ++i) {
       if (first + i < live && x[i] == 0) pairs[2 * rank_h++] = first + i;
       if (first + i >= live && x[i] > 0) pairs[2 * rank_m++ + 1] = first + i;
+      if (first + i < p.num_pages) place[first + i] = x[i] > 0 ? first + i : -1;
     }
     holes += all_h;
     moved += all_m;
@@ -441,17 +454,14 @@ __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid
     p.refs[to] = p.refs[from];
     p.refs[from] = 0;
   }
-  if (threadIdx.x == 0) {
-    p.work[1] = moved;
-    p.work[2] = live;
-  }
+  if (threadIdx.x == 0) p.work[1] = moved;
 }
 
 // Blocks below copy_blocks copy the moved pages, a share of a (page, layer, keys or values) at a time; the others rewrite the tables.
 template <typename V>
 __global__ void __launch_bounds__(kCopyThreads) compact_kernel(const __grid_constant__ PagesParams p, int copy_blocks) {
   enter_kernel<true>();
-  const int moved = p.work[1], live = p.work[2];
+  const int moved = p.work[1];
   const int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;
   if ((int)blockIdx.x < copy_blocks) {
     const int per_pair = p.layers * 2 * p.parts;
@@ -467,9 +477,9 @@ __global__ void __launch_bounds__(kCopyThreads) compact_kernel(const __grid_cons
     const int len = p.seq_lens[b], pages = length_ok(p, len) ? pages_for(p, len) : 0;
     int *row = p.page_table + b * p.table_stride;
     for (int i = threadIdx.x; i < pages; i += kCopyThreads) {
-      const int page = row[i];
-      if ((unsigned)page >= (unsigned)p.num_pages) report(p.status, SB_DEV_BAD_PAGE, b);
-      else if (page >= live) row[i] = place[page];
+      const int page = row[i], to = (unsigned)page < (unsigned)p.num_pages ? place[page] : -1;
+      if (to < 0) report(p.status, SB_DEV_BAD_PAGE, b);      // no page, or a free one: stays as it is
+      else if (to != page) row[i] = to;
     }
   }
 }

@@ -1,4 +1,4 @@
-"""The serving operators where they are easily wrong: bits of the weights, sticks that wear down slowly, lengths of 31 bits."""
+"""The serving operators where they are easily wrong: bits of the weights, sticks that wear down slowly, lengths of 31 bits, books that cannot be."""
 import math
 
 import pytest
@@ -148,3 +148,74 @@ def test_decode_of_the_longest_sequences(cuda_device, dtype, attend_current):
     short = torch.tensor([[1, 2], [0, -1]], dtype=torch.int32)              # older keys have no weight left
     want = R.decode(q[[0, 3]], k, v, short, torch.tensor([LONGEST - 32766 * page, 100], dtype=torch.int32), attend_current=attend_current)
     R.check_decode((o[[0, 3]], rem[[0, 3]]), want)
+
+
+# ---- books and lengths that cannot be --------------------------------------------------------------------------------------
+
+def small_cache(sb, device, lens=(6, 4, 0, 0)):
+    """Four sequences, six pages of four tokens; pools with a number for every element."""
+    cache = sb.PagedKVCache(2, 6, 1, 4, 8, 4, 16, dtype=FP32, device=device)
+    cache.extend(ints(*lens))
+    sb.check_status(device)
+    for t, at in ((cache.k, 0), (cache.v, 10 ** 6)):
+        t.copy_(torch.arange(at, at + t.numel(), dtype=FP32, device=device).view(t.shape))
+    return cache
+
+
+def everything(cache):
+    return [t.clone() for t in (cache.page_table, cache.seq_lens, cache.page_refs, cache.k, cache.v)]
+
+
+def refused(sb, device, cache, call, what):
+    """`call` changes nothing and leaves a status."""
+    before = everything(cache)
+    call()
+    with pytest.raises(sb._cabi.SbError, match=what):
+        sb.check_status(device)
+    for name, t, old in zip(("page_table", "seq_lens", "page_refs", "k", "v"), everything(cache), before):
+        assert torch.equal(t, old), name
+
+
+@gpu
+@pytest.mark.parametrize("count", [-1, -2 ** 31])
+@pytest.mark.parametrize("page", [0, 2, 5])
+def test_compact_refuses_negative_counts(cuda_device, page, count):
+    """A page that is neither free nor in use: where there are such, fewer pages in front are free than pages behind are in use."""
+    import stickbreaking_attention_b200 as sb
+    cache = small_cache(sb, cuda_device)
+    cache.page_refs[page] = count
+    refused(sb, cuda_device, cache, cache.compact, "negative")
+    cache.page_refs.fill_(-1)
+    refused(sb, cuda_device, cache, cache.compact, "negative")
+
+
+@gpu
+def test_compact_of_large_pools_refuses_negative_counts(cuda_device):
+    """The last of 40000 pages (the counts are read in more than one turn, 16 at a time, the last ones singly)."""
+    import stickbreaking_attention_b200 as sb
+    cache = sb.PagedKVCache(1, 40003, 1, 1, 8, 2, 64, dtype=BF16, device=cuda_device)
+    cache.k.zero_(), cache.v.zero_()
+    cache.extend(ints(20, 30))
+    cache.free(ints(0))
+    cache.page_refs[-1] = -1
+    refused(sb, cuda_device, cache, cache.compact, "negative")
+    cache.page_refs[-1] = 0
+    cache.compact()
+    sb.check_status(cuda_device)
+    assert cache.page_table[1, :30].tolist() == [*range(20, 30), *range(20)]
+    assert cache.page_refs[:32].tolist() == [1] * 30 + [0] * 2
+
+
+@gpu
+@pytest.mark.parametrize("page", [-1, 6, 2 ** 31 - 1, 5, 1])          # 5, 1: pages of the cache, but free ones
+def test_compact_leaves_entries_without_a_place_alone(cuda_device, page):
+    import stickbreaking_attention_b200 as sb
+    cache = small_cache(sb, cuda_device)
+    cache.free(ints(0))
+    cache.extend(ints(0, 4, 0, 0))                  # sequence 1 has pages 2 and 0; 2 moves to 1
+    cache.page_table[1, 1] = page
+    cache.compact()
+    with pytest.raises(sb._cabi.SbError, match="page"):
+        sb.check_status(cuda_device)
+    assert cache.page_table[1].tolist() == [1, page, -1, -1] and cache.page_refs.tolist() == [1, 1, 0, 0, 0, 0]
+    assert torch.equal(cache.k[:, 1].cpu(), torch.arange(384, dtype=FP32).view(2, 6, 1, 4, 8)[:, 2])
