@@ -409,6 +409,11 @@ __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid
   int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;    // (hole, page) pairs, no more than half the pages; new place of each, -1 of a free one
   int live = 0, mine = 0;
   bool bad = false;
+  for (int b = threadIdx.x; b < p.max_seqs; b += blockDim.x)
+    if (!length_ok(p, p.seq_lens[b])) {      // which entries of its row are to follow their pages, nothing says
+      bad = true;
+      report(p.status, SB_DEV_BAD_SEQ_LEN, b);
+    }
   for (int base = 0; base < p.num_pages; base += (int)blockDim.x * kPer) {
     const int first = base + threadIdx.x * kPer;
     int x[kPer];
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(kCopyThreads) compact_kernel(const __grid_cons
   }
   if (moved == 0) return;
   for (int b = blockIdx.x - copy_blocks; b < p.max_seqs; b += gridDim.x - copy_blocks) {
-    const int len = p.seq_lens[b], pages = length_ok(p, len) ? pages_for(p, len) : 0;
+    const int pages = pages_for(p, p.seq_lens[b]);
     int *row = p.page_table + b * p.table_stride;
     for (int i = threadIdx.x; i < pages; i += kCopyThreads) {
       const int page = row[i], to = (unsigned)page < (unsigned)p.num_pages ? place[page] : -1;

@@ -219,3 +219,17 @@ def test_compact_leaves_entries_without_a_place_alone(cuda_device, page):
         sb.check_status(cuda_device)
     assert cache.page_table[1].tolist() == [1, page, -1, -1] and cache.page_refs.tolist() == [1, 1, 0, 0, 0, 0]
     assert torch.equal(cache.k[:, 1].cpu(), torch.arange(384, dtype=FP32).view(2, 6, 1, 4, 8)[:, 2])
+
+
+@gpu
+@pytest.mark.parametrize("length", [-1, 17, 2 ** 31 - 1, -2 ** 31])
+def test_compact_refuses_lengths_that_cannot_be(cuda_device, length):
+    import stickbreaking_attention_b200 as sb
+    cache = small_cache(sb, cuda_device)
+    cache.free(ints(0))                             # pages 0 and 1 are free: compact has something to do
+    cache.seq_lens[3] = length
+    refused(sb, cuda_device, cache, cache.compact, "length")
+    cache.seq_lens[3] = 0
+    cache.compact()
+    sb.check_status(cuda_device)
+    assert cache.page_table[1].tolist() == [0, -1, -1, -1] and cache.page_refs.tolist() == [1, 0, 0, 0, 0, 0]
