@@ -254,14 +254,16 @@ constexpr int kFreeThreads = 128;
 __global__ void __launch_bounds__(kFreeThreads) free_kernel(const __grid_constant__ PagesParams p) {
   enter_kernel<true>();
   bool bad = false;
-  for (int i = threadIdx.x; i < p.n; i += kFreeThreads)
-    if ((unsigned)p.a[i] >= (unsigned)p.max_seqs) {
-      bad = true;
-      if (blockIdx.x == 0) report(p.status, SB_DEV_BAD_SEQUENCE, p.a[i]);
-    }
+  // Every block looks at the whole list.  Nothing that it refuses changes meanwhile: a length that another block has made 0
+  // was one that can be.
+  for (int i = threadIdx.x; i < p.n; i += kFreeThreads) {
+    const int s = p.a[i], code = (unsigned)s >= (unsigned)p.max_seqs ? SB_DEV_BAD_SEQUENCE : length_ok(p, p.seq_lens[s]) ? 0 : SB_DEV_BAD_SEQ_LEN;
+    if (code == 0) continue;
+    bad = true;
+    if (blockIdx.x == 0) report(p.status, code, s);
+  }
   if (__syncthreads_or(bad)) return;
-  const int b = p.a[blockIdx.x], len = *reinterpret_cast<volatile int *>(p.seq_lens + b);
-  const int pages = length_ok(p, len) ? pages_for(p, len) : 0;
+  const int b = p.a[blockIdx.x], pages = pages_for(p, *reinterpret_cast<volatile int *>(p.seq_lens + b));
   for (int i = threadIdx.x; i < pages; i += kFreeThreads) {
     const int page = atomicExch(p.page_table + b * p.table_stride + i, -1);
     if ((unsigned)page < (unsigned)p.num_pages) atomicSub(p.refs + page, 1);

@@ -233,3 +233,20 @@ def test_compact_refuses_lengths_that_cannot_be(cuda_device, length):
     cache.compact()
     sb.check_status(cuda_device)
     assert cache.page_table[1].tolist() == [0, -1, -1, -1] and cache.page_refs.tolist() == [1, 0, 0, 0, 0, 0]
+
+
+@gpu
+@pytest.mark.parametrize("length", [-1, 17, 2 ** 31 - 1, -2 ** 31])
+def test_free_refuses_lengths_that_cannot_be(cuda_device, length):
+    import stickbreaking_attention_b200 as sb
+    cache = small_cache(sb, cuda_device)
+    cache.seq_lens[3] = length
+    for seqs in (ints(3), ints(0, 3), ints(3, 1, 1), ints(*[1] * 300, 3)):
+        refused(sb, cuda_device, cache, lambda: cache.free(seqs), "length")
+    cache.free(ints(0, 1))                          # the others can be freed
+    sb.check_status(cuda_device)
+    assert cache.page_refs.tolist() == [0] * 6 and cache.seq_lens.tolist() == [0, 0, 0, length]
+    for call in (lambda: cache.extend(ints(1, 1, 0, 0)), lambda: cache.extend(1)):
+        refused(sb, cuda_device, cache, call, "length")
+    for call in (lambda: cache.fork(ints(3), ints(2)), lambda: cache.fork(ints(0), ints(3))):
+        refused(sb, cuda_device, cache, call, "listed")
