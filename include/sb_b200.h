@@ -342,7 +342,8 @@ SB_EXPORT int sb_kv_extend(const SbPagesParams *p, void *stream);
 /* second[i], an empty sequence, becomes a copy of first[i]: full pages are shared, the tokens of a last page that is not full
  * are copied to a page of its own, all layers.  A sequence may be forked several times in a call but not be a fork in it. */
 SB_EXPORT int sb_kv_fork(const SbPagesParams *p, void *stream);
-/* The listed sequences give their pages back and are empty; one that is empty, or listed twice, is no error. */
+/* The listed sequences give their pages back and are empty; one that is empty, or listed twice, is no error.  A table entry
+ * that names no page, or a free one, goes out of its row and counts nothing down (SB_DEV_BAD_PAGE). */
 SB_EXPORT int sb_kv_free(const SbPagesParams *p, void *stream);
 /* Moves the pages in use to the front of the pool: with N of them, the r-th one at or behind N goes to the r-th free one before
  * N, all layers, and the tables follow.  Pages that have become free keep what they held.  A table entry that names no page, or a

@@ -249,24 +249,32 @@ __global__ void __launch_bounds__(kBookThreads) extend_kernel(const __grid_const
   }
 }
 
-// A block per entry.  An entry that is listed twice is freed once: whoever takes a page out of the table counts it down.
+// A block per entry.  A sequence that is listed more than once is the first entry's.  No count goes below 0: a page that would is
+// taken out of the row, and reported.
 constexpr int kFreeThreads = 128;
 __global__ void __launch_bounds__(kFreeThreads) free_kernel(const __grid_constant__ PagesParams p) {
   enter_kernel<true>();
-  bool bad = false;
   // Every block looks at the whole list.  Nothing that it refuses changes meanwhile: a length that another block has made 0
   // was one that can be.
+  const int b = p.a[blockIdx.x];
+  bool leave = false;
   for (int i = threadIdx.x; i < p.n; i += kFreeThreads) {
     const int s = p.a[i], code = (unsigned)s >= (unsigned)p.max_seqs ? SB_DEV_BAD_SEQUENCE : length_ok(p, p.seq_lens[s]) ? 0 : SB_DEV_BAD_SEQ_LEN;
-    if (code == 0) continue;
-    bad = true;
-    if (blockIdx.x == 0) report(p.status, code, s);
+    leave |= code != 0 || (s == b && i < (int)blockIdx.x);
+    if (code != 0 && blockIdx.x == 0) report(p.status, code, s);
   }
-  if (__syncthreads_or(bad)) return;
-  const int b = p.a[blockIdx.x], pages = pages_for(p, *reinterpret_cast<volatile int *>(p.seq_lens + b));
+  if (__syncthreads_or(leave)) return;
+  const int pages = pages_for(p, p.seq_lens[b]);
   for (int i = threadIdx.x; i < pages; i += kFreeThreads) {
-    const int page = atomicExch(p.page_table + b * p.table_stride + i, -1);
-    if ((unsigned)page < (unsigned)p.num_pages) atomicSub(p.refs + page, 1);
+    int *const entry = p.page_table + b * p.table_stride + i;
+    const int page = *entry;
+    *entry = -1;
+    bool held = (unsigned)page < (unsigned)p.num_pages;
+    if (held && atomicSub(p.refs + page, 1) <= 0) {
+      atomicAdd(p.refs + page, 1);
+      held = false;
+    }
+    if (!held) report(p.status, SB_DEV_BAD_PAGE, b);
   }
   __syncthreads();
   if (threadIdx.x == 0) p.seq_lens[b] = 0;

@@ -250,3 +250,31 @@ def test_free_refuses_lengths_that_cannot_be(cuda_device, length):
         refused(sb, cuda_device, cache, call, "length")
     for call in (lambda: cache.fork(ints(3), ints(2)), lambda: cache.fork(ints(0), ints(3))):
         refused(sb, cuda_device, cache, call, "listed")
+
+
+@gpu
+@pytest.mark.parametrize("page", [-1, 6, 2 ** 31 - 1, -2 ** 31, 5, 2])      # 5: a free page; 2: sequence 1's, counted once
+@pytest.mark.parametrize("seqs", [[0, 1], [1, 0, 0], [0, 1] * 200])
+def test_free_counts_no_page_below_0(cuda_device, page, seqs):
+    """Rows that name a page which nobody counts for them: the sequences are empty afterwards, and no count is negative."""
+    import stickbreaking_attention_b200 as sb
+    cache = small_cache(sb, cuda_device)
+    cache.page_table[0, 0] = page                   # page 0 stays counted: nothing names it any more
+    cache.free(ints(*seqs))
+    with pytest.raises(sb._cabi.SbError, match="page"):
+        sb.check_status(cuda_device)
+    assert cache.page_refs.tolist() == [1, 0, 0, 0, 0, 0]
+    assert cache.seq_lens.tolist() == [0] * 4 and bool((cache.page_table == -1).all())
+
+
+@gpu
+def test_free_of_many_rows_that_name_the_same_page(cuda_device):
+    """600 sequences hold a page that 500 of them are counted for."""
+    import stickbreaking_attention_b200 as sb
+    table = torch.zeros(600, 3, dtype=torch.int32, device=cuda_device)
+    lens = torch.full((600,), 3, dtype=torch.int32, device=cuda_device)
+    refs = ints(500, 7)
+    sb.kv_free(table, lens, refs, torch.arange(600, dtype=torch.int32, device=cuda_device), 4)
+    with pytest.raises(sb._cabi.SbError, match="page"):
+        sb.check_status(cuda_device)
+    assert refs.tolist() == [0, 7] and not bool(lens.any()) and bool((table[:, 0] == -1).all()) and not bool(table[:, 1:].any())
