@@ -52,7 +52,7 @@ enum SbDeviceStatus {
                                 is filled with NaN (where the reference raises on the host,
                                 sb_varlen/__init__.py:72-74)                                   */
   SB_DEV_WAIT_TIMEOUT = 2,   /* a bounded on-chip wait gave up; status[1] = which barrier      */
-  SB_DEV_BAD_PAGE = 3,       /* a page table names a page that the pool does not have (for the keeping operators: or that is
+  SB_DEV_BAD_PAGE = 3,       /* a page table names a page that the pool does not have (sb_kv_free, sb_kv_compact: or that is
                                 counted as free), for a token that its sequence holds; status[1] = sequence.  The page
                                 is not touched                                                        */
   SB_DEV_BAD_SEQ_LEN = 4,    /* a sequence's length, or the length it would grow to, is negative, beyond its row of
@@ -340,7 +340,8 @@ SB_EXPORT size_t sb_kv_pages_workspace_bytes(const SbPagesParams *p);
 /* Room for new tokens: lengths grow by `first` (or `count`), and rows get the pages they lack. */
 SB_EXPORT int sb_kv_extend(const SbPagesParams *p, void *stream);
 /* second[i], an empty sequence, becomes a copy of first[i]: full pages are shared, the tokens of a last page that is not full
- * are copied to a page of its own, all layers.  A sequence may be forked several times in a call but not be a fork in it. */
+ * are copied to a page of its own, all layers.  A sequence may be forked several times in a call but not be a fork in it.
+ * Where a source's row names a page that the pool does not have, nothing is changed (SB_DEV_BAD_PAGE). */
 SB_EXPORT int sb_kv_fork(const SbPagesParams *p, void *stream);
 /* The listed sequences give their pages back and are empty; one that is empty, or listed twice, is no error.  A table entry
  * that names no page, or a free one, goes out of its row and counts nothing down (SB_DEV_BAD_PAGE). */

@@ -278,3 +278,35 @@ def test_free_of_many_rows_that_name_the_same_page(cuda_device):
     with pytest.raises(sb._cabi.SbError, match="page"):
         sb.check_status(cuda_device)
     assert refs.tolist() == [0, 7] and not bool(lens.any()) and bool((table[:, 0] == -1).all()) and not bool(table[:, 1:].any())
+
+
+@gpu
+@pytest.mark.parametrize("entry", [0, 1])          # a page that would be shared; the last one, partly filled
+@pytest.mark.parametrize("page", [-1, 6, 2 ** 31 - 1, -2 ** 31])
+def test_fork_of_a_sequence_whose_row_names_no_page(cuda_device, entry, page):
+    import stickbreaking_attention_b200 as sb
+    cache = small_cache(sb, cuda_device)
+    cache.page_table[0, entry] = page
+    refused(sb, cuda_device, cache, lambda: cache.fork(ints(1, 0), ints(2, 3)), "page")
+    cache.fork(ints(1), ints(2))                    # the other one can be forked
+    sb.check_status(cuda_device)
+    assert cache.seq_lens.tolist() == [6, 4, 4, 0] and cache.page_refs.tolist() == [1, 1, 2, 0, 0, 0]
+
+
+@gpu
+def test_fork_of_many_long_rows_looks_at_every_entry(cuda_device):
+    """40 forks of rows of 70 pages, one bad entry somewhere."""
+    import stickbreaking_attention_b200 as sb
+    cache = sb.PagedKVCache(1, 6000, 1, 4, 8, 80, 400, dtype=FP32, device=cuda_device)
+    cache.k.zero_(), cache.v.zero_()
+    cache.extend(ints(*([278] * 40 + [0] * 40)))
+    src, dst = ints(*range(39, -1, -1)), ints(*range(40, 80))
+    for row, entry in ((0, 0), (39, 69), (17, 31), (17, 32), (8, 68)):
+        page = int(cache.page_table[row, entry])
+        cache.page_table[row, entry] = 6000
+        refused(sb, cuda_device, cache, lambda: cache.fork(src, dst), "page")
+        cache.page_table[row, entry] = page
+    cache.page_table[5, 70] = 6000                  # behind the row's end: not looked at
+    cache.fork(src, dst)
+    sb.check_status(cuda_device)
+    assert cache.seq_lens.tolist() == [278] * 80 and int(cache.page_refs.sum()) == 80 * 70
