@@ -403,6 +403,13 @@ void count_launches(const char *what, int rc) {
 }
 void *stream_of(const Tensor &t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
+// The output for queries q, by a rule that an operator without data can follow too (ops.py): what torch.empty_like(q) gives, where
+// that has unit stride in head_dim, else contiguous; whether or not q itself has to be copied for the kernel.
+Tensor rows_like(const Tensor &q) {
+  const Tensor o = empty_as(q);
+  return o.size(3) <= 1 || o.stride(3) == 1 ? o : empty_cuda(q.sizes(), q.scalar_type(), q);
+}
+
 std::tuple<Tensor, Tensor> decode(const Tensor &q_in, const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &lens,
                                   double scale, bool attend_current, int64_t flags) {
   refuse_grad("sb_attn_decode", {&q_in, &k, &v});
@@ -419,7 +426,7 @@ std::tuple<Tensor, Tensor> decode(const Tensor &q_in, const Tensor &k, const Ten
   if (pairs && q_in.element_size() == 2 && q_in.size(3) % 8 == 0)
     pairs = reinterpret_cast<uintptr_t>(q_in.data_ptr()) % 4 == 0 && stride_of(q_in, 0) % 2 == 0 && stride_of(q_in, 1) % 2 == 0 && stride_of(q_in, 2) % 2 == 0;
   const Tensor q = pairs ? q_in : q_in.contiguous();
-  const Tensor o = empty_as(q), rem = empty_cuda(q.sizes().slice(0, 3), q.scalar_type(), q);
+  const Tensor o = rows_like(q_in), rem = empty_cuda(q.sizes().slice(0, 3), q.scalar_type(), q);
   SbDecodeParams p;
   memset(&p, 0, sizeof(p));
   p.struct_bytes = (int32_t)sizeof(p);

@@ -470,7 +470,10 @@ def decode_op(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
 
 @decode_op.register_fake
 def _(q, k_pages, v_pages, page_table, seq_lens, logit_scale, attend_current):
-    return torch.empty_like(q), q.new_empty(q.shape[:3])
+    o = torch.empty_like(q)
+    if q.shape[3] > 1 and o.stride(3) != 1:      # the layout that the binding gives it
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    return o, q.new_empty(q.shape[:3])
 
 
 @torch.library.custom_op(f"{NAMESPACE}::kv_append", mutates_args={"k_pages", "v_pages"}, device_types="cuda")

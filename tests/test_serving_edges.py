@@ -1,8 +1,9 @@
-"""The serving operators where they are easily wrong: bits of the weights, sticks that wear down slowly, lengths of 31 bits, books that cannot be."""
+"""The serving operators where they are easily wrong: the bits of weights and sticks, lengths, books, layouts of queries."""
 import math
 
 import pytest
 import torch
+import torch.compiler.config
 
 import serving_reference as R
 
@@ -310,3 +311,87 @@ def test_fork_of_many_long_rows_looks_at_every_entry(cuda_device):
     cache.fork(src, dst)
     sb.check_status(cuda_device)
     assert cache.seq_lens.tolist() == [278] * 80 and int(cache.page_refs.sum()) == 80 * 70
+
+
+# ---- layouts ---------------------------------------------------------------------------------------------------------------
+
+def layouts(device, dtype=BF16):
+    """Queries (2, 4, 3, 64) in many layouts, and whether an output in that layout has unit stride in its last axis."""
+    def numbers(*shape):
+        return torch.arange(math.prod(shape), dtype=FP32, device=device).remainder(97).sub(48).div(32).to(dtype).view(shape)
+    base = numbers(2, 4, 3, 64)
+    yield "contiguous", base
+    yield "tokens before heads", numbers(2, 3, 4, 64).transpose(1, 2)
+    yield "tokens behind columns", numbers(2, 4, 64, 3).transpose(2, 3)
+    yield "columns first", numbers(64, 2, 3, 4).permute(1, 3, 2, 0)
+    yield "rows at odd elements", numbers(2 * 4 * 3 * 64 + 1)[1:].view(2, 4, 3, 64)
+    yield "rows at odd elements, tokens before heads", numbers(2 * 3 * 4 * 64 + 1)[1:].view(2, 3, 4, 64).transpose(1, 2)
+    yield "rows of odd length", numbers(2, 4, 3, 65)[..., :64]
+    yield "a third of a packed projection", numbers(2, 3, 3, 4, 64)[:, :, 1].transpose(1, 2)
+    yield "one batch element", numbers(1, 4, 3, 64).expand(2, -1, -1, -1)
+    yield "one head", numbers(2, 1, 3, 64).expand(-1, 4, -1, -1)
+    yield "one column", numbers(2, 4, 3, 1).expand(-1, -1, -1, 64)
+    yield "one column, tokens before heads", numbers(2, 3, 4, 1).transpose(1, 2).expand(-1, -1, -1, 64)
+    yield "windows", numbers(2, 4, 66).unfold(2, 64, 1)
+    yield "every other column", numbers(2, 4, 3, 128)[..., ::2]
+
+
+def announced(q, *args):
+    """Strides of (o, rem) as the operator without data gives them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from stickbreaking_attention_b200 import ops
+    with FakeTensorMode() as mode:
+        def fake(t):
+            size = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+            return torch.empty(t.storage_offset() + size, dtype=t.dtype, device="cuda").as_strided(t.shape, t.stride(), t.storage_offset())
+        return tuple(t.stride() for t in ops.decode_op(fake(q), *(fake(t) for t in args), 0.125, False))
+
+
+def cache_of(gen, dtype=BF16):
+    return R.make_cache(gen, [40, 9], 2, 16, 64, dtype)
+
+
+def test_decode_announces_rows_without_gaps():
+    """Strides that compiled code goes by: those of the queries where rows are runs of elements, contiguous else."""
+    cache = cache_of(torch.Generator().manual_seed(70))
+    got = {name: announced(q, *cache) for name, q in layouts("cpu")}
+    assert all(o[3] == 1 and rem == (12, 3, 1) for o, rem in got.values())
+    contiguous, turned = (768, 192, 64, 1), (768, 64, 256, 1)
+    for name in ("contiguous", "tokens behind columns", "columns first", "rows at odd elements", "rows of odd length", "one column", "windows"):
+        assert got[name][0] == contiguous, name
+    for name in ("tokens before heads", "rows at odd elements, tokens before heads", "a third of a packed projection"):
+        assert got[name][0] == turned, name
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_decode_gives_the_layout_that_it_announces(cuda_device, dtype):
+    import stickbreaking_attention_b200 as sb
+    cache = cache_of(torch.Generator().manual_seed(71), dtype)
+    on_gpu = [t.to(cuda_device) for t in cache]
+    for name, q in layouts(cuda_device, dtype):
+        with torch.no_grad():
+            o, rem = sb.sb_attn_decode(q, *on_gpu)
+        sb.check_status(cuda_device)
+        assert (o.stride(), rem.stride()) == announced(q, *cache), name
+        R.check_decode((o, rem), R.decode(q.contiguous(), *cache))
+
+
+@gpu
+def test_decode_compiled_with_queries_in_many_layouts(cuda_device):
+    """Compiled code and eager code agree on what o holds where."""
+    import stickbreaking_attention_b200 as sb
+    cache = [t.to(cuda_device) for t in cache_of(torch.Generator().manual_seed(72))]
+
+    def step(q):
+        o, rem = sb.sb_attn_decode(q, *cache)
+        return o.transpose(1, 2).reshape(6, -1) * 2, rem + 1
+
+    with torch.no_grad():
+        for name, q in layouts(cuda_device):
+            torch.compiler.reset()
+            # (code kept on the disk may be for another build's layouts)
+            with torch.compiler.config.patch(force_disable_caches=True):
+                eager, compiled = step(q), torch.compile(step, fullgraph=True)(q)
+            assert torch.equal(eager[0], compiled[0]) and torch.equal(eager[1], compiled[1]), name
+    sb.check_status(cuda_device)
