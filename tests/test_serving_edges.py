@@ -1,4 +1,6 @@
-"""The serving operators where they are easily wrong: the bits of weights and sticks, lengths, books, layouts of queries."""
+"""The serving operators where they are easily wrong: the bits of weights and sticks, lengths, books, layouts of queries, which
+kernel runs."""
+import ctypes
 import math
 
 import pytest
@@ -394,4 +396,53 @@ def test_decode_compiled_with_queries_in_many_layouts(cuda_device):
             with torch.compiler.config.patch(force_disable_caches=True):
                 eager, compiled = step(q), torch.compile(step, fullgraph=True)(q)
             assert torch.equal(eager[0], compiled[0]) and torch.equal(eager[1], compiled[1]), name
+    sb.check_status(cuda_device)
+
+
+# ---- which kernel ----------------------------------------------------------------------------------------------------------
+
+@gpu
+def test_decode_takes_the_tensor_cores_where_rows_are_whole_chunks(cuda_device):
+    """What sb_attn_decode_path answers, and which kernels are launched."""
+    import stickbreaking_attention_b200 as sb
+    from stickbreaking_attention_b200 import _cabi
+    lib = _cabi.load()
+    simt, tensor_cores = 0, 1
+
+    def path(dtype, d, flags=0, offset=0, odd_query=0, stride=None):
+        at = 1 << 20
+        p = _cabi.SbDecodeParams(struct_bytes=ctypes.sizeof(_cabi.SbDecodeParams), dtype=dtype, batch=2, heads=4, kv_heads=2, new_tokens=1,
+                                 head_dim=d, page_size=16, num_pages=8, max_pages=4, logit_scale=0.125, flags=flags)
+        p.q = _cabi.SbTensor(at + odd_query, 4 * d, d, d)
+        p.k = p.v = _cabi.SbCache(at + offset, 0, 32 * d, 16 * d, stride or d)
+        return lib.sb_attn_decode_path(p)
+
+    with torch.cuda.device(cuda_device):
+        for dtype in (1, 2):
+            assert [path(dtype, d) for d in (8, 64, 72, 128, 256)] == [tensor_cores] * 5
+            assert [path(dtype, d) for d in (1, 50, 100)] == [simt] * 3
+            assert path(dtype, 64, offset=8) == path(dtype, 64, stride=68) == path(dtype, 64, odd_query=2) == simt
+            assert path(dtype, 64, flags=_cabi.SB_FLAG_FORCE_SIMT) == simt
+        assert path(0, 64) == simt and path(1, 257) == path(9, 64) == -1
+
+    gen = torch.Generator().manual_seed(73)
+    cache = [t.to(cuda_device) for t in cache_of(gen)]
+    q = torch.randn(2, 4, 1, 64, generator=gen).to(BF16).to(cuda_device)
+    wide = torch.full((2, *cache[0].shape[:-1], 68), float("nan"), dtype=BF16, device=cuda_device)
+    wide[0, ..., :64], wide[1, ..., :64] = cache[0], cache[1]
+
+    def ran(call):
+        with torch.no_grad(), torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as profile:
+            call()
+            torch.cuda.synchronize()
+        names = [event.name for event in profile.events() if "decode_" in event.name]
+        return {kernel for kernel in ("decode_tc_kernel", "decode_simt_kernel") if any(kernel in name for name in names)}
+
+    def on_cuda_cores():
+        with sb.force_simt():
+            sb.sb_attn_decode(q, *cache)
+
+    assert ran(lambda: sb.sb_attn_decode(q, *cache)) == {"decode_tc_kernel"}
+    assert ran(on_cuda_cores) == {"decode_simt_kernel"}
+    assert ran(lambda: sb.sb_attn_decode(q, wide[0, ..., :64], wide[1, ..., :64], *cache[2:])) == {"decode_simt_kernel"}
     sb.check_status(cuda_device)
