@@ -205,8 +205,11 @@ __global__ void __launch_bounds__(kBookThreads) extend_kernel(const __grid_const
   int *const shared = book.scan;
   enter_kernel<true>();
   int *list = p.work + kPagesHeader, *const prefix = p.max_seqs <= kShort ? book.other : list + p.num_pages;
+  __shared__ unsigned long long needed;
   int want = 0;
+  unsigned long long asked = 0;
   bool bad = false;
+  if (threadIdx.x == 0) needed = 0;
   for (int base = 0; base < p.max_seqs; base += blockDim.x) {
     const int b = base + threadIdx.x;
     int need = 0;
@@ -216,7 +219,9 @@ __global__ void __launch_bounds__(kBookThreads) extend_kernel(const __grid_const
         bad = true;
         report(p.status, SB_DEV_BAD_SEQ_LEN, b);
       } else {
-        need = min(pages_for(p, len + more) - pages_for(p, len), p.num_pages + 1);
+        need = pages_for(p, len + more) - pages_for(p, len);
+        asked += need;
+        need = min(need, p.num_pages + 1);
       }
     }
     int all;
@@ -228,7 +233,9 @@ __global__ void __launch_bounds__(kBookThreads) extend_kernel(const __grid_const
   if (__syncthreads_or(bad)) return;
   if (want <= kShort) list = book.list;
   if (want > 0 && !list_free(p, want, list, shared)) {
-    if (threadIdx.x == 0) report(p.status, SB_DEV_OUT_OF_PAGES, want);
+    atomicAdd(&needed, asked);
+    __syncthreads();
+    if (threadIdx.x == 0) report(p.status, SB_DEV_OUT_OF_PAGES, (int)min(needed, 0x7fffffffULL));
     return;
   }
   for (int r = threadIdx.x; r < want; r += blockDim.x) {

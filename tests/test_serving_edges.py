@@ -315,6 +315,19 @@ def test_fork_of_many_long_rows_looks_at_every_entry(cuda_device):
     assert cache.seq_lens.tolist() == [278] * 80 and int(cache.page_refs.sum()) == 80 * 70
 
 
+@gpu
+@pytest.mark.parametrize("rows,columns,counts,needed", [(4, 50, [6, 0, 9, 200], 2 + 3 + 50), (3000, 40, [160] * 3000, 120000),
+                                                        (3, 2 ** 20, [2 ** 22] * 3, 3 * 2 ** 20), (4, 50, [0, 0, 17, 12], 5 + 3)])
+def test_extend_says_how_many_pages_it_needs(cuda_device, rows, columns, counts, needed):
+    import stickbreaking_attention_b200 as sb
+    table = torch.full((rows, columns), -1, dtype=torch.int32, device=cuda_device)
+    lens, refs = torch.zeros(rows, dtype=torch.int32, device=cuda_device), torch.zeros(6, dtype=torch.int32, device=cuda_device)
+    sb.kv_extend(table, lens, refs, ints(*counts), 4)
+    with pytest.raises(sb._cabi.SbError, match=f" {needed} needed"):
+        sb.check_status(cuda_device)
+    assert not bool(lens.any()) and not bool(refs.any()) and bool((table == -1).all())
+
+
 # ---- layouts ---------------------------------------------------------------------------------------------------------------
 
 def layouts(device, dtype=BF16):
