@@ -24,10 +24,12 @@
 // instead of standing still at fp32's smallest numbers.
 //
 // P enters the second product as the sum of 16-bit numbers: three in bf16 (24 bits, as many as the weights have) and two in fp16
-// (22 bits).  With two in bf16, 16 bits, the share of output values that are not the nearest of their type to the exact one is
-// 1.9e-3 for 5.2e-4 with three (48 ragged sequences of shared key heads) and 2.6e-3 for 1.7e-3 (64 x 16 heads of their own); the
-// third costs 92.4 us for 89.7, and 153.5 for 152.8.  In fp16 weights are scaled by 2^15 and so held in steps of 2^-39: each is
-// off by up to 2^-40.  Scores, weights and the output's accumulators are 32-bit, the stick 32-bit with what its sums lost.
+// (22 bits).  Up to four query rows leave columns of a product empty, and the parts of the weights take these: one product for
+// one or two rows, two (bf16) or one (fp16) for up to four.  In bf16 two parts, 16 bits, in two products took 154.3 us for 154.9
+// (64 sequences x 16 heads x 512..4096 tokens), 89.6 for 91.3 (48 ragged ones, 4 query heads to a key head), 62.9 for 58.8 (32 of 256 columns);
+// the share of output values that are not the nearest of their type to the exact one was 2.6e-3 for 6.5e-4 (32-bit CUDA cores: 5.7e-4) in
+// the first, 1.9e-3 for 4.2e-4 in the second.  In fp16 weights are scaled by 2^15 and so held in steps of 2^-39: each is off by up to 2^-40.
+// Scores, weights and the output's accumulators are 32-bit, the stick 32-bit with what its sums lost.
 #include "sb_decode.cuh"
 #include "sb_ptx.cuh"
 
@@ -102,10 +104,14 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 // The key of the tile that row g (second false) or g + 8 of a product's operand is.
 __device__ __forceinline__ int key_of(int g, bool second) { return 2 * g + (second != (g >= 4)); }
 
-// The tensor-core engine.  kN: blocks of 8 query rows.
-template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
+// The tensor-core engine.  kN: blocks of 8 query rows.  kSets: where the rows are few (kN 1) they are in the 8 columns of the products
+// kSets times, and each set of columns has a part of the weights of its own in one product; the sets' sums are added up at the end.
+template <typename T, int kD, int kN, int kSets> struct TcEngine : TcShape<kD, kN> {
   using S = TcShape<kD, kN>;
   using S::kHalf;
+  static_assert(kSets == 1 || kN == 1, "");
+  static constexpr int kOfSet = kN * 8 / kSets;                              // rows of a set; a thread's two columns are in the same one
+  static constexpr int kPasses = (kParts<T> + kSets - 1) / kSets;            // products that the parts of the weights take
   uint32_t q[kN][kD / 16][2];
   float acc[kD / 16][kN][4];
   LongSum stick[kN][2];
@@ -113,6 +119,13 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
   bool real[kN][2];
 
   __device__ static __forceinline__ void prefetch_rows(const DecodeParams &p, const Piece &w) { prefetch_q(p, w, 2); }
+
+  // What the sets of columns sum up to, in all of them.  (In the same order in each: the sets of a row stay the same.)
+  __device__ static __forceinline__ float over_sets(float x) {
+#pragma unroll
+    for (int d = kOfSet / 2; d < 4; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+  }
 
   // 16 rows from slot `slot` of one page on; columns behind head_dim are zeros.
   __device__ static __forceinline__ void copy_run(const DecodeParams &p, const Piece &w, int page, int slot, char *to) {
@@ -155,7 +168,7 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      const int r = n * 8 + g;
+      const int r = (n * 8 + g) % kOfSet;
       const char *row = p.q.ptr + 2 * row_offset(p, p.q, w.seq, w.head, w.row0 + min(r, w.rows - 1));
 #pragma unroll
       for (int i = 0; i < kD / 16; ++i)
@@ -166,7 +179,7 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
         }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int query = n * 8 + t * 2 + j;
+        const int query = (n * 8 + t * 2 + j) % kOfSet;
         stick[n][j] = LongSum{1.0f, 0.0f};
         real[n][j] = query < w.rows;
         limit[n][j] = row_limit(p, w.keys, w.row0 + min(query, w.rows - 1));
@@ -178,9 +191,9 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
     }
   }
 
-  // O^T += V^T P^T; `b`: the weights, [row block][rows m, m + 8][part, the largest first].  kSome: only for the queries whose
-  // limits are in [low, high).
-  template <bool kSome> __device__ __forceinline__ void add_values(uint32_t values, const uint32_t (&b)[kN][2][kParts<T>], int low, int high) {
+  // O^T += V^T P^T; `b`: the weights, [row block][rows m, m + 8][product].  kSome: only for the queries whose limits are in
+  // [low, high).
+  template <bool kSome> __device__ __forceinline__ void add_values(uint32_t values, const uint32_t (&b)[kN][2][kPasses], int low, int high) {
     const int lane = threadIdx.x & 31;
     const int r = key_of(lane & 7, lane >> 4), c = (lane >> 3) & 1;
 #pragma unroll
@@ -193,7 +206,7 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] = acc[i][n][j];
 #pragma unroll
-        for (int part = 0; part < kParts<T>; ++part) mma<T>(o, a, b[n][0][part], b[n][1][part]);
+        for (int pass = 0; pass < kPasses; ++pass) mma<T>(o, a, b[n][0][pass], b[n][1][pass]);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (!kSome || (limit[n][j & 1] >= low && limit[n][j & 1] < high)) acc[i][n][j] = o[j];
@@ -255,30 +268,36 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
         a[n][2 + j] = beta[1] * (g < 4 ? whole : whole * kept[0]);
       }
     }
-    // the 16-bit parts of the weights, moved from (key, query) to (query, key)
-    uint32_t b[kN][2][kParts<T>];
+    // the 16-bit parts of the weights, the largest first, part i in set i % kSets of product i / kSets, moved from (key, query) to
+    // (query, key)
+    uint32_t b[kN][2][kPasses];
+    const int set = (lane & 3) * 2 / kOfSet;
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int row = 0; row < 2; ++row)
+      for (int row = 0; row < 2; ++row) {
+        uint32_t own[kPasses] = {};
 #pragma unroll
         for (int part = 0; part < kParts<T>; ++part) {
           const uint32_t rounded = pack<T>(a[n][2 * row], a[n][2 * row + 1]);
           const float2 back = unpack<T>(rounded);
           a[n][2 * row] -= back.x;               // what is left for the parts behind this one, exactly
           a[n][2 * row + 1] -= back.y;
-          b[n][row][part] = transpose8x8(rounded);
+          if (kSets == 1 || set == part % kSets) own[part / kSets] = rounded;
         }
+#pragma unroll
+        for (int pass = 0; pass < kPasses; ++pass) b[n][row][pass] = transpose8x8(own[pass]);
+      }
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       const uint32_t ones[4] = {kOnes<T>, kOnes<T>, kOnes<T>, kOnes<T>};
       float sum[4] = {};                             // [j]: all weights of query 2 t + j
 #pragma unroll
-      for (int part = 0; part < kParts<T>; ++part) mma<T>(sum, ones, b[n][0][part], b[n][1][part]);
+      for (int pass = 0; pass < kPasses; ++pass) mma<T>(sum, ones, b[n][0][pass], b[n][1][pass]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float whole = stick[n][j].sum;
-        if (rest[n][j] > 0.875f && whole > kSmallStick<T>) stick[n][j].add(sum[j] * (-1.0f / kScaleP<T>));
+        const float whole = stick[n][j].sum, taken = over_sets(sum[j]);
+        if (rest[n][j] > 0.875f && whole > kSmallStick<T>) stick[n][j].add(taken * (-1.0f / kScaleP<T>));
         else stick[n][j] = LongSum{whole > 0x1p-100f ? whole * rest[n][j] : __fmul_rz(whole, rest[n][j]), 0.0f};
       }
     }
@@ -316,6 +335,12 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
   __device__ __forceinline__ void finish(const DecodeParams &p, const Piece &w, int slot, bool bad) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int i = 0; i < kD / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][n][j] = over_sets(acc[i][n][j]);
     if (bad) {
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
@@ -354,12 +379,12 @@ template <typename T, int kD, int kN> struct TcEngine : TcShape<kD, kN> {
   }
 };
 
-template <typename T, int kD, int kN>
+template <typename T, int kD, int kN, int kSets>
 __global__ void __launch_bounds__(TcShape<kD, kN>::kWarps * 32, 1) decode_tc_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) char ring[];
   __shared__ ChunkShared<TcShape<kD, kN>::kWarps> shared;
   enter_kernel<true>();
-  decode_chunks<TcEngine<T, kD, kN>>(p, ring, shared);
+  decode_chunks<TcEngine<T, kD, kN, kSets>>(p, ring, shared);
 }
 
 // Joins the pieces of the items that were cut, newest first, 8 rows x 16 columns at a time as a warp's registers held them: a lane has two
@@ -461,18 +486,23 @@ __global__ void __launch_bounds__(kWarps * 32) decode_tc_join_kernel(const __gri
   }
 }
 
-template <typename T, int kD, int kN> cudaError_t launch_one(const DecodeParams &p, cudaStream_t s) {
+template <typename T, int kD, int kN, int kSets = 1> cudaError_t launch_one(const DecodeParams &p, cudaStream_t s) {
   using S = TcShape<kD, kN>;
-  const auto kernel = decode_tc_kernel<T, kD, kN>;
+  const auto kernel = decode_tc_kernel<T, kD, kN, kSets>;
   const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kBytes);
   if (e != cudaSuccess) return e;
   return launch_kernel(kernel, dim3(p.chunks / S::kWarps), S::kWarps * 32, S::kBytes, s, p);
 }
+// Eight rows or fewer: as many sets as there is room for and parts of the weights to put there.
+template <typename T, int kD> cudaError_t launch_few(const DecodeParams &p, cudaStream_t s) {
+  if (kParts<T> > 2 && p.rows <= 2) return launch_one<T, kD, 1, kParts<T> == 2 ? 2 : 4>(p, s);
+  return p.rows <= 4 ? launch_one<T, kD, 1, 2>(p, s) : launch_one<T, kD, 1>(p, s);
+}
 template <typename T> cudaError_t launch_shape(const DecodeParams &p, cudaStream_t s) {
   const int n = p.rows_per_block / 8;
-  if (p.head_dim <= 64) return n == 1 ? launch_one<T, 64, 1>(p, s) : n == 2 ? launch_one<T, 64, 2>(p, s) : launch_one<T, 64, 4>(p, s);
-  if (p.head_dim <= 128) return n == 1 ? launch_one<T, 128, 1>(p, s) : launch_one<T, 128, 2>(p, s);
-  return launch_one<T, 256, 1>(p, s);
+  if (p.head_dim <= 64) return n == 1 ? launch_few<T, 64>(p, s) : n == 2 ? launch_one<T, 64, 2>(p, s) : launch_one<T, 64, 4>(p, s);
+  if (p.head_dim <= 128) return n == 1 ? launch_few<T, 128>(p, s) : launch_one<T, 128, 2>(p, s);
+  return launch_few<T, 256>(p, s);
 }
 
 }  // namespace
