@@ -80,6 +80,28 @@ def test_decode_sticks_that_wear_down_slowly(cuda_device, dtype, bits):
     R.check_decode(got, tuple(t.expand(seqs, *t.shape[1:]) for t in (o, rem, o_err, rem_err)))
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("heads,new", [(2, 2), (2, 3), (4, 2), (2, 4), (6, 1), (8, 1), (10, 1), (4, 3)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_decode_of_one_to_six_query_rows(cuda_device, dtype, heads, new, d):
+    """Rows that share a product's columns in every way there is, cut and whole items, newest keys and values that are no numbers."""
+    import stickbreaking_attention_b200 as sb
+    lens, page = [0, 1, 3, 16, 113, 1500], 16
+    gen = torch.Generator().manual_seed(62)
+    k, v, table, lengths = R.make_cache(gen, lens, 2, page, d, dtype, shift=0.2)
+    q = (torch.randn(len(lens), heads, new, d, generator=gen) + 0.2).to(dtype)
+    want = R.decode(q, k, v, table, lengths)
+    for b, n in enumerate(lens):                    # the newest token of each: no row attends to it
+        if n:
+            at = table[b, (n - 1) // page].long(), slice(None), (n - 1) % page
+            k[at], v[at] = float("nan"), float("inf")
+    with torch.no_grad():
+        got = sb.sb_attn_decode(*(t.to(cuda_device) for t in (q, k, v, table, lengths)))
+    sb.check_status(cuda_device)
+    R.check_decode(got, want)
+
+
 def ints(*x):
     return torch.tensor(x, dtype=torch.int32, device="cuda")
 
