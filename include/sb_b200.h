@@ -348,7 +348,7 @@ SB_EXPORT int sb_kv_fork(const SbPagesParams *p, void *stream);
 SB_EXPORT int sb_kv_free(const SbPagesParams *p, void *stream);
 /* Moves the pages in use to the front of the pool: with N of them, the r-th one at or behind N goes to the r-th free one before
  * N, all layers, and the tables follow.  Pages that have become free keep what they held.  A table entry that names no page, or a
- * free one, is left as it is (SB_DEV_BAD_PAGE, where any page moves). */
+ * free one behind N, is left as it is (SB_DEV_BAD_PAGE, where any page moves). */
 SB_EXPORT int sb_kv_compact(const SbPagesParams *p, void *stream);
 
 /* Which kernels sb_fwd / sb_bwd run for these parameters (an SbKernelPath), or -1 if invalid. */

@@ -256,35 +256,63 @@ __global__ void __launch_bounds__(kBookThreads) extend_kernel(const __grid_const
   }
 }
 
-// A block per entry.  A sequence that is listed more than once is the first entry's.  No count goes below 0: a page that would is
-// taken out of the row, and reported.
-constexpr int kFreeThreads = 128;
+// No count goes below 0: a page whose count would is taken out of the row, and reported.
+constexpr int kFreeThreads = 128, kFreeBlocks = 8;
+__device__ __forceinline__ void free_row(const PagesParams &p, int b, int len, int thread, int threads) {
+  const int pages = pages_for(p, len);
+  int *const row = p.page_table + b * p.table_stride;
+  constexpr int kDeep = 4;
+  for (int i0 = thread; i0 < pages; i0 += kDeep * threads) {
+    int page[kDeep], count[kDeep];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const int i = i0 + k * threads;
+      page[k] = 0;
+      count[k] = i < pages ? 0 : 1;
+      if (i < pages) {
+        page[k] = row[i];
+        row[i] = -1;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k)
+      if (count[k] == 0 && (unsigned)page[k] < (unsigned)p.num_pages) {
+        count[k] = atomicSub(p.refs + page[k], 1);
+        if (count[k] <= 0) atomicAdd(p.refs + page[k], 1);
+      }
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k)
+      if (count[k] <= 0) report(p.status, SB_DEV_BAD_PAGE, b);
+  }
+}
+// A block per entry, or, where the entries are more than kFreeBlocks times the SMs, a warp for every so many.  Each block looks at the
+// whole list first.  Nothing that it refuses changes meanwhile: a length that another block has made 0 was one that can be.
+// A sequence that is listed more than once is the first entry's (blocks), or theirs who takes its length (warps: an atomic in the
+// chain, which a short call feels by 0.5 us).  3000 sequences of 20 pages: 18.4 us, 29.6 with a block per entry; 65535 of 10: 280, 7440.
 __global__ void __launch_bounds__(kFreeThreads) free_kernel(const __grid_constant__ PagesParams p) {
   enter_kernel<true>();
-  // Every block looks at the whole list.  Nothing that it refuses changes meanwhile: a length that another block has made 0
-  // was one that can be.
-  const int b = p.a[blockIdx.x];
-  bool leave = false;
+  const int own = p.a[blockIdx.x];
+  bool leave = false, first = true;
   for (int i = threadIdx.x; i < p.n; i += kFreeThreads) {
     const int s = p.a[i], code = (unsigned)s >= (unsigned)p.max_seqs ? SB_DEV_BAD_SEQUENCE : length_ok(p, p.seq_lens[s]) ? 0 : SB_DEV_BAD_SEQ_LEN;
-    leave |= code != 0 || (s == b && i < (int)blockIdx.x);
+    leave |= code != 0;
+    first &= s != own || i >= (int)blockIdx.x;
     if (code != 0 && blockIdx.x == 0) report(p.status, code, s);
   }
-  if (__syncthreads_or(leave)) return;
-  const int pages = pages_for(p, p.seq_lens[b]);
-  for (int i = threadIdx.x; i < pages; i += kFreeThreads) {
-    int *const entry = p.page_table + b * p.table_stride + i;
-    const int page = *entry;
-    *entry = -1;
-    bool held = (unsigned)page < (unsigned)p.num_pages;
-    if (held && atomicSub(p.refs + page, 1) <= 0) {
-      atomicAdd(p.refs + page, 1);
-      held = false;
-    }
-    if (!held) report(p.status, SB_DEV_BAD_PAGE, b);
+  const bool by_block = p.n == (int)gridDim.x;
+  if (__syncthreads_or(leave || (by_block && !first))) return;
+  if (by_block) {
+    free_row(p, own, p.seq_lens[own], threadIdx.x, kFreeThreads);
+    __syncthreads();
+    if (threadIdx.x == 0) p.seq_lens[own] = 0;
+    return;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) p.seq_lens[b] = 0;
+  constexpr int kWarps = kFreeThreads / 32;
+  const int lane = threadIdx.x & 31;
+  for (int e = blockIdx.x * kWarps + (threadIdx.x >> 5); e < p.n; e += gridDim.x * kWarps) {
+    const int b = p.a[e], len = lane == 0 ? atomicExch(p.seq_lens + b, 0) : 0;
+    free_row(p, b, __shfl_sync(0xffffffffu, len, 0), lane, 32);
+  }
 }
 
 // The first `rows` slots of page `from` to page `to`, the heads of part `part`, one layer's keys or values, by the block.
@@ -330,27 +358,35 @@ __device__ __forceinline__ void copy_page(const PagesParams &p, const CacheRef &
   }
 }
 
-// header of `work`: [0] fork: whether there is something to carry out, [1] compact: pages to move
+// header of `work`: [0] fork: whether there is something to carry out, [1] compact: pages to move, [2] live pages
 // fork: behind the lists, for each pair the source's length and the page that its copied rows get (or -1)
 __device__ __forceinline__ int *fork_plan(const PagesParams &p) { return p.work + kPagesHeader + 2 * p.num_pages + p.max_seqs; }
 
 // Whether the rows of a fork's sources name pages.  Looked at before anything is given out: a destination whose last page could
-// not be filled would hold what that page's last owner left there.  Eight rows by the warp at a time, whose loads are on their
-// way together.  (64 forks of 5 to 27 pages, extended and freed: 28.8 us with eight, 29.1 with four, 32.3 with one.)
+// not be filled would hold what that page's last owner left there.  A warp takes eight rows at a time, whose loads are on their
+// way together, and where rows are few each is cut into 2^shift parts.  (64 forks of 5 to 27 pages, extended and freed: 29.1 us with
+// eight rows, 29.4 with four, 32.6 with one; 4 forks of 8192 pages: 29.7 us, 142 with whole rows.)
 __device__ __forceinline__ bool source_rows_ok(const PagesParams &p) {
   constexpr int kRows = 8;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, at_once = (int)(blockDim.x >> 5) * kRows;
+  const int shift = max(__clz(p.n - 1) - 1 - __clz(at_once), 0), total = p.n << shift;
   bool ok = true;
-  for (int i0 = (threadIdx.x >> 5) * kRows; i0 < p.n; i0 += (blockDim.x >> 5) * kRows) {
-    const bool own = lane < kRows && i0 + lane < p.n;
-    const int s = own ? p.a[i0 + lane] : 0, pages = own ? pages_for(p, p.seq_lens[s]) : 0;
-    const int most = __reduce_max_sync(0xffffffffu, pages);
+  for (int q0 = (threadIdx.x >> 5) * kRows; q0 < total; q0 += at_once) {
+    const int q = q0 + lane;
+    int s = 0, begin = 0, count = 0;
+    if (lane < kRows && q < total) {
+      s = p.a[q >> shift];
+      const int pages = pages_for(p, p.seq_lens[s]), span = (((pages + (1 << shift) - 1) >> shift) + 31) & ~31;
+      begin = (q & ((1 << shift) - 1)) * span;
+      count = min(pages - begin, span);
+    }
+    const int most = __reduce_max_sync(0xffffffffu, count);
     for (int j0 = 0; j0 < most; j0 += 32) {
       int page[kRows];
 #pragma unroll
       for (int k = 0; k < kRows; ++k) {
-        const long long row = __shfl_sync(0xffffffffu, s, k) * p.table_stride;
-        page[k] = j0 + lane < __shfl_sync(0xffffffffu, pages, k) ? p.page_table[row + j0 + lane] : 0;
+        const long long at = __shfl_sync(0xffffffffu, s, k) * p.table_stride + __shfl_sync(0xffffffffu, begin, k) + j0 + lane;
+        page[k] = j0 + lane < __shfl_sync(0xffffffffu, count, k) ? p.page_table[at] : 0;
       }
 #pragma unroll
       for (int k = 0; k < kRows; ++k) {
@@ -450,8 +486,8 @@ __global__ void __launch_bounds__(kCopyThreads) fork_kernel(const __grid_constan
 __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid_constant__ PagesParams p) {
   __shared__ int shared[33];
   enter_kernel<true>();
-  int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;    // (hole, page) pairs, no more than half the pages; new place of each, -1 of a free one
-  int live = 0, mine = 0;
+  int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;    // (hole, page) pairs, no more than half the pages; which pair a page is in
+  int live = 0, mine = 0, negative = -1;
   bool bad = false;
   for (int b = threadIdx.x; b < p.max_seqs; b += blockDim.x)
     if (!length_ok(p, p.seq_lens[b])) {      // which entries of its row are to follow their pages, nothing says
@@ -465,13 +501,11 @@ __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       mine += x[i] > 0;
-      if (x[i] < 0 && first + i < p.num_pages) {      // a page neither free nor in use: there would be fewer holes than pages to move
-        bad = true;
-        report(p.status, SB_DEV_BAD_COUNT, first + i);
-      }
+      if (x[i] < 0 && first + i < p.num_pages) negative = first + i;
     }
   }
-  if (__syncthreads_or(bad)) {
+  if (negative >= 0) report(p.status, SB_DEV_BAD_COUNT, negative);      // neither free nor in use: there would be fewer holes than pages to move
+  if (__syncthreads_or(bad || negative >= 0)) {
     if (threadIdx.x == 0) p.work[1] = 0;
     return;
   }
@@ -491,7 +525,6 @@ __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid
     for (int i = 0; i < kPer; ++i) {
       if (first + i < live && x[i] == 0) pairs[2 * rank_h++] = first + i;
       if (first + i >= live && x[i] > 0) pairs[2 * rank_m++ + 1] = first + i;
-      if (first + i < p.num_pages) place[first + i] = x[i] > 0 ? first + i : -1;
     }
     holes += all_h;
     moved += all_m;
@@ -499,18 +532,21 @@ __global__ void __launch_bounds__(kBookThreads) compact_plan_kernel(const __grid
   __syncthreads();
   for (int r = threadIdx.x; r < moved; r += blockDim.x) {
     const int to = pairs[2 * r], from = pairs[2 * r + 1];
-    place[from] = to;
+    place[from] = r;
     p.refs[to] = p.refs[from];
     p.refs[from] = 0;
   }
-  if (threadIdx.x == 0) p.work[1] = moved;
+  if (threadIdx.x == 0) {
+    p.work[1] = moved;
+    p.work[2] = live;
+  }
 }
 
 // Blocks below copy_blocks copy the moved pages, a share of a (page, layer, keys or values) at a time; the others rewrite the tables.
 template <typename V>
 __global__ void __launch_bounds__(kCopyThreads) compact_kernel(const __grid_constant__ PagesParams p, int copy_blocks) {
   enter_kernel<true>();
-  const int moved = p.work[1];
+  const int moved = p.work[1], live = p.work[2];
   const int *pairs = p.work + kPagesHeader, *place = pairs + p.num_pages;
   if ((int)blockIdx.x < copy_blocks) {
     const int per_pair = p.layers * 2 * p.parts;
@@ -526,9 +562,12 @@ __global__ void __launch_bounds__(kCopyThreads) compact_kernel(const __grid_cons
     const int pages = pages_for(p, p.seq_lens[b]);
     int *row = p.page_table + b * p.table_stride;
     for (int i = threadIdx.x; i < pages; i += kCopyThreads) {
-      const int page = row[i], to = (unsigned)page < (unsigned)p.num_pages ? place[page] : -1;
-      if (to < 0) report(p.status, SB_DEV_BAD_PAGE, b);      // no page, or a free one: stays as it is
-      else if (to != page) row[i] = to;
+      const int page = row[i];
+      if ((unsigned)page < (unsigned)live) continue;
+      // no page, or a free one, in whose place there is anything: stays as it is
+      const int pair = (unsigned)page < (unsigned)p.num_pages ? place[page] : -1;
+      if ((unsigned)pair < (unsigned)moved && pairs[2 * pair + 1] == page) row[i] = pairs[2 * pair];
+      else report(p.status, SB_DEV_BAD_PAGE, b);
     }
   }
 }
@@ -567,7 +606,12 @@ cudaError_t launch_append(const AppendParams &p, cudaStream_t s) {
 
 cudaError_t launch_extend(const PagesParams &p, cudaStream_t s) { return launch_kernel(extend_kernel, dim3(1), book_threads(p), 0, s, p); }
 
-cudaError_t launch_free(const PagesParams &p, cudaStream_t s) { return launch_kernel(free_kernel, dim3(p.n), kFreeThreads, 0, s, p); }
+cudaError_t launch_free(const PagesParams &p, cudaStream_t s) {
+  int sms = 0;
+  const cudaError_t e = sm_count(&sms);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(free_kernel, dim3(std::min(p.n, kFreeBlocks * sms)), kFreeThreads, 0, s, p);
+}
 
 // A page's heads are shared out so that there are `blocks` pieces of work, or each is one head's.
 static void set_parts(PagesParams &p, long long jobs, long long blocks) {

@@ -232,7 +232,7 @@ def test_compact_of_large_pools_refuses_negative_counts(cuda_device):
 
 
 @gpu
-@pytest.mark.parametrize("page", [-1, 6, 2 ** 31 - 1, 5, 1])          # 5, 1: pages of the cache, but free ones
+@pytest.mark.parametrize("page", [-1, 6, 2 ** 31 - 1, 5])          # 5: a page of the cache, but a free one
 def test_compact_leaves_entries_without_a_place_alone(cuda_device, page):
     import stickbreaking_attention_b200 as sb
     cache = small_cache(sb, cuda_device)
@@ -335,6 +335,41 @@ def test_fork_of_many_long_rows_looks_at_every_entry(cuda_device):
     cache.fork(src, dst)
     sb.check_status(cuda_device)
     assert cache.seq_lens.tolist() == [278] * 80 and int(cache.page_refs.sum()) == 80 * 70
+
+
+@gpu
+@pytest.mark.parametrize("n,pages", [(3000, 7), (1300, 150), (65535, 2)])
+def test_free_of_thousands_of_sequences(cuda_device, n, pages):
+    """More entries than blocks run at a time, many of them twice; then with one that is refused, and with pages counted too few."""
+    import stickbreaking_attention_b200 as sb
+    gen = torch.Generator().manual_seed(63)
+    max_seqs = n - n // 4
+    total = max_seqs * pages
+    table = torch.randperm(total, generator=gen).int().view(max_seqs, pages).to(cuda_device)
+    lens = torch.randint(0, 4 * pages + 1, (max_seqs,), generator=gen, dtype=torch.int32).to(cuda_device)
+    held = torch.arange(pages, device=cuda_device)[None] < ((lens + 3) // 4)[:, None]
+    refs = torch.zeros(total, dtype=torch.int32, device=cuda_device)
+    refs[table[held].long()] = 2                    # somebody else holds them as well
+    seqs = torch.cat((torch.randperm(max_seqs, generator=gen), torch.randint(0, max_seqs, (n - max_seqs,), generator=gen)))
+    seqs = seqs[torch.randperm(n, generator=gen)].int().to(cuda_device)
+    before = [t.clone() for t in (table, lens, refs)]
+    bad = seqs.clone()
+    bad[n // 2] = max_seqs
+    sb.kv_free(table, lens, refs, bad, 4)
+    with pytest.raises(sb._cabi.SbError, match="listed"):
+        sb.check_status(cuda_device)
+    for t, old in zip((table, lens, refs), before):
+        assert torch.equal(t, old)
+    sb.kv_free(table, lens, refs, seqs, 4)
+    sb.check_status(cuda_device)
+    assert not bool(lens.any()) and torch.equal(refs, before[2] // 2) and torch.equal(table, torch.where(held, -1, before[0]))
+    table.copy_(before[0]), lens.copy_(before[1])
+    short = table[held].long()[::97]
+    refs[short] = 0
+    sb.kv_free(table, lens, refs, seqs, 4)
+    with pytest.raises(sb._cabi.SbError, match="page"):
+        sb.check_status(cuda_device)
+    assert not bool(lens.any()) and not bool(refs.any()) and torch.equal(table, torch.where(held, -1, before[0]))
 
 
 @gpu
