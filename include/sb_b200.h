@@ -314,8 +314,9 @@ SB_EXPORT int sb_kv_append(const SbAppendParams *p, void *stream);
 
 /* The keeping of the pages.  `page_refs[page]` is the number of sequences that hold a page, 0 for a free one; page tables and
  * lengths as above, an empty sequence having length 0.  Pages are given out lowest first, in the order of sequences (or listed
- * pairs) and positions.  A call that cannot do all it is asked to changes nothing and sets the status word.  Only the last
- * page of a sequence can be partly filled, and no two sequences share one that is. */
+ * pairs) and positions.  A call that cannot do all it is asked to changes nothing and sets the status word, but for table
+ * entries that sb_kv_free and sb_kv_compact pass over (below).  Only the last page of a sequence can be partly filled, and no two
+ * sequences share one that is. */
 typedef struct SbPagesParams {
   int32_t struct_bytes;   /* = sizeof(SbPagesParams)                                         */
   int32_t max_seqs;       /* rows of page_table, entries of seq_lens                         */

@@ -14,7 +14,9 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool ta
 
 // kCols: columns a lane holds (32 kCols >= head_dim); kRows: query rows.  As many warps as registers and shared memory allow: a
 // tile is a long chain (16 dots, a scan, 16 sums), other warps' tiles fill it, and their copies are in flight as well.
-// (fp32, 8 heads x 128 columns, 20 sequences of 157 to 8150 tokens: 122, 92, 73 us with 4, 6, 12 warps of 3, 2, 1 stages.)
+// (fp32, 8 heads x 128 columns, 20 sequences of 157 to 8150 tokens: 122, 92, 73 us with 4, 6, 12 warps of 3, 2, 1 stages; 64 columns 76, 60
+// with 8, 12 warps of 3, 2; 128 columns and 4 rows 124, 107 with 8, 12 of 1, although 12 warps leave 168 registers, of which those rows need
+// 8 to 15 more; 256 columns, 157 to 4000 tokens, 132, 98 with 4, 6 of 1.)
 template <int kCols, int kRows> struct SimtShape {
   static constexpr int kWidth = 32 * kCols;                              // floats of a row in shared memory
   static constexpr int kWarps = kCols <= 2 ? 12 : kCols <= 4 ? (kRows <= 4 ? 12 : 8) : 6;
@@ -321,7 +323,7 @@ template <typename T, int kVec> cudaError_t launch_cols(const DecodeParams &p, c
 
 }  // namespace
 
-// (More rows of a head_dim over 128 than four do not fit into a thread's registers.)
+// (Four rows of a head_dim over 128 need 26 registers more than a thread has; twice as many rows would need twice the accumulators.)
 int decode_simt_rows(int rows, int head_dim) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 || head_dim > 128 ? 4 : 8; }
 int decode_simt_warps(int rows, int head_dim) {
   if (head_dim <= 64) return SimtShape<2, 1>::kWarps;
@@ -341,8 +343,10 @@ cudaError_t launch_decode_simt(const DecodeParams &p, int dtype, cudaStream_t s)
 }
 
 // The columns behind head_dim that a part reads (up to 127) lie in the next row, or behind the last one in the padding that the
-// workspace has there.  By the pieces that an item is cut into on the average, 1, 4, 8 or 32 warps
-// share a part.
+// workspace has there.  1, 4, 8 or 32 warps share a part, by the chunks that there are for an item.  (The whole call in us with 1, 4, 8, 32,
+// fp32, 64 columns.  1.7 chunks per item, 64 sequences x 16 heads, 1024 tokens: 148.7, 148.5, 149.9, 164; 3.8, 29 x 16: 74.9, 74.5, 73.5, 81;
+// 4.4, 25 x 16: 67.6, 66.6, 66.4, 72; 15, 15 x 8: 31, 29, 28.8, 29.2; 17, 13 x 8: 26.4, 24, 24.1, 24.4; 222, 1 x 8, 16384 tokens: 74, 39, 33.9, 29.9;
+// 296, 1 x 6: 79, 32, 28.5, 24.7.)
 cudaError_t launch_decode_join(const DecodeParams &p, int dtype, cudaStream_t s) {
   const long long items = (long long)p.batch * p.items_per_seq;
   const int notes = (int)(p.by_item ? items : p.chunks);

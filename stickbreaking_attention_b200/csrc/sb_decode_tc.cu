@@ -1,8 +1,9 @@
 // Attention of new tokens over a paged key-value cache, tensor-core kernel: bf16 and fp16, rows of whole 16-byte chunks.
 //
-// What bounds it: every key and value is read once from HBM and takes part in 4 * rows operations per element, `rows` (query
-// heads per key head times new tokens) being 1 to 16 here: 1 to 16 operations per byte, where the GPU's ratio is 250.  So the
-// kernel is built around the copies: each warp has a ring of 16-key stages of its own, filled with cp.async, and no barrier with
+// What bounds it: every key and value is read once from HBM and takes part in 4 * rows operations per element.  With `rows` (query
+// heads per key head times new tokens) of 1 to 16 that is 1 to 16 operations per byte, where the GPU's ratio is 250.  (More rows
+// are taken 16, or 8 or 32, at a time, for each of which all keys are read again, through L2: 16 / 4 heads, 8192 tokens and 64, 256, 1024
+// new ones take 68, 200, 724 us, 63 to 95 TFLOP/s.)  So the kernel is built around the copies: each warp has a ring of 16-key stages of its own, filled with cp.async, and no barrier with
 // other warps; 192 KiB of stages per SM keep more bytes in flight than the latency of HBM needs (some 50 KiB).  (TMA, boxes of 64
 // columns x 16 rows issued by one lane, took the same time to within 2 %, its longer latency weighing as much as the instructions that it saves.)
 //
@@ -42,9 +43,11 @@ using ptx::rcp;
 using ptx::smem_u32;
 
 // kD: head_dim rounded up to 64, 128, 256; kN: blocks of 8 query rows.  As many warps as their registers allow: a tile is a
-// chain of some 700 cycles (scores, scan over keys, weights, values), and other warps' tiles are what fills them.  (128 columns, 8
-// rows: 64 sequences x 16 heads x 512..4096 tokens 161, 155, 150 us with 8, 12, 16 warps, 48 ragged sequences of shared key heads,
-// half of them local, 120, 89, 93; 16 warps spill.)
+// chain of some 700 cycles (scores, scan over keys, weights, values), and other warps' tiles are what fills them.  Times in us with
+// 8, 10, 12, 16 warps.  128 columns, 8 rows: 64 sequences x 16 heads x 512..4096 tokens 153, 153, 155, 148; 48 ragged sequences of
+// shared key heads, half of them local, 119, 114, 91, 94; one of 131072 tokens 56, 57, 57, 59.  64 columns, 8 rows: 64 x 16 x 512..4096 117, 105, 83, 84;
+// 16 rows: 24 sequences with 4 new tokens 29.5, 29.9, 28.5, 32.6.  With 12 warps a thread has 168 registers, which 64 columns and 16 rows
+// overrun by 4 (fp16) or 7 (bf16), with 16 it has 128, which these and 128 columns overrun by 4 to 26.
 template <int kD, int kN> struct TcShape {
   static constexpr int kChunks = kD / 8;                            // 16-byte chunks of a row
   static constexpr int kHalf = kTileKeys * kD * 2;                  // bytes of a stage's keys (or values)
@@ -523,8 +526,11 @@ cudaError_t launch_decode_tc(const DecodeParams &p, int dtype, cudaStream_t s) {
   return dtype == SB_DTYPE_BF16 ? launch_shape<__nv_bfloat16>(p, s) : launch_shape<__half>(p, s);
 }
 
-// By the pieces that an item is cut into on the average: 1, 4, 8 or 32 warps share a part.  (64 sequences x 16 heads, 1.7 pieces: 19 us
-// after the main kernel with 4 warps to a part, 32768 of them, and 6 with one.)
+// 1, 4, 8 or 32 warps share a part, by the chunks that there are for an item, which is about how many pieces it has where it is long
+// enough.  The whole call in us with 1, 4, 8, 32, bf16, 128 columns.  1.7 chunks per item (64 sequences x 16 heads): 155, 166, 184, 307;
+// 3.8 (29 x 16, 4096 tokens): 162, 167, 177, 240; 4.4 (25 x 16): 141, 145, 154, 208; 9 (12 x 16): 76.6, 76.3, 80, 108; 15 (15 x 8, 8192 tokens):
+// 92, 90, 93, 112; 17 (13 x 8): 84, 81, 83, 100; 37 (12 x 4): 52, 46, 45, 53; 111 (1 x 16, 16384 tokens): 55, 39, 34, 35; 222 (1 x 8,
+// 32768): 79, 44, 37.5, 34.8; 296 (1 x 6): 94, 45, 35, 31; 444 (1 x 4, 131072): 150, 79, 63, 57.
 cudaError_t launch_decode_tc_join(const DecodeParams &p, int dtype, cudaStream_t s) {
   const long long items = (long long)p.batch * p.items_per_seq;
   const int notes = (int)(p.by_item ? items : p.chunks), jobs = p.rows_per_block / 8 * (p.part_cols / 16);

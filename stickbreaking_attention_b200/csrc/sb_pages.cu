@@ -2,8 +2,9 @@
 // sequences, compaction) with the tables on the device, so that a serving step needs no host synchronisation and can be captured.
 //
 // Which page a sequence gets is a rule, not a race: the lowest free pages (count 0), in the order of sequences and positions.
-// An operator that cannot do all it is asked to (too few pages, an index that is none) changes nothing and says so in the
-// status word.
+// An operator that cannot do all it is asked to (too few pages, an index that is none, a length that cannot be) changes nothing and
+// says so in the status word.  Entries of the table that name no page, or a free one, are found on the way by freeing and
+// compaction: these are passed over, and reported.
 #include "sb_pages.cuh"
 
 #include <algorithm>
@@ -119,8 +120,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // ---- the keeping of the pages ----------------------------------------------------------------------------------------------
 // One block decides what happens (which pages go where), many carry it out.  The deciding block reads the counts of all pages,
 // 16 per thread at a time.  What it takes for a small pool is a chain of trips to memory and barriers, so its lists are in shared
-// memory where they are short, and it has 256 threads where those do (a fork of 4 sequences in 160 pages: 4.0 us, 7.6 with
-// 1024 and lists in the workspace).
+// memory where they are short, and it has 256 threads where those do (a fork of 4 sequences in 160 pages took 4.0 us, 7.6 with
+// 1024 and lists in the workspace; 5.1 with the look at the sources' rows).
 constexpr int kBookThreads = 1024, kFewThreads = 256, kPer = 16, kShort = 2048;
 struct Book {
   int scan[33];

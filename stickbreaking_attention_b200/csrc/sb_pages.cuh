@@ -5,7 +5,7 @@
 
 namespace sb {
 
-// Keys or values of a cache: (layers, pages, heads, slots, head_dim), in units of `vec` bytes (16, or one element).
+// Keys or values of a cache: (layers, pages, heads, slots, head_dim); strides in elements (append) or bytes (fork, compact).
 struct CacheRef {
   char *ptr;
   long long sl, sp, sh, st;
@@ -53,7 +53,7 @@ struct PagesParams {
   int layers, heads, row_bytes, vec;
   int per_row, parts, part_heads;  // copies of a row; a page's heads are copied by `parts` blocks, part_heads each
   FastDiv by_row, by_parts;
-  int *work;                       // see work_ints
+  int *work;                       // see pages_work_ints
   int *status;
 };
 

@@ -3,7 +3,8 @@
 Everything a step needs stays on the device: page tables, lengths and the count of sequences that hold each page are int32
 tensors which the operators read and write in place.  No call synchronises, all can be captured into a graph, and which page a
 sequence gets is a rule (the lowest free ones, in the order of sequences and positions), so that runs repeat.  A call that
-cannot do all it is asked to (too few pages, an index that is no sequence) changes nothing; ``check_status()`` raises.
+cannot do all it is asked to (too few pages, an index that is no sequence, a length that cannot be) changes nothing;
+``check_status()`` raises.
 
 ``PagedKVCache`` holds the tensors of a cache; the functions work on any tensors laid out like them.  The reference has no cache.
 """
@@ -44,13 +45,15 @@ def kv_fork(k_cache, v_cache, page_table, seq_lens, page_refs, src, dst):
 
 def kv_free(page_table, seq_lens, page_refs, seqs, page_size):
     """The listed sequences (int32 tensor) give their pages back and are empty.  A page goes free when no sequence holds it.
-    Empty sequences, and the same one twice, are allowed."""
+    Empty sequences, and the same one twice, are allowed.  An entry that names no page, or a free one, goes out of its row, counts
+    nothing down, and is an error at ``check_status()``."""
     _sb_torch.kv_free(page_table, seq_lens, page_refs, seqs, page_size)
 
 
 def kv_compact(k_cache, v_cache, page_table, seq_lens, page_refs):
     """Moves the pages in use to the front of the cache: with N in use, the r-th of those at or behind N goes to the r-th free
-    one before N, in all layers, and the tables follow."""
+    one before N, in all layers, and the tables follow.  With a negative count nothing is changed; an entry that names no page, or a
+    free one behind N, is left as it is, an error at ``check_status()``."""
     _sb_torch.kv_compact(k_cache, v_cache, page_table, seq_lens, page_refs)
 
 
